@@ -1,5 +1,7 @@
 """B200-native (sm_100a) FP32 BLAS-kernel library: row-major SGEMM (FFMA and 3xTF32 paths),
-ABFT fault-tolerant SGEMM, SAXPY and SDOT behind the reference project's launcher signatures.
+ABFT fault-tolerant SGEMM, SAXPY and SDOT behind the reference project's launcher signatures, and
+the operators of a layer around those products: layer norm with its gradients, and matrix-vector
+products with 4-bit weights.
 
 The arithmetic lives in ``libb2blas.so`` (hand-written CUDA, C ABI in ``include/b2blas.h``);
 this package is the host-side mirror of the reference interface and uses PyTorch only for
@@ -12,9 +14,10 @@ def __getattr__(name):
     # Operators are resolved lazily so that importing the package (and building the library)
     # works on a machine without a GPU; using an operator without the built library raises.
     import importlib
-    if name in ("blas", "build", "dist", "gen_ft_sgemm", "_lib"):
+    if name in ("blas", "build", "dist", "gen_ft_sgemm", "layer", "_lib"):
         return importlib.import_module(f"{__name__}.{name}")
-    blas = importlib.import_module(f"{__name__}.blas")
-    if hasattr(blas, name):
-        return getattr(blas, name)
+    for module in ("blas", "layer"):
+        m = importlib.import_module(f"{__name__}.{module}")
+        if hasattr(m, name):
+            return globals().setdefault(name, getattr(m, name))
     raise AttributeError(name)

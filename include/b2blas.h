@@ -206,6 +206,71 @@ int b2_sdot_fused(b2_handle h, int64_t n, const float *x, const float *y, float 
  *    (different streams, no dependency) race with each other; serialise them. */
 int b2_sdot_static(int64_t n, const float *x, const float *y, float *result_dev, void *stream);
 
+/* ---- layer norm ------------------------------------------------------------------------------ */
+
+/* Element types of the operators from here to the SGEMM on host arrays.  Whatever the type, every sum, mean, variance
+ * and scale is held in FP32 and rounded to the type once, when it is stored. */
+enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };
+
+/* y = (x - mean) * rstd * gamma + beta for each of `rows` rows of `cols` elements, with
+ * mean = sum(x) / cols and rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps).
+ * x, y: type `type`, rows ldx / ldy >= cols elements apart.  gamma, beta: `cols` elements of type `param_type` (B2_F32 or
+ * `type`); NULL gamma means 1, NULL beta means 0.  mean, rstd: `rows` floats for the backward pass, or NULL.
+ * eps >= 0.  rows = 0 is a no-op; cols must be at least 1.  y may be x itself (ldy = ldx); any other overlap of y with x is
+ * refused.  A row that holds an infinity or a NaN gives NaN in its own outputs and nowhere else. */
+int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, const void *x, int64_t ldx, int param_type,
+                 const void *gamma, const void *beta, void *y, int64_t ldy, float *mean, float *rstd, void *stream);
+
+/* The gradients of the above from dy = dL/dy and the forward pass's mean and rstd: with xhat = (x - mean) * rstd and
+ * u = dy * gamma,
+ *   dx = rstd * (u - sum(u) / cols - xhat * sum(u * xhat) / cols)   (type `type`, rows lddx apart),
+ *   dgamma = sum over rows of dy * xhat,  dbeta = sum over rows of dy   (`cols` elements of `param_type`).
+ * dx may be NULL, and dgamma and dbeta may each be NULL: what is NULL is not computed.  gamma = NULL means 1 (dgamma may
+ * be asked for all the same).  dx may be dy itself (lddx = lddy); any other overlap of dx with dy or x is refused.
+ * rows = 0 writes zeros to dgamma and dbeta.
+ * The sums over rows go through `workspace` (16-byte aligned, b2_layernorm_backward_workspace_bytes(rows, cols) bytes; may
+ * be NULL when that is 0 or neither dgamma nor dbeta is asked for) in a fixed order: results repeat bit for bit.
+ * Nothing of the handle's own scratch is used, so calls on several streams need several workspaces but not several
+ * handles, and two captured graphs may replay at once when each was captured with a workspace of its own. */
+size_t b2_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, const void *dy, int64_t lddy, const void *x,
+                          int64_t ldx, int param_type, const void *gamma, const float *mean, const float *rstd, void *dx,
+                          int64_t lddx, void *dgamma, void *dbeta, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- 4-bit weights with group scales ------------------------------------------------------------ */
+
+/* An N x K matrix W (row n: the weights of output n) is held as
+ *   codes   N rows of (K + 1) / 2 bytes, rows ldq bytes apart: element k is the low (k even) or high (k odd) half of byte k / 2
+ *           (K odd: the last high half is written 0 and ignored);
+ *   scales  N x G of type `scale_type`, G = ceil(K / group), packed row-major;
+ *   zeros   N x G bytes 0..15, packed row-major, or NULL for a zero point of 8 everywhere;
+ *   W[n][k] = (code - zero[n][k / group]) * scale[n][k / group].
+ * group is 32, 64, 128 or 256; the last group of a row may be shorter.  Types: type and scale_type are each any of B2_F32,
+ * B2_BF16, B2_F16.  Rows of codes that start on 16-byte boundaries (ldq a multiple of 16) are read fastest.  None of these
+ * calls uses the handle's scratch: they may run on any number of streams at once. */
+
+/* Quantises W (N x K, rows ldw elements apart).  Without zeros: scale = absmax / 7 over the group, codes 1..15 around 8.
+ * With zeros: lo = min(0, smallest), hi = max(0, largest), scale = (hi - lo) / 15, zero = -lo / scale to the nearest integer.
+ * The scale is computed in FP32 and rounded to scale_type (a finite scale beyond the type's range becomes its largest value);
+ * each code is the integer nearest to w / scale (ties to even), shifted by the zero point and clamped, by the rounded scale
+ * and without an error of its own.  A group whose scale is 0 gets codes and zero point 8; a group that holds an infinity or a
+ * NaN gets scale NaN and codes and zero point 8, so that it shows in every result. */
+int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const void *W, int64_t ldw, uint8_t *codes,
+                   int64_t ldq, int scale_type, void *scales, uint8_t *zeros, void *stream);
+
+/* Expands codes to W of type `type`: N x K with rows ldw elements apart, or, with transpose != 0, K x N (element (k, n) at
+ * k * ldw + n), which is the right operand B of b2_sgemm for C = X * W^T; untransposed it is B for dX = dC * W. */
+int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t *codes, int64_t ldq, int scale_type,
+                     const void *scales, const uint8_t *zeros, int type, void *W, int64_t ldw, int transpose, void *stream);
+
+/* y = alpha * x * W^T + beta * y for M = 0..64 rows of x (M x K, ldx) and y (M x N, ldy), both of type `type`: the product of
+ * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
+ * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm.  y must not overlap x.
+ * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit. */
+int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
+                 const uint8_t *codes, int64_t ldq, int scale_type, const void *scales, const uint8_t *zeros, float beta,
+                 void *y, int64_t ldy, void *stream);
+
 /* ---- SGEMM on host arrays --------------------------------------------------------------- */
 
 /* The reference drivers hold their matrices on the host and move them with blocking cudaMemcpy calls around the
