@@ -123,72 +123,61 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
 }
 
 // ---- matrix-vector product -----------------------------------------------------------------------
-// y = alpha * x * W^T + beta * y.  The codes are read once and decide the time, so everything else is arranged around
-// streaming them; the arithmetic runs on mma.sync m16n8k16 (16 weight rows x 8 columns of x), which has room for 8 columns at
-// the price of one.  (A tcgen05 tile would want 128 rows and operands rewritten to shared memory in 16 bits first; at
-// 0.5 byte per weight the kernel is bound by reading and unpacking, not by the tensor cores.)
+// y = alpha * x * W^T + beta * y.  The codes are read once and should decide the time; what stands in the way is unpacking
+// them, so the arithmetic is arranged to need five instructions for eight codes.  It runs on mma.sync m16n8k16 (16 weight rows x
+// 8 columns of x), which has room for 8 columns at the price of one; a tcgen05 tile would want its operands written back to
+// shared memory in 16 bits first.
 //
-//   W[n][k] = (c - z) * s, so per group  sum_k W x = s * sum_k (c - z) x:
-// the integers (c - z) are exact in both 16-bit types, their products with x are exact in the FP32 accumulator, and the
-// scale, in FP32, multiplies a group's sum.  Unpacking: a code or-ed into the low mantissa bits of 8.0 (bf16) or 64.0 (f16)
-// reads 8 + c/16 or 64 + c/16; subtracting the same number with z leaves (c - z)/16 exactly.  (The 1/16 keeps sums of x near
-// the end of its range finite; it is undone on the final sum.)  Two codes four apart in a word come out of one mask, so the
-// elements of x are stored paired (0,4) (1,5) (2,6) (3,7).
-// FP32 x is cut into three bf16 terms of 8 bits each (by truncation: exact, and no overflow) that take a column each.
+// Per group,  sum_k W x = s * (sum_k c x - z * sum_k x).  A code c in the lowest bits of a 16-bit half IS the FP16 number
+// c * 2^-24 (a subnormal; the tensor cores take those exactly), four bits higher it is 16 c * 2^-24, so a mask alone makes an
+// operand: words w and w >> 8 under 0x000f000f and 0x00f000f0 give the pairs of codes (0,4) (1,5) (2,6) (3,7), the odd pairs 16
+// times too large.  x takes part as FP16 too: a small kernel in front (w4_x_kernel) scales each row by a power of two that brings
+// its largest element to [2^14, 2^15), divides the odd elements by 16, and pairs them alike.  The scaled row is exact for every
+// element above 2^-28 of the largest (bf16 and FP16 in one term, FP32 in three terms of 11 bits, a column of the tile each), and
+// what lies below is off by 2^-39 of the largest at most: nothing beside the FP32 sums.  All products are exact in FP32; group
+// sums, scales and zero points are FP32.  The same kernel sums x over each group.
+// An infinity or NaN in x would make z * sum_k x meaningless: such elements count as 0 above and are added, with their exact
+// weights, by the thread that writes the output (w4 rows flagged so are slow).
 //
-// A CTA streams tiles of 128 rows x 256 k (16 KB of codes) through a ring of shared-memory stages.  Four producer warps fill
-// it: one thread issues the TMA loads of the codes (128-byte swizzle: the 16-byte unit u of row r lies at u ^ (r & 7), so that
-// the words that a warp reads lie in 32 banks), the others fetch scales and zero points, eight groups of each row at a time.  Eight consumer warps, 4 (rows) x 2
-// (k), multiply 32 rows x 128 k each.  The k range is cut over the CTAs of a cluster, each of which keeps its part of x, already
-// cut and paired, in shared memory while it walks over row blocks; the sums of a row block meet over distributed shared memory
-// in the order of the ranks: no atomics, no workspace.
+// A CTA streams tiles of 128 rows x 256 k (16 KB of codes and x of those k) through a ring of shared-memory stages.  Four
+// producer warps fill it: one thread issues the TMA loads (codes with the 128-byte swizzle: the 16-byte unit u of row r lies at
+// u ^ (r & 7), so that the words that a warp reads lie in 32 banks), the others fetch scales and zero points, eight groups of
+// each row at a time.  Eight consumer warps, 4 (rows) x 2 (k), multiply 32 rows x 128 k each.  Where there are fewer row blocks
+// than CTAs, the k range is cut over the CTAs of a cluster, whose sums meet over distributed shared memory in the order of the
+// ranks: no atomics.
 constexpr int kMvConsumers = 256, kMvProducers = 128, kMvThreads = kMvConsumers + kMvProducers;
 constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2, kMvCodeBytes = kMvRows * kMvRowBytes;
 constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns of a warp's store in 32 banks
 constexpr int kMvWindow = 1024;             // scales and zero points held together: 8 groups of each row, the group / 32 chunks
 constexpr int kMvWindows = 2;               // they span
 constexpr int kMvMaxStages = 8, kMvBarrierBytes = 256 + 1024;   // barriers, and room to align
+constexpr int kMvXThreads = 512;
 
-template <class T>
-struct MvType;   // the 16-bit type of the tensor-core operands, and how many columns a row of x takes
-template <>
-struct MvType<float> {
-  using half_t = __nv_bfloat16;
-  static constexpr int kParts = 3;
-};
-template <>
-struct MvType<__nv_bfloat16> {
-  using half_t = __nv_bfloat16;
-  static constexpr int kParts = 1;
-};
-template <>
-struct MvType<__half> {
-  using half_t = __half;
-  static constexpr int kParts = 1;
-};
-
-template <class T, int NB>
+template <int NB>
 struct MvTile {
-  static constexpr int kParts = MvType<T>::kParts;
-  static constexpr bool kStream = kParts == 1;                      // 16-bit x comes through the ring as it lies in memory
-  static constexpr int kM = 8 * NB / kParts;                        // rows of x per item
-  static constexpr int kXBytes = kMvChunk * 8 * NB * 2;             // x of one chunk
-  static constexpr int kStage = kMvCodeBytes + (kStream ? kXBytes : 0);
+  static constexpr int kXBytes = NB * (kMvChunk * 8 * 2 + 256);     // x of one chunk: fragments, then sums [part of a group][8 NB]
+  static constexpr int kStage = (kMvCodeBytes + kXBytes + 1023) / 1024 * 1024;
   static constexpr int kSumBytes = 2 * 8 * NB * kMvPitch * 4;
   static constexpr int kCtasPerSm = NB <= 2 ? 2 : 1;
   static constexpr int kSmem = kCtasPerSm == 2 ? 115712 : 232448;   // what a CTA may have
-  static constexpr int kXLargest = kStream ? 0 : kCtasPerSm == 2 ? 32768 : 65536;
 };
+
+// Columns that a row of x takes, blocks of 8 columns per item for M rows, rows per item.
+static int mv_parts(int type) { return type == B2_F32 ? 3 : 1; }
+static int mv_blocks(int64_t M, int type) { return M * mv_parts(type) <= 8 ? 1 : M * mv_parts(type) <= 16 ? 2 : 4; }
+static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
 
 struct MvArgs {
   int64_t N, K, ldx, ldq, ldy, groups;
-  int M, group_shift, scale_type, xvec;
-  int stages, items, row_blocks, chunks_per_cta, panel_chunks;   // a panel: the chunks whose x is held at a time
+  int M, rows_per_item, parts, type, group_shift, scale_type;
+  int stages, items, row_blocks, chunks, chunks_per_cta;
   float alpha, beta;
   const void *x;
   const uint8_t *codes, *zeros;
   const void *scales;
   void *y;
+  const unsigned char *image;      // [item's rows][chunk][kXBytes]
+  const int2 *row_info;            // of each row of x: the power of two it was scaled by, and whether it holds an infinity or NaN
   int *status;
   unsigned int seq;
 };
@@ -222,110 +211,141 @@ __device__ __forceinline__ uint4 mv_load_any(const uint8_t *row, int64_t at, int
   return out.v;
 }
 
-// 16 bits of x in pairs (0,4) (1,5) (2,6) (3,7) from 8 in order.
-__device__ __forceinline__ uint4 mv_pair(uint4 h) {
-  return make_uint4(__byte_perm(h.x, h.z, 0x5410), __byte_perm(h.x, h.z, 0x7632), __byte_perm(h.y, h.w, 0x5410),
-                    __byte_perm(h.y, h.w, 0x7632));
-}
-
-// 8 elements of one row of x (k, k + 8) as they lie, zero behind K.
+// x[k .. k + 8) of a row in FP32, zero behind K.
 template <class T>
-struct MvUnit {
-  uint32_t w[sizeof(T) * 2];
-  __device__ __forceinline__ void load(const T *row, int64_t k, int64_t K, bool vec) {
-    if (vec && k + 8 <= K) {
-      const uint4 *q = reinterpret_cast<const uint4 *>(row + k);
+__device__ __forceinline__ void mv_load_x(float (&v)[8], const T *row, int64_t k, int64_t K, bool vec) {
+  if (vec && k + 8 <= K) {
+    union {
+      uint4 q[sizeof(T) / 2];
+      T e[8];
+    } u;
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-        const uint4 v = __ldg(q + i);
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-      }
-    } else if constexpr (sizeof(T) == 4) {
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.q[i] = reinterpret_cast<const uint4 *>(row + k)[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = k + i < K ? __float_as_uint(row[k + i]) : 0u;
-    } else {
-      const uint16_t *q = reinterpret_cast<const uint16_t *>(row);
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(u.e[i]);
+  } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = k + 2 * i < K ? q[k + 2 * i] : 0u;
-        if (k + 2 * i + 1 < K) w[i] |= (uint32_t)q[k + 2 * i + 1] << 16;
-      }
-    }
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
   }
-  // part p (0..2) of FP32: 8 bits of the mantissa each, what is left handed to the next call
-  __device__ __forceinline__ uint4 part(int p) {
-    uint32_t h[4];
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = w[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t lo = w[2 * i] & 0xffff0000u, hi = w[2 * i + 1] & 0xffff0000u;
-        const float f0 = __uint_as_float(w[2 * i]), f1 = __uint_as_float(w[2 * i + 1]);
-        if (p == 0) {
-          if (f0 != f0) lo = 0x7fff0000u;      // a NaN whose upper half alone would read as infinity
-          if (f1 != f1) hi = 0x7fff0000u;
-        }
-        h[i] = (lo >> 16) | hi;
-        // an infinity or NaN is whole in the first part
-        w[2 * i] = isfinite(f0) ? __float_as_uint(f0 - __uint_as_float(lo)) : 0u;
-        w[2 * i + 1] = isfinite(f1) ? __float_as_uint(f1 - __uint_as_float(hi)) : 0u;
-      }
-    }
-    return mv_pair(make_uint4(h[0], h[1], h[2], h[3]));
-  }
-};
-
-__device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// One block per row of x: its largest finite element, then the scaled, paired FP16 terms and the sums over parts of groups
+// (1 << part_log elements: a group, or the 128 of a longer one that a warp multiplies).  Four units of 8 elements per thread are
+// kept between the two passes; a longer row is read again.
+template <class T>
+__global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ldx, int vec, const T *x, int chunks, int nb, int rows_per_item,
+                                                           int part_log, unsigned char *image, int2 *row_info) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kKept = 4;
+  __shared__ float largest[kMvXThreads / 32];
+  __shared__ int odd[kMvXThreads / 32];
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int m = blockIdx.x, item = m / rows_per_item, col0 = (m - item * rows_per_item) * kParts;
+  const T *row = x + m * ldx;
+  const int units = chunks * (kMvChunk / 8);
+  float v[kKept][8];
+  float top = 0.f;
+  bool bad = false;
+  auto look = [&](const float (&e)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (isfinite(e[i])) top = fmaxf(top, fabsf(e[i]));
+      else bad = true;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (tid + i * kMvXThreads < units) mv_load_x<T>(v[i], row, 8 * (int64_t)(tid + i * kMvXThreads), K, vec != 0);
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (tid + i * kMvXThreads < units) look(v[i]);
+  for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
+    float e[8];
+    mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
+    look(e);
+  }
+  top = w4_warp_max(top);
+  const bool any = __any_sync(0xffffffffu, bad);
+  if (lane == 0) largest[tid >> 5] = top, odd[tid >> 5] = any;
+  __syncthreads();
+  top = w4_warp_max(lane < kMvXThreads / 32 ? largest[lane] : 0.f);
+  bad = __any_sync(0xffffffffu, lane < kMvXThreads / 32 && odd[lane]);
+  int q = 0;
+  if (top > 0.f) frexpf(top, &q), q = 15 - q;       // top * 2^q in [2^14, 2^15)
+  if (tid == 0) row_info[m] = make_int2(q, bad);
+  const int q1 = q / 2, q2 = q - q1;               // 2^q itself may pass FP32's range
+  const float f1 = ldexpf(1.f, q1), f2 = ldexpf(1.f, q2);
+
+  const int chunk_bytes = nb * (kMvChunk * 8 * 2 + 256);
+  auto put = [&](const float (&e)[8], int u) {
+    unsigned char *chunk = image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes;
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) ? 0.0625f : 1.f) : 0.f;
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      const int col = col0 + p;
+      __half h[8];
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        h[i] = __float2half_rn(r[i]);
+        const float back = __half2float(h[i]);
+        sum += (i & 1) ? 16.f * back : back;
+        r[i] = (r[i] - back) * 2048.f;       // what the term left, 11 bits up, for the next
+      }
+      union {
+        __half2 h2[4];
+        uint4 q;
+      } out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out.h2[i] = __halves2half2(h[i], h[i + 4]);
+      reinterpret_cast<uint4 *>(chunk)[((((u >> 2) & 7) * nb + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = out.q;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1)
+        if (o < (1 << (part_log - 3))) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((u & ((1 << (part_log - 3)) - 1)) == 0)
+        reinterpret_cast<float *>(chunk + nb * (kMvChunk * 8 * 2))[((u & 31) >> (part_log - 3)) * 8 * nb + col] = sum * 0x1p-24f;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (tid + i * kMvXThreads < units) put(v[i], tid + i * kMvXThreads);     // whole warps: units is a multiple of 32
+  for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
+    float e[8];
+    mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
+    put(e, u);
+  }
+}
+
+__device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The zero point in the form that unpacking subtracts: 8 + z/16 (bf16), 64 + z/16 (f16), in both halves.
-__device__ __forceinline__ uint32_t mv_zero(uint32_t z, __nv_bfloat16) { return 0x41004100u | z * 0x00010001u; }
-__device__ __forceinline__ uint32_t mv_zero(uint32_t z, __half) { return 0x54005400u | z * 0x00010001u; }
-
-// (w & mask) | bits in one instruction (left to itself the compiler makes two of it, having two constants: 69.5 us for 63.3)
-__device__ __forceinline__ uint32_t mv_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
-  return r;
-}
-// (c - z) / 16 of codes j and j + 4 of a word, j = 0..3.
-__device__ __forceinline__ uint32_t mv_unpack(uint32_t w, int j, uint32_t zero, __nv_bfloat16) {
-  const uint32_t v = mv_and_or(w >> (4 * j), 0x000f000fu, 0x41004100u);
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&zero));
-  return *reinterpret_cast<const uint32_t *>(&r);
-}
-__device__ __forceinline__ uint32_t mv_unpack(uint32_t w, int j, uint32_t zero, __half) {
-  const uint32_t v = mv_and_or(w >> (4 * j), 0x000f000fu, 0x54005400u);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&zero));
-  return *reinterpret_cast<const uint32_t *>(&r);
-}
-
-__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) { return __uint_as_float(ld_shared_cluster_u32(cluster_addr)); }
-
-// A tensor map of `rows` rows of `cols` elements, `pitch` bytes apart, in boxes of 128 bytes x box_rows.
-static int mv_map(CUtensorMap *out, CUtensorMapDataType type, int elem, const void *base, int64_t cols, int64_t rows, int64_t pitch,
-                  int box_rows) {
+// A tensor map of `rows` rows of `cols` bytes, `pitch` bytes apart, in boxes of 128 bytes x box_rows.
+static int mv_map(CUtensorMap *out, const void *base, int64_t cols, int64_t rows, int64_t pitch, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
   B2_REQUIRE(fn != nullptr, B2_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / elem), (cuuint32_t)box_rows}, steps[2] = {1, 1};
-  const CUresult r = fn(out, type, 2, (void *)base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void *)base, dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   B2_REQUIRE(r == CUDA_SUCCESS, B2_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (%lld x %lld, pitch %lld)", (int)r,
              (long long)rows, (long long)cols, (long long)pitch);
   return B2_OK;
 }
 
+// `bytes` (a multiple of 16, both addresses 16-byte aligned) from global to this CTA's shared memory, completion on an mbarrier.
+__device__ __forceinline__ void bulk_load(void *smem_dst, const void *global, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(smem_dst)),
+               "l"(global), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
@@ -340,6 +360,7 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) { return __uint_as_float(ld_shared_cluster_u32(cluster_addr)); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void mv_consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kMvConsumers) : "memory"); }
@@ -368,7 +389,6 @@ struct MvWait {
   }
 };
 
-// ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
 // A place in a ring of buffers, and the parity of its turn.
 struct MvRing {
   int at = 0, size;
@@ -379,39 +399,54 @@ struct MvRing {
   }
 };
 
-template <class T, int NB, bool ALIGNED>
-__global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
-    w4_matvec_kernel(const MvArgs a, const __grid_constant__ CUtensorMap code_map, const __grid_constant__ CUtensorMap x_map) {
-  using Tile = MvTile<T, NB>;
-  using H = typename MvType<T>::half_t;
+__device__ __forceinline__ float mv_load_any_type(const void *p, int type, int64_t at) {
+  if (type == B2_F32) return ((const float *)p)[at];
+  if (type == B2_BF16) return to_f32(((const __nv_bfloat16 *)p)[at]);
+  return to_f32(((const __half *)p)[at]);
+}
+
+// What the infinities and NaN of row m of x add to output n.
+__device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n) {
+  float v = 0.f;
+  for (int64_t k = 0; k < a.K; ++k) {
+    const float e = mv_load_any_type(a.x, a.type, m * a.ldx + k);
+    if (isfinite(e)) continue;
+    const int c = (a.codes[n * a.ldq + (k >> 1)] >> (4 * (k & 1))) & 15;
+    const int64_t g = n * a.groups + (k >> a.group_shift);
+    v += e * (((float)c - w4_zero(a.zeros, g)) * mv_load_any_type(a.scales, a.scale_type, g));
+  }
+  return v;
+}
+
+// ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
+template <int NB, bool ALIGNED>
+__global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
+    w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
+  using Tile = MvTile<NB>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle is one of addresses
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster_ctarank(), ctas = (int)gridDim.y;        // blockIdx.y is the rank within the cluster
   const int first = rank * a.chunks_per_cta;
-  int chunks = (int)((a.K + kMvChunk - 1) / kMvChunk) - first;
+  int chunks = a.chunks - first;
   chunks = chunks < 0 ? 0 : chunks < a.chunks_per_cta ? chunks : a.chunks_per_cta;
   const int window_log = a.group_shift - 5;                                // chunks of a window: group / 32
-  const int64_t width = (a.K + 1) >> 1;
-  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]
-  unsigned char *const xs = reinterpret_cast<unsigned char *>(windows + kMvWindows * kMvWindow);   // [chunk][block of 32][NB][column][word] x 16 bytes
-  float *const sums = reinterpret_cast<float *>(xs + a.panel_chunks * Tile::kXBytes);   // [2][8 NB][kMvPitch]
+  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, zero point
+  float *const sums = reinterpret_cast<float *>(windows + kMvWindows * kMvWindow);       // [2][8 NB][kMvPitch]
   uint64_t *const full = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sums) + Tile::kSumBytes);
   uint64_t *const empty = full + kMvMaxStages, *const wfull = empty + kMvMaxStages, *const wempty = wfull + kMvWindows;
-  uint64_t *const xfull = wempty + kMvWindows, *const xempty = xfull + 1, *const ready = xfull + 2, *const done = xfull + 3;
-  constexpr int kFillers = ALIGNED ? kMvProducers - 32 : kMvProducers;     // threads that write shared memory themselves
+  uint64_t *const ready = wempty + kMvWindows, *const done = ready + 1;
+  constexpr int kFillers = kMvProducers - 32;     // threads that write shared memory themselves
 
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&full[s], ALIGNED ? (Tile::kStream && !a.xvec ? 1 + kFillers : 1) : kFillers);
+      mbar_init(&full[s], ALIGNED ? 1 : 1 + kFillers);
       mbar_init(&empty[s], kMvConsumers / 32);
     }
     for (int s = 0; s < kMvWindows; ++s) {
       mbar_init(&wfull[s], kFillers);
       mbar_init(&wempty[s], kMvConsumers / 32);
     }
-    mbar_init(xfull, kFillers);
-    mbar_init(xempty, kMvConsumers / 32);
     mbar_init(ready, ctas);
     mbar_init(done, ctas);
     mbar_fence_init();
@@ -421,22 +456,35 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
   MvWait wait{a.status, a.seq};
 
   if (warp >= kMvConsumers / 32) {
-    if (ALIGNED && warp == kMvConsumers / 32) {
+    if (warp == kMvConsumers / 32) {
       if (lane == 0) {
+        // Weights may be read at once: the kernel in front of this one, w4_x_kernel, began after all earlier work had ended.
+        // Its own results, x, have to be waited for; the ring is filled with codes first.
         MvRing ring(a.stages);
         uint32_t sent = 0;
+        const unsigned char *late[kMvMaxStages];
+        bool waited = false;
+        auto send_x = [&](int s, const unsigned char *from) {
+          bulk_load(smem + s * Tile::kStage + kMvCodeBytes, from, Tile::kXBytes, &full[s]);
+        };
         for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
           const int mc = item / a.row_blocks, row = (item - mc * a.row_blocks) * kMvRows;
-          for (int c = 0; c < chunks; ++c, ring.next()) {
+          const unsigned char *image = a.image + ((int64_t)mc * a.chunks + first) * Tile::kXBytes;
+          for (int c = 0; c < chunks; ++c, ring.next(), image += Tile::kXBytes) {
             if (sent >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
             if (!wait.alive) continue;
-            unsigned char *stage = smem + ring.at * Tile::kStage;
-            mbar_expect_tx(&full[ring.at], kMvCodeBytes + (Tile::kStream && a.xvec ? Tile::kXBytes : 0));
-            tma_load_2d(stage, &code_map, &full[ring.at], (first + c) * kMvRowBytes, row);
-            if (Tile::kStream && a.xvec) {      // columns that are not used lie behind M: zeros
-#pragma unroll
-              for (int q = 0; q < kMvChunk / 64; ++q)
-                tma_load_2d(stage + kMvCodeBytes + q * (Tile::kXBytes / 4), &x_map, &full[ring.at], (first + c) * kMvChunk + 64 * q, mc * Tile::kM);
+            mbar_expect_tx(&full[ring.at], (ALIGNED ? kMvCodeBytes : 0) + Tile::kXBytes);
+            if (ALIGNED) tma_load_2d(smem + ring.at * Tile::kStage, &code_map, &full[ring.at], (first + c) * kMvRowBytes, row);
+            if (waited) {
+              send_x(ring.at, image);
+            } else {
+              late[sent] = image;
+              const bool last = c + 1 == chunks && item + (int)gridDim.x >= a.items;
+              if (sent + 1 == (uint32_t)a.stages || last) {
+                pdl_wait();
+                waited = true;
+                for (uint32_t i = 0; i <= sent; ++i) send_x((int)i, late[i]);
+              }
             }
             ++sent;
           }
@@ -445,53 +493,18 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
       }
       __syncwarp();
     } else {
-      const int me = tid - kMvConsumers - (ALIGNED ? 32 : 0);
+      const int me = tid - kMvConsumers - 32;
       MvRing ring(a.stages), window(kMvWindows);
-      uint32_t filled = 0, opened = 0, xcount = 0;
-      int held_mc = -1, held_panel = -1;
+      uint32_t filled = 0, opened = 0;
       for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-        const int mc = item / a.row_blocks, m0 = mc * Tile::kM;
-        const int64_t n0 = (int64_t)(item - mc * a.row_blocks) * kMvRows;
-        int panel = 0, in_panel = 0;
+        const int64_t n0 = (int64_t)(item % a.row_blocks) * kMvRows, n_rows = a.N - n0;
         for (int c = 0; c < chunks; ++c) {
-          if (!Tile::kStream && (mc != held_mc || panel != held_panel)) {      // this panel's x: 8 elements of k per thread and turn, zeros in unused columns
-            held_mc = mc, held_panel = panel;
-            if (xcount > 0) wait(xempty, (xcount - 1) & 1);
-            ++xcount;
-            const int left = chunks - c, n_chunks = left < a.panel_chunks ? left : a.panel_chunks;
-            const int64_t k0 = (int64_t)(first + c) * kMvChunk;
-            uint4 *to = reinterpret_cast<uint4 *>(xs);
-            const int units = n_chunks * (kMvChunk / 8);
-            // unit v: 8 elements of k of row v / units; several in flight per thread
-            constexpr int kFlight = sizeof(T) == 4 ? 2 : 4, kXRows = (8 * NB + Tile::kParts - 1) / Tile::kParts;
-            for (int v0 = me; v0 < kXRows * units; v0 += kFlight * kFillers) {
-              MvUnit<T> v[kFlight];
-#pragma unroll
-              for (int i = 0; i < kFlight; ++i) {
-                const int at = v0 + i * kFillers, m = at / units, u = at - m * units;
-                v[i] = MvUnit<T>{};
-                if (m < Tile::kM && m0 + m < a.M) v[i].load((const T *)a.x + (int64_t)(m0 + m) * a.ldx, k0 + 8 * u, a.K, a.xvec != 0);
-              }
-#pragma unroll
-              for (int i = 0; i < kFlight; ++i) {
-                const int at = v0 + i * kFillers, m = at / units, u = at - m * units;
-#pragma unroll
-                for (int p = 0; p < Tile::kParts; ++p) {
-                  const int col = m * Tile::kParts + p;
-                  const uint4 h = v[i].part(p);
-                  if (col < 8 * NB) to[(((u >> 2) * NB + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = h;
-                }
-              }
-            }
-            mbar_arrive(xfull);
-          }
           if ((c & ((1 << window_log) - 1)) == 0) {
             // scales and zero points of a window: entry e is group e & 7 of row e >> 3; all loads before the first use
             constexpr int kTurns = (kMvWindow + kFillers - 1) / kFillers;
             uint32_t scale[kTurns], zero[kTurns];
             const int64_t q0 = ((int64_t)(first + c) * kMvChunk) >> a.group_shift;
             const int count = a.groups - q0 < 8 ? (int)(a.groups - q0) : 8;
-            const int64_t n_rows = a.N - n0;
             const int64_t base = n0 * a.groups + q0;
 #pragma unroll
             for (int i = 0; i < kTurns; ++i) {
@@ -511,48 +524,25 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
               const float s = a.scale_type == B2_F32    ? __uint_as_float(scale[i])
                               : a.scale_type == B2_BF16 ? __uint_as_float(scale[i] << 16)
                                                         : __half2float(__ushort_as_half((unsigned short)scale[i]));
-              if (e < kMvWindow) to[e] = make_float2(s, __uint_as_float(mv_zero(zero[i] & 15, H())));
+              if (e < kMvWindow) to[e] = make_float2(s, (float)(zero[i] & 15));
             }
             mbar_arrive(&wfull[window.at]);
             window.next();
           }
-          if (!ALIGNED || (Tile::kStream && !a.xvec)) {
+          if (!ALIGNED) {
             if (filled >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
             ++filled;
             unsigned char *stage = smem + ring.at * Tile::kStage;
-            if constexpr (Tile::kStream) {        // as the TMA would lay it: 128-byte rows of 64 k, 16-byte unit u at u ^ (row & 7)
-              const int64_t k0 = (int64_t)(first + c) * kMvChunk;
-              constexpr int kFlight = 4;
-              for (int v0 = me; v0 < 8 * NB * 32; v0 += kFlight * kFillers) {
-                MvUnit<T> v[kFlight];
-#pragma unroll
-                for (int i = 0; i < kFlight; ++i) {
-                  const int m = (v0 + i * kFillers) >> 5, u = (v0 + i * kFillers) & 31;
-                  v[i] = MvUnit<T>{};
-                  if (m < 8 * NB && m0 + m < a.M) v[i].load((const T *)a.x + (int64_t)(m0 + m) * a.ldx, k0 + 8 * u, a.K, a.xvec != 0);
-                }
-#pragma unroll
-                for (int i = 0; i < kFlight; ++i) {
-                  const int m = (v0 + i * kFillers) >> 5, u = (v0 + i * kFillers) & 31;
-                  if (m < 8 * NB)
-                    *reinterpret_cast<uint4 *>(stage + kMvCodeBytes + (u >> 3) * (Tile::kXBytes / 4) + m * 128 + (((u & 7) ^ (m & 7)) << 4)) =
-                        make_uint4(v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]);
-                }
-              }
-            }
-            if (!ALIGNED) {
-              const int64_t at = (int64_t)(first + c) * kMvRowBytes;
-              for (int u = me; u < kMvCodeBytes / 16; u += kFillers) {
-                const int r = u >> 3, cc = u & 7;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (n0 + r < a.N && at + 16 * cc < width) v = mv_load_any(a.codes + (n0 + r) * a.ldq, at + 16 * cc, width);
-                *reinterpret_cast<uint4 *>(stage + r * kMvRowBytes + ((cc ^ (r & 7)) << 4)) = v;
-              }
+            const int64_t at = (int64_t)(first + c) * kMvRowBytes, width = (a.K + 1) >> 1;
+            for (int u = me; u < kMvCodeBytes / 16; u += kFillers) {
+              const int r = u >> 3, cc = u & 7;
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (r < n_rows && at + 16 * cc < width) v = mv_load_any(a.codes + (n0 + r) * a.ldq, at + 16 * cc, width);
+              *reinterpret_cast<uint4 *>(stage + r * kMvRowBytes + ((cc ^ (r & 7)) << 4)) = v;
             }
             mbar_arrive(&full[ring.at]);
             ring.next();
           }
-          if (++in_panel == a.panel_chunks) in_panel = 0, ++panel;
         }
       }
     }
@@ -560,33 +550,20 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
     cluster_wait();
   } else {
     const int g = lane >> 2, t = lane & 3, wn = warp & 3, wk = warp >> 2;
-    // A column of the tensor-core tile holds this row of a streamed x: two neighbouring lanes of a load 4 rows apart, so that
-    // its quarter warps fall into different halves of the banks.
-    const int xcol = (g >> 1) + 4 * (g & 1);
-    uint32_t xcount = 0, turn = 0;
+    const int parts_log = a.group_shift < 7 ? a.group_shift - 5 : 2;      // blocks of 32 in a part of a group
+    uint32_t turn = 0;
     MvRing ring(a.stages), window(kMvWindows);
-    int held_mc = -1, held_panel = -1;
     for (int item = blockIdx.x; item < a.items; item += gridDim.x, ++turn) {
       const int mc = item / a.row_blocks;
-      int panel = 0, in_panel = 0;
       float total[2][NB][4] = {};
       for (int c = 0; c < chunks; ++c) {
-        if (!Tile::kStream && (mc != held_mc || panel != held_panel)) {
-          if (held_mc >= 0) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(xempty);
-          }
-          held_mc = mc, held_panel = panel;
-          wait(xfull, xcount & 1);
-          ++xcount;
-        }
         const int in_window = c & ((1 << window_log) - 1);
         if (in_window == 0) wait(&wfull[window.at], window.phase);
         wait(&full[ring.at], ring.phase);
         const unsigned char *const stage = smem + ring.at * Tile::kStage;
         const unsigned char *codes = stage + (wn * 32 + g) * kMvRowBytes + 4 * t;
-        const uint4 *xf = reinterpret_cast<const uint4 *>(xs) + in_panel * (Tile::kXBytes / 16) + lane;
-        const unsigned char *xr = stage + kMvCodeBytes + xcol * 128;
+        const uint4 *xf = reinterpret_cast<const uint4 *>(stage + kMvCodeBytes) + wk * 4 * NB * 32 + lane;
+        const float *xsum = reinterpret_cast<const float *>(stage + kMvCodeBytes + NB * (kMvChunk * 8 * 2)) + 2 * t;
         const float2 *sz = windows + window.at * kMvWindow + ((wn * 32 + g) << 3);
         const int block0 = in_window * 8 + wk * 4;                    // this warp's first block of 32 k within the window
         // the warp's 128 k in straight-line code, BLOCKS blocks of 32 to a group (or to the warp's part of one)
@@ -594,48 +571,40 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
           constexpr int BLOCKS = decltype(blocks)::value;
 #pragma unroll
           for (int b0 = 0; b0 < 4; b0 += BLOCKS) {
-            float sc[4], acc[2][NB][4] = {};
-            uint32_t z[4];
-            const float2 *from = sz + ((block0 + b0) >> window_log);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float2 v = from[(8 * r) << 3];
-              sc[r] = v.x, z[r] = __float_as_uint(v.y);
-            }
+            float acc[2][NB][4] = {};
 #pragma unroll
             for (int b4 = b0; b4 < b0 + BLOCKS; ++b4) {
-              const int b = wk * 4 + b4;
               uint4 xv[NB];
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                if constexpr (Tile::kStream) {
-                  // (wk * 4 + b4) >> 1 and & 1, with b4 known
-                  const int unit = ((b4 & 1) * 4 + t) ^ xcol;
-                  xv[nb] = mv_pair(*reinterpret_cast<const uint4 *>(xr + (wk * 2 + (b4 >> 1)) * (Tile::kXBytes / 4) + nb * 1024 + (unit << 4)));
-                } else {
-                  xv[nb] = xf[(b * NB + nb) * 32];
-                }
-              }
+              for (int nb = 0; nb < NB; ++nb) xv[nb] = xf[(b4 * NB + nb) * 32];
 #pragma unroll
               for (int rt = 0; rt < 2; ++rt) {
-                const int place = (b ^ g) << 4;                     // rows g, g + 8, ... have one place
+                const int place = ((wk * 4 + b4) ^ g) << 4;           // rows g, g + 8, ... have one place
                 const uint32_t w0 = *reinterpret_cast<const uint32_t *>(codes + (rt * 16) * kMvRowBytes + place);
                 const uint32_t w1 = *reinterpret_cast<const uint32_t *>(codes + (rt * 16 + 8) * kMvRowBytes + place);
-                const uint32_t z0 = z[2 * rt], z1 = z[2 * rt + 1];
-                const uint32_t f[4] = {mv_unpack(w0, 0, z0, H()), mv_unpack(w1, 0, z1, H()), mv_unpack(w0, 1, z0, H()), mv_unpack(w1, 1, z1, H())};
+                const uint32_t f[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y, H());
-                const uint32_t h[4] = {mv_unpack(w0, 2, z0, H()), mv_unpack(w1, 2, z1, H()), mv_unpack(w0, 3, z0, H()), mv_unpack(w1, 3, z1, H())};
+                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+                const uint32_t h[4] = {v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u};
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], h, xv[nb].z, xv[nb].w, H());
+                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], h, xv[nb].z, xv[nb].w);
               }
             }
+            const float2 *from = sz + ((block0 + b0) >> window_log);
+            const float *xs = xsum + ((wk * 4 + b0) >> parts_log) * 8 * NB;
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
+            for (int nb = 0; nb < NB; ++nb) {
+              const float2 x2 = *reinterpret_cast<const float2 *>(xs + nb * 8);
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) total[rt][nb][i] = fmaf(sc[2 * rt + (i >> 1)], acc[rt][nb][i], total[rt][nb][i]);
+              for (int r = 0; r < 4; ++r) {
+                const float2 v = from[(8 * r) << 3];                  // scale and zero point of row g + 8 r
+                float(&tot)[4] = total[r >> 1][nb];
+                const float(&ac)[4] = acc[r >> 1][nb];
+                tot[2 * (r & 1)] = fmaf(v.x, fmaf(-v.y, x2.x, ac[2 * (r & 1)]), tot[2 * (r & 1)]);
+                tot[2 * (r & 1) + 1] = fmaf(v.x, fmaf(-v.y, x2.y, ac[2 * (r & 1) + 1]), tot[2 * (r & 1) + 1]);
+              }
+            }
           }
         };
         if (a.group_shift >= 7) multiply(std::integral_constant<int, 4>());
@@ -649,7 +618,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
         }
         ring.next();
         if (window_ends) window.next();
-        if (++in_panel == a.panel_chunks) in_panel = 0, ++panel;
       }
 
       __syncwarp();
@@ -661,40 +629,43 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<T, NB>::kCtasPerSm)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = 2 * t + (i & 1), m = Tile::kStream ? (col >> 1) + 4 * (col & 1) : col;
-            sums[(wk * 8 * NB + nb * 8 + m) * kMvPitch + wn * 32 + rt * 16 + g + (i >> 1) * 8] = total[rt][nb][i];
-          }
+          for (int i = 0; i < 4; ++i)
+            sums[(wk * 8 * NB + nb * 8 + 2 * t + (i & 1)) * kMvPitch + wn * 32 + rt * 16 + g + (i >> 1) * 8] = total[rt][nb][i];
       mv_consumers_sync();
       if (ctas > 1) {
         if (tid < ctas) mbar_arrive_cluster(mapa_u32(smem_u32(ready), (uint32_t)tid));
         wait.cluster(ready, turn & 1);
       }
-      const int m0 = mc * Tile::kM, mm = a.M - m0 < Tile::kM ? a.M - m0 : Tile::kM;
+      const int m0 = mc * a.rows_per_item, mm = a.M - m0 < a.rows_per_item ? a.M - m0 : a.rows_per_item;
       const int64_t n0 = (int64_t)(item - mc * a.row_blocks) * kMvRows;
+      if (turn == 0) pdl_wait();                                    // row_info is w4_x_kernel's
       for (int i = tid + rank * kMvConsumers; i < mm * kMvRows; i += kMvConsumers * ctas) {
         const int m = i / kMvRows, r = i % kMvRows;
-        const float *at = sums + m * Tile::kParts * kMvPitch + r;
+        if (n0 + r >= a.N) continue;
         float v = 0.f;
-        if (ctas > 1) {
-          for (int q = 0; q < ctas; ++q) {
-            const uint32_t from = mapa_u32(smem_u32(at), (uint32_t)q);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int p = 0; p < Tile::kParts; ++p) v += ld_shared_cluster_f32(from + (k * 8 * NB + p) * kMvPitch * 4);
+        if (a.chunks > 0) {
+          const int2 info = a.row_info[m0 + m];
+          for (int p = 0; p < a.parts; ++p) {
+            const float *at = sums + (m * a.parts + p) * kMvPitch + r;
+            float s = 0.f;
+            if (ctas > 1) {
+              for (int q = 0; q < ctas; ++q) {
+                const uint32_t from = mapa_u32(smem_u32(at), (uint32_t)q);
+                s += ld_shared_cluster_f32(from) + ld_shared_cluster_f32(from + 8 * NB * kMvPitch * 4);
+              }
+            } else {
+              s = at[0] + at[8 * NB * kMvPitch];
+            }
+            v += ldexpf(s, 24 - 11 * p - info.x);                   // the codes' 2^-24, the row's scale and the term's
           }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int p = 0; p < Tile::kParts; ++p) v += at[(k * 8 * NB + p) * kMvPitch];
+          if (info.y) v += mv_not_finite(a, m0 + m, n0 + r);
         }
-        if (n0 + r < a.N) {
-          T *to = (T *)a.y + (int64_t)(m0 + m) * a.ldy + n0 + r;
-          v = a.alpha * (16.f * v);
-          *to = from_f32<T>(a.beta != 0.f ? fmaf(a.beta, to_f32(*to), v) : v);
-        }
+        v *= a.alpha;
+        const int64_t to = (int64_t)(m0 + m) * a.ldy + n0 + r;
+        if (a.beta != 0.f) v = fmaf(a.beta, mv_load_any_type(a.y, a.type, to), v);
+        if (a.type == B2_F32) ((float *)a.y)[to] = v;
+        else if (a.type == B2_BF16) ((__nv_bfloat16 *)a.y)[to] = from_f32<__nv_bfloat16>(v);
+        else ((__half *)a.y)[to] = from_f32<__half>(v);
       }
       mv_consumers_sync();
       if (ctas > 1 && tid < ctas) mbar_arrive_cluster(mapa_u32(smem_u32(done), (uint32_t)tid));
@@ -736,44 +707,38 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   return B2_OK;
 }
 
-template <class T, int NB, bool ALIGNED>
+template <int NB, bool ALIGNED>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
-  using Tile = MvTile<T, NB>;
-  const auto kernel = w4_matvec_kernel<T, NB, ALIGNED>;
+  using Tile = MvTile<NB>;
+  const auto kernel = w4_matvec_kernel<NB, ALIGNED>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
-  const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows, chunks = (a.K + kMvChunk - 1) / kMvChunk;
-  const int m_chunks = (a.M + Tile::kM - 1) / Tile::kM;
+  const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows;
+  const int m_chunks = (a.M + a.rows_per_item - 1) / a.rows_per_item;
   B2_REQUIRE(row_blocks * m_chunks <= INT32_MAX / 2, B2_ERR_UNSUPPORTED, "b2_w4_matvec: N = %lld is too large", (long long)a.N);
   a.row_blocks = (int)row_blocks;
   a.items = (int)row_blocks * m_chunks;
-  // CTAs of a cluster, each with a chunk at least: the number that makes the longest CTA shortest, counted in chunks.  A row
-  // block's exchange counts as one more, and so does bringing x of a chunk into shared memory: once if all of a CTA's part
-  // fits, for every row block if not.
-  const int largest = Tile::kXLargest / Tile::kXBytes;
+  // CTAs of a cluster, each with a chunk at least: the number that makes the longest CTA shortest, counted in chunks, where a
+  // row block's exchange counts as one more
   int ctas = 1, clusters = 1;
   int64_t shortest = INT64_MAX;
-  for (int n = 1; n <= 8 && (n == 1 || n <= chunks); n *= 2) {
+  for (int n = 1; n <= 8 && (n == 1 || n <= a.chunks); n *= 2) {
     int held = 1;
     const int e = mv_clusters((const void *)kernel, ctx->device, n, Tile::kSmem, &held);
     if (e != B2_OK) return e;
     if (held > a.items) held = a.items;
-    const int64_t turns = (a.items + held - 1) / held, each = (chunks + n - 1) / n;
-    const int64_t length = turns * (each + 1) + (Tile::kStream ? 0 : each <= largest ? each : turns * each);
+    const int64_t length = (int64_t)((a.items + held - 1) / held) * ((a.chunks + n - 1) / n + 1);
     if (length < shortest) shortest = length, ctas = n, clusters = held;
   }
-  a.chunks_per_cta = (int)((chunks + ctas - 1) / ctas);
-  a.panel_chunks = a.chunks_per_cta < largest ? a.chunks_per_cta : largest;
-  const int other = a.panel_chunks * Tile::kXBytes + Tile::kSumBytes + kMvWindows * kMvWindow * 8 + kMvBarrierBytes;
+  a.chunks_per_cta = (a.chunks + ctas - 1) / ctas;
+  const int other = Tile::kSumBytes + kMvWindows * kMvWindow * 8 + kMvBarrierBytes;
   a.stages = (Tile::kSmem - other) / Tile::kStage;
   if (a.stages > kMvMaxStages) a.stages = kMvMaxStages;
   const int64_t per_cta = (int64_t)a.chunks_per_cta * ((a.items + clusters - 1) / clusters);
   if (a.stages > per_cta) a.stages = per_cta > 0 ? (int)per_cta : 1;
-  CUtensorMap code_map = {}, x_map = {};
-  if (ALIGNED && a.K > 0) {
-    int e = mv_map(&code_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, (a.K + 1) / 2, a.N, a.ldq, kMvRows);
-    if (e == B2_OK && Tile::kStream && a.xvec)
-      e = mv_map(&x_map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.x, a.K, a.M, a.ldx * 2, 8 * NB);
+  CUtensorMap code_map = {};
+  if (ALIGNED && a.chunks > 0) {
+    const int e = mv_map(&code_map, a.codes, (a.K + 1) / 2, a.N, a.ldq, kMvRows);
     if (e != B2_OK) return e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -781,30 +746,33 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   cfg.blockDim = dim3(kMvThreads);
   cfg.dynamicSmemBytes = (size_t)(a.stages * Tile::kStage + other);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = (unsigned)ctas;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.chunks > 0 ? 2 : 1;        // without w4_x_kernel in front there is nothing to overlap
   a.status = (int *)((char *)ctx->fixed + kFixedStatus);
   a.seq = next_launch_seq(ctx);
-  B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const MvArgs)a, (const CUtensorMap)code_map, (const CUtensorMap)x_map));
+  B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const MvArgs)a, (const CUtensorMap)code_map));
   return B2_OK;
 }
 
-template <class T, bool ALIGNED>
-static int w4_matvec_rows(Context *ctx, const MvArgs &a, cudaStream_t s) {
-  if constexpr (sizeof(T) == 4) {
-    if (a.M <= 2) return w4_matvec_launch<T, 1, ALIGNED>(ctx, a, s);
-    if (a.M <= 5) return w4_matvec_launch<T, 2, ALIGNED>(ctx, a, s);
-    return w4_matvec_launch<T, 3, ALIGNED>(ctx, a, s);
-  } else {
-    if (a.M <= 8) return w4_matvec_launch<T, 1, ALIGNED>(ctx, a, s);
-    if (a.M <= 16) return w4_matvec_launch<T, 2, ALIGNED>(ctx, a, s);
-    return w4_matvec_launch<T, 4, ALIGNED>(ctx, a, s);
-  }
+template <bool ALIGNED>
+static int w4_matvec_blocks(Context *ctx, const MvArgs &a, int nb, cudaStream_t s) {
+  return nb == 1   ? w4_matvec_launch<1, ALIGNED>(ctx, a, s)
+         : nb == 2 ? w4_matvec_launch<2, ALIGNED>(ctx, a, s)
+                   : w4_matvec_launch<4, ALIGNED>(ctx, a, s);
+}
+
+// The workspace of a product: the image of x, then row_info.
+static size_t mv_image_bytes(int64_t M, int64_t K, int type) {
+  const int nb = mv_blocks(M, type);
+  const int64_t items = (M + mv_rows(nb, type) - 1) / mv_rows(nb, type);
+  return (size_t)(items * ((K + kMvChunk - 1) / kMvChunk)) * nb * (kMvChunk * 8 * 2 + 256);
 }
 
 // The checks that the three calls share: sizes, types, the codes' rows.
@@ -880,9 +848,14 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
   return B2_OK;
 }
 
+size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t K, int type) {
+  if (M <= 0 || M > kW4MaxRows || K <= 0 || K > INT32_MAX || type_bytes(type) == 0) return 0;
+  return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int2);
+}
+
 int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
                  const uint8_t *codes, int64_t ldq, int scale_type, const void *scales, const uint8_t *zeros, float beta,
-                 void *y, int64_t ldy, void *stream) {
+                 void *y, int64_t ldy, void *workspace, size_t workspace_bytes, void *stream) {
   const int st = w4_check("b2_w4_matvec", N, K, group, type, scale_type, codes, ldq, scales);
   if (st != B2_OK) return st;
   const int tb = type_bytes(type);
@@ -895,18 +868,36 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   B2_REQUIRE(y != nullptr && (K == 0 || x != nullptr), B2_ERR_INVALID_ARG, "b2_w4_matvec: x or y is NULL");
   B2_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (tb - 1)) == 0, B2_ERR_INVALID_ARG, "b2_w4_matvec: x or y is not aligned to its type");
   B2_REQUIRE(!matrices_overlap(x, M, K * tb, ldx * tb, y, M, N * tb, ldy * tb), B2_ERR_INVALID_ARG, "b2_w4_matvec: y overlaps x");
+  const size_t need = b2_w4_matvec_workspace_bytes(M, K, type);
+  B2_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), B2_ERR_WORKSPACE,
+             "b2_w4_matvec: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+  B2_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, B2_ERR_INVALID_ARG, "b2_w4_matvec: workspace is not 16-byte aligned");
   B2_CONTEXT(ctx, h, "b2_w4_matvec");
+  cudaStream_t s = (cudaStream_t)stream;
   MvArgs a = {};
   a.N = N, a.K = alpha != 0.f ? K : 0, a.ldx = ldx, a.ldq = ldq, a.ldy = ldy, a.groups = (K + group - 1) / group;
-  a.M = (int)M, a.scale_type = scale_type, a.alpha = alpha, a.beta = beta;
+  a.M = (int)M, a.type = type, a.scale_type = scale_type, a.alpha = alpha, a.beta = beta;
   a.group_shift = group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8;
   a.x = x, a.codes = codes, a.zeros = zeros, a.scales = scales, a.y = y;
+  const int nb = mv_blocks(M, type);
+  a.parts = mv_parts(type);
+  a.rows_per_item = mv_rows(nb, type);
+  a.chunks = (int)((a.K + kMvChunk - 1) / kMvChunk);
+  if (a.chunks > 0) {
+    unsigned char *image = (unsigned char *)workspace;
+    int2 *info = (int2 *)(image + mv_image_bytes(M, K, type));
+    a.image = image, a.row_info = info;
+    const int vec = (((uintptr_t)x | (uintptr_t)(ldx * tb)) & 15) == 0;
+    with_type(type, [&](auto t) {
+      using T = decltype(t);
+      w4_x_kernel<T><<<(unsigned)M, kMvXThreads, 0, s>>>(K, ldx, vec, (const T *)x, a.chunks, nb, a.rows_per_item,
+                                                         a.group_shift < 7 ? a.group_shift : 7, image, info);
+      return 0;
+    });
+    B2_CUDA(cudaGetLastError());
+  }
   const bool aligned = (((uintptr_t)codes | (uintptr_t)ldq) & 15) == 0;
-  a.xvec = (((uintptr_t)x | (uintptr_t)(ldx * tb)) & 15) == 0;
-  return with_type(type, [&](auto t) {
-    using T = decltype(t);
-    return aligned ? w4_matvec_rows<T, true>(ctx, a, (cudaStream_t)stream) : w4_matvec_rows<T, false>(ctx, a, (cudaStream_t)stream);
-  });
+  return aligned ? w4_matvec_blocks<true>(ctx, a, nb, s) : w4_matvec_blocks<false>(ctx, a, nb, s);
 }
 
 }  // extern "C"

@@ -208,10 +208,17 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
     return W
 
 
+def w4_matvec_workspace_bytes(M: int, K: int, dtype) -> int:
+    """Bytes that ``w4_matvec`` lays x out in."""
+    return int(_lib.load().b2_w4_matvec_workspace_bytes(M, K, TYPE_CODES[dtype]))
+
+
 def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, ldx=None, ldy=None, ldq=None,
-              handle: Handle | None = None):
+              workspace=None, handle: Handle | None = None):
     """y = alpha * x * W^T + beta * y with W (N x K) in 4-bit form, x (M x K) and y (M x N) of one type, M = 0..64 rows (more:
-    ``w4_dequantize`` once and ``sgemm``).  ``y`` None: a new tensor (beta must be 0).  Returns ``y``."""
+    ``w4_dequantize`` once and ``sgemm``).  ``y`` None: a new tensor (beta must be 0).  ``workspace``: a tensor of at least
+    ``w4_matvec_workspace_bytes(M, K, x.dtype)`` bytes that no other call uses meanwhile; None takes one from torch's allocator
+    on the current stream for this call.  Returns ``y``."""
     _tensor(x, "x")
     device = torch.cuda.current_device()
     if y is None:
@@ -223,6 +230,10 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
     py, ldy = _matrix(y, M, N, ldy, "y", device)
     _same_type(y, x.dtype, "y")
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
+    L = _lib.load()
+    if workspace is None:
+        workspace = torch.empty(L.b2_w4_matvec_workspace_bytes(M, K, t), dtype=torch.uint8, device=x.device)
+    ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
     h = handle or default_handle()
-    check(_lib.load().b2_w4_matvec(h.raw, M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, _stream(device)))
+    check(L.b2_w4_matvec(h.raw, M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
     return y

@@ -247,7 +247,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
  *   W[n][k] = (code - zero[n][k / group]) * scale[n][k / group].
  * group is 32, 64, 128 or 256; the last group of a row may be shorter.  Types: type and scale_type are each any of B2_F32,
  * B2_BF16, B2_F16.  Rows of codes that start on 16-byte boundaries (ldq a multiple of 16) are read fastest.  None of these
- * calls uses the handle's scratch: they may run on any number of streams at once. */
+ * calls uses the handle's scratch: they may run on any number of streams at once (the product with a workspace for each). */
 
 /* Quantises W (N x K, rows ldw elements apart).  Without zeros: scale = absmax / 7 over the group, codes 1..15 around 8.
  * With zeros: lo = min(0, smallest), hi = max(0, largest), scale = (hi - lo) / 15, zero = -lo / scale to the nearest integer.
@@ -266,10 +266,14 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 /* y = alpha * x * W^T + beta * y for M = 0..64 rows of x (M x K, ldx) and y (M x N, ldy), both of type `type`: the product of
  * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
  * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm.  y must not overlap x.
- * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit. */
+ * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.
+ * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, K, type) bytes (16 to 272 KB for K = 4096) that no other call
+ * uses meanwhile; x is laid out there for the tensor cores first.  A bounded wait that runs out on the device is left for
+ * b2_check_status as for the SGEMM. */
+size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t K, int type);
 int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
                  const uint8_t *codes, int64_t ldq, int scale_type, const void *scales, const uint8_t *zeros, float beta,
-                 void *y, int64_t ldy, void *stream);
+                 void *y, int64_t ldy, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- SGEMM on host arrays --------------------------------------------------------------- */
 

@@ -81,8 +81,8 @@ def dequantize(L, N=4, K=64, group=32, codes=at(0x8000), ldq=32, st=F32, scales=
 
 
 def matvec(L, M=2, N=4, K=64, group=32, alpha=1.0, type_=F32, x=at(0x1000), ldx=64, codes=at(0x8000), ldq=32, st=F32, scales=at(0x9000),
-           zeros=NULL, beta=0.0, y=at(0x2000), ldy=4):
-    return L.b2_w4_matvec(NULL, M, N, K, group, alpha, type_, x, ldx, codes, ldq, st, scales, zeros, beta, y, ldy, NULL)
+           zeros=NULL, beta=0.0, y=at(0x2000), ldy=4, ws=at(0x10000), nws=1 << 20):
+    return L.b2_w4_matvec(NULL, M, N, K, group, alpha, type_, x, ldx, codes, ldq, st, scales, zeros, beta, y, ldy, ws, nws, NULL)
 
 
 SHARED = [dict(N=-1), dict(K=-1), dict(group=0), dict(group=48), dict(group=512), dict(type_=3), dict(st=3), dict(ldq=31),
@@ -103,7 +103,7 @@ def test_w4_dequantize_refuses(L, bad):
 
 
 @pytest.mark.parametrize("bad", SHARED + [dict(M=-1), dict(ldx=63), dict(ldy=3), dict(x=NULL), dict(y=NULL), dict(x=at(0x1002)),
-                                          dict(y=at(0x1000)), dict(y=at(0x1100))])
+                                          dict(y=at(0x1000)), dict(y=at(0x1100)), dict(ws=at(0x10008))])
 def test_w4_matvec_refuses(L, bad):
     assert matvec(L, **bad) == INVALID
     assert L.b2_last_error()
@@ -112,6 +112,16 @@ def test_w4_matvec_refuses(L, bad):
 def test_w4_matvec_refuses_many_rows(L):
     assert matvec(L, M=layer.W4_MAX_ROWS + 1) == UNSUPPORTED
     assert b"b2_w4_dequantize" in L.b2_last_error()
+
+
+def test_w4_matvec_workspace(L):
+    for type_ in (F32, BF16, F16):
+        need = L.b2_w4_matvec_workspace_bytes(2, 64, type_)
+        assert need > 0
+        assert matvec(L, type_=type_, nws=need - 1) == WORKSPACE
+        assert matvec(L, type_=type_, ws=NULL) == WORKSPACE
+    assert L.b2_w4_matvec_workspace_bytes(0, 64, F32) == 0 and L.b2_w4_matvec_workspace_bytes(4, 0, F32) == 0
+    assert L.b2_w4_matvec_workspace_bytes(4, 64, 7) == 0
 
 
 def test_w4_empty_calls_are_no_ops(L):
