@@ -43,6 +43,11 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
   return __float2half_rn(v);
 }
 
+// Programmatic dependent launch: a kernel launched with the stream-serialization attribute may start while the one in front of
+// it still runs; it waits for that one's end, and so for its results, in pdl_wait.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Calls f with a value of the element type that `type` names; the type has been checked before.
 template <class F>
 inline int with_type(int type, F &&f) {

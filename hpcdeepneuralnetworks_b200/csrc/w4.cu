@@ -229,9 +229,6 @@ __device__ __forceinline__ void mv_load_x(float (&v)[8], const T *row, int64_t k
   }
 }
 
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // One block per row of x: its largest finite element, then the scaled, paired FP16 terms and the sums over parts of groups
 // (1 << part_log elements: a group, or the 128 of a longer one that a warp multiplies).  Four units of 8 elements per thread are
 // kept between the two passes; a longer row is read again.
