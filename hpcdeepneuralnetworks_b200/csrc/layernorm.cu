@@ -7,7 +7,9 @@
 #include <math.h>
 
 #include <initializer_list>
+#include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "types.cuh"
 
@@ -31,115 +33,291 @@ template <>
 struct LnRaw<2> {
   using type = uint16_t;
 };
-// V elements of type T as one access, and their values.
+// W = 1 or 2 FP32 values that are worked on together: sm_100 adds, multiplies and fuses two at a time, and these kernels spend
+// as many issue slots on arithmetic as the memory leaves them.
+template <int W>
+struct LnF;
+template <>
+struct LnF<1> {
+  float v;
+  __device__ __forceinline__ LnF() {}
+  __device__ __forceinline__ explicit LnF(float a) : v(a) {}
+  __device__ __forceinline__ LnF operator+(LnF o) const { return LnF(__fadd_rn(v, o.v)); }
+  __device__ __forceinline__ LnF operator*(LnF o) const { return LnF(__fmul_rn(v, o.v)); }
+  __device__ __forceinline__ float sum() const { return v; }
+};
+__device__ __forceinline__ LnF<1> ln_fma(LnF<1> a, LnF<1> b, LnF<1> c) { return LnF<1>(__fmaf_rn(a.v, b.v, c.v)); }
+template <>
+struct LnF<2> {
+  uint64_t v;
+  __device__ __forceinline__ LnF() {}
+  __device__ __forceinline__ LnF(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit LnF(float a) : LnF(a, a) {}
+  __device__ __forceinline__ float2 both() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+  __device__ __forceinline__ LnF operator+(LnF o) const {
+    LnF r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(v), "l"(o.v));
+    return r;
+  }
+  __device__ __forceinline__ LnF operator*(LnF o) const {
+    LnF r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(v), "l"(o.v));
+    return r;
+  }
+  __device__ __forceinline__ float sum() const {
+    const float2 r = both();
+    return r.x + r.y;
+  }
+};
+__device__ __forceinline__ LnF<2> ln_fma(LnF<2> a, LnF<2> b, LnF<2> c) {
+  LnF<2> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// V elements of type T as one access, and their values, W at a time.
 template <class T, int V>
 struct LnPack {
   using raw_t = typename LnRaw<V * sizeof(T)>::type;
+  static constexpr int W = V >= 2 ? 2 : 1, kParts = V / W;
+  using F = LnF<W>;
   union {
     raw_t raw;
     T e[V];
+    uint32_t words[V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1];
   };
   __device__ __forceinline__ LnPack() {}
   __device__ __forceinline__ void load_stream(const T *p) { raw = __ldcs(reinterpret_cast<const raw_t *>(p)); }   // read once
   __device__ __forceinline__ void load(const T *p) { raw = *reinterpret_cast<const raw_t *>(p); }
   __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<raw_t *>(p) = raw; }
-  __device__ __forceinline__ float get(int i) const { return to_f32(e[i]); }
-  __device__ __forceinline__ void set(int i, float v) { e[i] = from_f32<T>(v); }
+  __device__ __forceinline__ F get(int i) const {
+    if constexpr (W == 1) return F(to_f32(e[0]));
+    else if constexpr (sizeof(T) == 4) return F(e[2 * i], e[2 * i + 1]);
+    else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&words[i]));
+      return F(f.x, f.y);
+    } else return F(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u));
+  }
+  __device__ __forceinline__ void set(int i, F f) {
+    if constexpr (W == 1) e[0] = from_f32<T>(f.v);
+    else {
+      const float2 r = f.both();
+      if constexpr (sizeof(T) == 4) e[2 * i] = r.x, e[2 * i + 1] = r.y;
+      else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(r.x, r.y);
+        words[i] = *reinterpret_cast<const uint32_t *>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(r.x, r.y);
+        words[i] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+    }
+  }
 };
 // V values of a parameter vector (16-byte accesses where V elements are that long or longer), or a constant without one.
 template <class P, int V>
-__device__ __forceinline__ void ln_params(float (&v)[V], const P *p, int64_t at, float without) {
+__device__ __forceinline__ void ln_params(LnF<(V >= 2 ? 2 : 1)> (&v)[V >= 2 ? V / 2 : 1], const P *p, int at, float without) {
+  constexpr int W = V * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : V;
   if (!p) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = without;
+    for (int i = 0; i < (V >= 2 ? V / 2 : 1); ++i) v[i] = LnF<(V >= 2 ? 2 : 1)>(without);
     return;
   }
-  constexpr int W = V * (int)sizeof(P) > 16 ? 16 / (int)sizeof(P) : V;
 #pragma unroll
   for (int i = 0; i < V; i += W) {
     LnPack<P, W> q;
     q.load(p + at + i);
 #pragma unroll
-    for (int k = 0; k < W; ++k) v[i + k] = q.get(k);
+    for (int k = 0; k < LnPack<P, W>::kParts; ++k) v[i / LnPack<P, W>::W + k] = q.get(k);
   }
 }
 
-// Sums over the threads that share a row, the same bits in each of them: shuffles within a warp, then, where a block shares
-// it, the warps' sums in order.  `scratch` alternates between two arrays, so that one barrier per sum is enough.
-template <bool WARP>
-__device__ __forceinline__ float2 ln_sum2(float2 v, float2 *scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+// ---- teams --------------------------------------------------------------------------------------------
+// A row belongs to a team of `share` threads, whole warps; a block holds blockDim.x / share teams, each with rows of its own.
+// Each warp takes a run of the row, `turns` accesses of 32 lanes one behind the other: access i of a thread lies i * 32 * V
+// elements behind its first, a distance that is known when the kernel is compiled (with the threads' number in it instead, the
+// addresses took more instructions than the arithmetic).  FULL: every access of every thread lies within the row.
+struct LnTeam {
+  int team, teams, tid, warps, lane;
+  int64_t step, first;      // a team's rows: first, first + step, ...
+  __device__ __forceinline__ explicit LnTeam(int share) {
+    team = (int)threadIdx.x / share;
+    teams = (int)blockDim.x / share;
+    tid = (int)threadIdx.x - team * share;
+    warps = share >> 5;
+    lane = threadIdx.x & 31;
+    step = (int64_t)gridDim.x * teams;
+    first = (int64_t)blockIdx.x * teams + team;
   }
-  if (WARP) return v;
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
-  v = lane < warps ? scratch[lane] : make_float2(0.f, 0.f);
+  __device__ __forceinline__ int unit(int turns) const { return (tid >> 5) * 32 * turns + lane; }      // first unit of V elements
+  // accesses of this thread that lie within the row
+  __device__ __forceinline__ int valid(int units, int turns) const {
+    const int n = (units - unit(turns) + 31) >> 5;
+    return n < 0 ? 0 : n < turns ? n : turns;
+  }
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * warps) : "memory"); }
+};
+using LnScratch = float[2][32];      // [value][warp of the block]
+
+// Sums of two values over a team, the same bits in each thread, in a fixed order.  The lower half of a warp adds the first
+// value and the upper half the second, which takes half the shuffles.  A caller's next sum uses another scratch, so that one
+// barrier per sum is enough.
+__device__ __forceinline__ float2 ln_sum2(float2 v, LnScratch &scratch, const LnTeam &t) {
+  const bool up = t.lane & 16;
+  float keep = (up ? v.y : v.x) + __shfl_xor_sync(0xffffffffu, up ? v.x : v.y, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  for (int o = 8; o > 0; o >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, o);
+  if (t.warps > 1) {
+    if ((t.lane & 15) == 0) scratch[up][threadIdx.x >> 5] = keep;
+    t.sync();
+    const float *from = &scratch[up][t.team * t.warps];
+    const int w = t.lane & 15;
+    keep = (w < t.warps ? from[w] : 0.f) + (w + 16 < t.warps ? from[w + 16] : 0.f);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) keep += __shfl_xor_sync(0xffffffffu, keep, o);
+  }
+  const float other = __shfl_xor_sync(0xffffffffu, keep, 16);
+  return up ? make_float2(other, keep) : make_float2(keep, other);
+}
+__device__ __forceinline__ float ln_sum(float v, LnScratch &scratch, const LnTeam &t) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (t.warps > 1) {
+    if (t.lane == 0) scratch[0][threadIdx.x >> 5] = v;
+    t.sync();
+    v = t.lane < t.warps ? scratch[0][t.team * t.warps + t.lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   }
   return v;
 }
 
-// y = (x - mean) * rstd * gamma + beta.  The variance is that of the distances from a first mean, and what the first mean was
-// off by (the mean of those distances) is taken out of both: a large mean costs no digits.
-template <class T, class P, int V, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) layernorm_kernel(int64_t rows, int cols, float eps, const T *x, int64_t ldx,
-                                                                      const P *gamma, const P *beta, T *y, int64_t ldy,
-                                                                      float *mean, float *rstd) {
-  __shared__ float2 scratch[2][32];
-  const int share = WARP ? 32 : (int)blockDim.x, tid = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const int units = cols / V;
-  const float n = (float)cols;
-  const int64_t step = WARP ? (int64_t)gridDim.x * 8 : (int64_t)gridDim.x;
-  for (int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x; row < rows; row += step) {
-    LnPack<T, V> v[N];
-    const T *xr = x + row * ldx;
-    float s = 0.f;
+// Rows to come are fetched by cp.async, each thread's elements into places of its own, so that no barrier guards them:
+// `kLnAhead` rows besides the one in hand, or none where a block's memory does not hold them.  (FP16 and bf16 elements that
+// must be read one by one have no cp.async of their size and go through registers.)
+constexpr int kLnAhead = 2;
+__device__ __forceinline__ void ln_copy_async(void *smem, const void *global, int bytes) {
+  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void ln_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// y = (x - mean) * rstd * gamma + beta, E elements of the row per thread.  The variance is that of the distances from a first
+// mean, and what the first mean was off by (the mean of those distances) is taken out of both: a large mean costs no digits.
+template <class T, class P, int V, int E, int THREADS, bool FULL>
+__global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int cols, int share, int turns, int ahead, float eps, const T *x,
+                                                            int64_t ldx, const P *gamma, const P *beta, T *y, int64_t ldy, float *mean,
+                                                            float *rstd) {
+  using Pack = LnPack<T, V>;
+  using F = typename Pack::F;
+  constexpr int N = E / V, K = Pack::kParts;
+  constexpr bool RING = V * sizeof(T) >= 4, HOLD = E <= 16;       // HOLD: gamma and beta stay in registers over the rows
+  __shared__ LnScratch scratch[2];
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  const LnTeam t(share);
+  if (FULL) turns = N;
+  const int valid = FULL ? N : t.valid(cols / V, turns);
+  const int64_t col = (int64_t)t.unit(turns) * V;
+  const float inv = 1.f / (float)cols;
+  const T *px = x + t.first * ldx + col;                    // the next row to fetch
+  T *py = y + t.first * ldy + col;
+  const P *const pg = gamma ? gamma + col : nullptr, *const pb = beta ? beta + col : nullptr;
+  const int64_t x_step = t.step * ldx, y_step = t.step * ldy;
+  int64_t next = t.first;
+  // RING: [ahead + 1][warp][N][lane], so that a thread's accesses are a known distance apart
+  Pack *const ring = reinterpret_cast<Pack *>(dynamic) + (threadIdx.x >> 5) * 32 * N + t.lane;
+  const int slot = (int)blockDim.x * N;
+  Pack *fetched = ring, *in_hand = ring, *const ring_end = ring + (ahead + 1) * slot;
+  Pack v[N];
+  auto fetch = [&]() {
+    if (next < rows) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || i < valid) {
+          if constexpr (RING) ln_copy_async(fetched + i * 32, px + i * 32 * V, V * sizeof(T));
+          else v[i].load_stream(px + i * 32 * V);
+        }
+    }
+    if constexpr (RING) {
+      ln_commit();
+      fetched += slot;
+      if (fetched == ring_end) fetched = ring;
+    }
+    next += t.step;
+    px += x_step;
+  };
+  if constexpr (RING)
+    for (int i = 0; i < ahead; ++i) fetch();
+  F g[HOLD ? N : 1][K], b[HOLD ? N : 1][K];
+  if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) v[i].load_stream(xr + (int64_t)(tid + i * share) * V);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
-#pragma unroll
-        for (int k = 0; k < V; ++k) s += v[i].get(k);
+      if (FULL || i < valid) {
+        ln_params<P, V>(g[i], pg, i * 32 * V, 1.f);
+        ln_params<P, V>(b[i], pb, i * 32 * V, 0.f);
       }
-    float m = ln_sum2<WARP>(make_float2(s, 0.f), scratch[0]).x / n;
-    float2 d = make_float2(0.f, 0.f);
+  }
+  for (int64_t row = t.first; row < rows; row += t.step, py += y_step) {
+    fetch();
+    if constexpr (RING) {
+      if (ahead) ln_wait<kLnAhead>();
+      else ln_wait<0>();
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || i < valid) v[i] = in_hand[i * 32];
+      in_hand += slot;
+      if (in_hand == ring_end) in_hand = ring;
+    }
+    F f[N * K], s(0.f);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
+      if (FULL || i < valid) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float e = v[i].get(k) - m;
-          d.x += e;
-          d.y = fmaf(e, e, d.y);
+        for (int k = 0; k < K; ++k) {
+          f[i * K + k] = v[i].get(k);
+          s = s + f[i * K + k];
         }
       }
-    d = ln_sum2<WARP>(d, scratch[1]);
-    const float off = d.x / n;
+    float m = ln_sum(s.sum(), scratch[0], t) * inv;
+    F d1(0.f), d2(0.f);
+    const F less(-m);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (FULL || i < valid) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const F e = f[i * K + k] + less;
+          d1 = d1 + e;
+          d2 = ln_fma(e, e, d2);
+        }
+      }
+    const float2 d = ln_sum2(make_float2(d1.sum(), d2.sum()), scratch[1], t);
+    const float off = d.x * inv;
     m += off;
-    const float r = 1.f / sqrtf(fmaf(-off, off, d.y / n) + eps);
-    if (tid == 0) {
+    const float r = rsqrtf(fmaf(-off, off, d.y * inv) + eps);
+    if (t.tid == 0) {
       if (mean) mean[row] = m;
       if (rstd) rstd[row] = r;
     }
-    T *yr = y + row * ldy;
+    const F minus(-m), by(r);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
-        float g[V], b[V];
-        ln_params<P, V>(g, gamma, (int64_t)(tid + i * share) * V, 1.f);
-        ln_params<P, V>(b, beta, (int64_t)(tid + i * share) * V, 0.f);
+      if (FULL || i < valid) {
+        if constexpr (!HOLD) {
+          ln_params<P, V>(g[0], pg, i * 32 * V, 1.f);
+          ln_params<P, V>(b[0], pb, i * 32 * V, 0.f);
+        }
+        Pack out;
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[i].set(k, fmaf((v[i].get(k) - m) * r, g[k], b[k]));
-        v[i].store(yr + (int64_t)(tid + i * share) * V);
+        for (int k = 0; k < K; ++k) out.set(k, ln_fma((f[i * K + k] + minus) * by, g[HOLD ? i : 0][k], b[HOLD ? i : 0][k]));
+        out.store(py + i * 32 * V);
       }
   }
 }
@@ -148,148 +326,229 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) layernorm_kernel(int64_t ro
 template <class T, class P, int V>
 __global__ void __launch_bounds__(1024) layernorm_long_kernel(int64_t rows, int cols, float eps, const T *x, int64_t ldx, const P *gamma,
                                                               const P *beta, T *y, int64_t ldy, float *mean, float *rstd) {
-  __shared__ float2 scratch[2][32];
-  const float n = (float)cols;
+  using F = typename LnPack<T, V>::F;
+  constexpr int K = LnPack<T, V>::kParts;
+  __shared__ LnScratch scratch[2];
+  const LnTeam t(1024);
+  const float inv = 1.f / (float)cols;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T *xr = x + row * ldx;
     LnPack<T, V> v;
-    float s = 0.f;
+    F s(0.f);
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
       v.load(xr + i);
 #pragma unroll
-      for (int k = 0; k < V; ++k) s += v.get(k);
+      for (int k = 0; k < K; ++k) s = s + v.get(k);
     }
-    float m = ln_sum2<false>(make_float2(s, 0.f), scratch[0]).x / n;
-    float2 d = make_float2(0.f, 0.f);
+    float m = ln_sum(s.sum(), scratch[0], t) * inv;
+    F d1(0.f), d2(0.f);
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
       v.load(xr + i);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float e = v.get(k) - m;
-        d.x += e;
-        d.y = fmaf(e, e, d.y);
+      for (int k = 0; k < K; ++k) {
+        const F e = v.get(k) + F(-m);
+        d1 = d1 + e;
+        d2 = ln_fma(e, e, d2);
       }
     }
-    d = ln_sum2<false>(d, scratch[1]);
-    const float off = d.x / n;
+    const float2 d = ln_sum2(make_float2(d1.sum(), d2.sum()), scratch[1], t);
+    const float off = d.x * inv;
     m += off;
-    const float r = 1.f / sqrtf(fmaf(-off, off, d.y / n) + eps);
+    const float r = rsqrtf(fmaf(-off, off, d.y * inv) + eps);
     if (threadIdx.x == 0) {
       if (mean) mean[row] = m;
       if (rstd) rstd[row] = r;
     }
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
-      float g[V], b[V];
+      F g[K], b[K];
       v.load(xr + i);
-      ln_params<P, V>(g, gamma, i, 1.f);
-      ln_params<P, V>(b, beta, i, 0.f);
+      ln_params<P, V>(g, gamma, (int)i, 1.f);
+      ln_params<P, V>(b, beta, (int)i, 0.f);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v.set(k, fmaf((v.get(k) - m) * r, g[k], b[k]));
+      for (int k = 0; k < K; ++k) v.set(k, ln_fma((v.get(k) + F(-m)) * F(r), g[k], b[k]));
       v.store(y + row * ldy + i);
     }
   }
 }
 
-// Backward: a block (or each warp of one) walks over rows of its own with the next row's loads under way, and keeps the sums
-// dy * xhat and dy of its columns in registers over all of them; they end as one line of `partial` per block.
+// Backward: a team walks over its rows and keeps the sums dy * xhat and dy of its columns in registers over all of them; the
+// teams' sums end as one line of `partial` per block.
 //   xhat = (x - mean) * rstd,  u = dy * gamma,  dx = rstd * (u - sum(u) / n - xhat * sum(u * xhat) / n)
 // dx may be dy: a thread writes only what it has read.
-template <class T, class P, int V, int N, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) layernorm_backward_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x,
-                                                                               int64_t ldx, const P *gamma, const float *mean,
-                                                                               const float *rstd, T *dx, int64_t lddx,
-                                                                               float *partial) {
-  __shared__ float2 scratch[2][32];
-  extern __shared__ float joined[];                // WARP: [2][cols], the warps' sums
+template <class T, class P, int V, int E, bool FULL>
+__global__ void __launch_bounds__(512) layernorm_backward_kernel(int64_t rows, int cols, int share, int turns, const T *dy, int64_t lddy,
+                                                                 const T *x, int64_t ldx, const P *gamma, const float *mean,
+                                                                 const float *rstd, T *dx, int64_t lddx, float *partial) {
+  using Pack = LnPack<T, V>;
+  using F = typename Pack::F;
+  constexpr int N = E / V, K = Pack::kParts, W = Pack::W;
+  constexpr bool RING = V * sizeof(T) >= 4;
+  __shared__ LnScratch scratch[2];
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  float *const joined = reinterpret_cast<float *>(dynamic);                // at the end, with several teams: [2][cols]
   pdl_launch_dependents();
-  const int share = WARP ? 32 : (int)blockDim.x, tid = WARP ? (int)threadIdx.x & 31 : (int)threadIdx.x;
-  const int units = cols / V;
+  const LnTeam t(share);
+  if (FULL) turns = N;
+  // gamma in FP32, [warp of a team][access][16 bytes of it][lane]: read from memory, two 16-byte halves of every 32 bytes apart,
+  // it took as long as dy
+  constexpr int G = V >= 4 ? 4 : V;                                        // its elements per access to shared memory
+  using Gamma = LnPack<float, G>;
+  Gamma *const weights = reinterpret_cast<Gamma *>(dynamic + (RING ? (kLnAhead + 1) * 2 * N * sizeof(Pack) * blockDim.x : 0)) +
+                         (t.tid >> 5) * N * (V / G) * 32 + t.lane;
+  const int valid = FULL ? N : t.valid(cols / V, turns);
+  const int64_t col = (int64_t)t.unit(turns) * V;
   const float inv = 1.f / (float)cols;
-  const int64_t step = WARP ? (int64_t)gridDim.x * 8 : (int64_t)gridDim.x;
-  float dg[N * V] = {}, db[N * V] = {};
-  LnPack<T, V> xn[N], gn[N];
-  float mn = 0.f, rn = 0.f;
-  auto fetch = [&](int64_t row) {
+  F dg[N * K], db[N * K];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
-        xn[i].load_stream(x + row * ldx + (int64_t)(tid + i * share) * V);
-        gn[i].load_stream(dy + row * lddy + (int64_t)(tid + i * share) * V);
-      }
-    mn = mean[row];
-    rn = rstd[row];
+  for (int i = 0; i < N * K; ++i) dg[i] = F(0.f), db[i] = F(0.f);
+  const T *px = x + t.first * ldx + col, *pg = dy + t.first * lddy + col;  // the next row to fetch
+  const P *const pw = gamma ? gamma + col : nullptr;
+  T *to = dx + t.first * lddx + col;
+  const int64_t x_step = t.step * ldx, g_step = t.step * lddy, to_step = t.step * lddx;
+  int64_t next = t.first;
+  // RING: [kLnAhead + 1][warp][x, dy][N][lane]
+  Pack *const ring = reinterpret_cast<Pack *>(dynamic) + (threadIdx.x >> 5) * 64 * N + t.lane;
+  const int slot = (int)blockDim.x * 2 * N;
+  Pack *fetched = ring, *in_hand = ring, *const ring_end = ring + (kLnAhead + 1) * slot;
+  Pack xn[RING ? 1 : N], gn[RING ? 1 : N];
+  auto fetch = [&]() {
+    if (next < rows) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || i < valid) {
+          if constexpr (RING) {
+            ln_copy_async(fetched + i * 32, px + i * 32 * V, V * sizeof(T));
+            ln_copy_async(fetched + (N + i) * 32, pg + i * 32 * V, V * sizeof(T));
+          } else {
+            xn[i].load_stream(px + i * 32 * V);
+            gn[i].load_stream(pg + i * 32 * V);
+          }
+        }
+    }
+    if constexpr (RING) {
+      ln_commit();
+      fetched += slot;
+      if (fetched == ring_end) fetched = ring;
+    }
+    next += t.step;
+    px += x_step;
+    pg += g_step;
   };
-  int64_t row = WARP ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
-  if (row < rows) fetch(row);
-  for (int turn = 0; row < rows; row += step, turn ^= 1) {
-    LnPack<T, V> xc[N], gc[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) xc[i] = xn[i], gc[i] = gn[i];
-    const float m = mn, r = rn;
-    if (row + step < rows) fetch(row + step);
-    float2 s = make_float2(0.f, 0.f);
+  if (t.team == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
-        float g[V];
-        ln_params<P, V>(g, gamma, (int64_t)(tid + i * share) * V, 1.f);
+      if (FULL || i < valid) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float d = gc[i].get(k), h = (xc[i].get(k) - m) * r, u = d * g[k];
-          s.x += u;
-          s.y = fmaf(u, h, s.y);
-          dg[i * V + k] = fmaf(d, h, dg[i * V + k]);
-          db[i * V + k] += d;
+        for (int q = 0; q < V / G; ++q) {
+          Gamma w;
+#pragma unroll
+          for (int k = 0; k < G; ++k) w.e[k] = pw ? to_f32(pw[i * 32 * V + q * G + k]) : 1.f;
+          weights[(i * (V / G) + q) * 32] = w;
+        }
+      }
+  }
+  __syncthreads();
+  // mean and rstd of this team's next 32 rows, a row per lane
+  int64_t at = t.first + t.lane * t.step;
+  float mean32 = at < rows ? mean[at] : 0.f, rstd32 = at < rows ? rstd[at] : 0.f, mean_next = 0.f, rstd_next = 0.f;
+#pragma unroll
+  for (int i = 0; i < (RING ? kLnAhead : 1); ++i) fetch();
+  int turn = 0;
+  for (int64_t row = t.first; row < rows; row += t.step, to += to_step, ++turn) {
+    const float m = __shfl_sync(0xffffffffu, mean32, turn & 31), r = __shfl_sync(0xffffffffu, rstd32, turn & 31);
+    if ((turn & 31) == 16) {                       // the 32 after these, well before they are needed
+      at += 32 * t.step;
+      mean_next = at < rows ? mean[at] : 0.f;
+      rstd_next = at < rows ? rstd[at] : 0.f;
+    }
+    if ((turn & 31) == 31) mean32 = mean_next, rstd32 = rstd_next;
+    Pack xc[N], gc[N];
+    if constexpr (RING) {
+      fetch();      // into the place that the row before this one left
+      ln_wait<kLnAhead>();
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (FULL || i < valid) {
+          xc[i] = in_hand[i * 32];
+          gc[i] = in_hand[(N + i) * 32];
+        }
+      in_hand += slot;
+      if (in_hand == ring_end) in_hand = ring;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) xc[i] = xn[i], gc[i] = gn[i];
+      fetch();
+    }
+    // with c = x - mean:  sum(u * xhat) = rstd * sum(u * c),  dx = u * rstd + (c * (-rstd^2 * sum(u * xhat) / n) - rstd * sum(u) / n)
+    F c[N * K], u[N * K], s1(0.f), s2(0.f);
+    const F minus(-m), by(r);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (FULL || i < valid) {
+        F g[K];
+#pragma unroll
+        for (int q = 0; q < V / G; ++q) {
+          const Gamma w = weights[(i * (V / G) + q) * 32];
+#pragma unroll
+          for (int k = 0; k < Gamma::kParts; ++k) g[q * Gamma::kParts + k] = w.get(k);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int q = i * K + k;
+          const F d = gc[i].get(k);
+          c[q] = xc[i].get(k) + minus;
+          u[q] = d * g[k];
+          s1 = s1 + u[q];
+          s2 = ln_fma(u[q], c[q], s2);
+          dg[q] = ln_fma(d * by, c[q], dg[q]);
+          db[q] = db[q] + d;
         }
       }
     if (dx) {
-      s = ln_sum2<WARP>(s, scratch[turn]);
-      const float a = s.x * inv, b = s.y * inv;
+      const float2 s = ln_sum2(make_float2(s1.sum(), s2.sum()), scratch[turn & 1], t);
+      const F a(-r * (s.x * inv)), b(-(r * r) * (r * s.y * inv));
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (tid + i * share < units) {
-          float g[V];
-          ln_params<P, V>(g, gamma, (int64_t)(tid + i * share) * V, 1.f);
-          LnPack<T, V> out;
+        if (FULL || i < valid) {
+          Pack out;
 #pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float h = (xc[i].get(k) - m) * r, u = gc[i].get(k) * g[k];
-            out.set(k, r * (u - fmaf(h, b, a)));
-          }
-          out.store(dx + row * lddx + (int64_t)(tid + i * share) * V);
+          for (int k = 0; k < K; ++k) out.set(k, ln_fma(u[i * K + k], by, ln_fma(c[i * K + k], b, a)));
+          out.store(to + i * 32 * V);
         }
     }
   }
+  if constexpr (RING) ln_wait<0>();
   if (!partial) return;
   float *line = partial + (int64_t)blockIdx.x * 2 * cols;
-  if constexpr (!WARP) {
+  float *const sums = t.teams > 1 ? joined : line;
+  __syncthreads();                                   // the ring's memory is used again
+  for (int w = 0; w < t.teams; ++w) {                // team by team, in order
+    if (t.team == w) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (tid + i * share < units) {
+      for (int i = 0; i < N; ++i)
+        if (FULL || i < valid) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          line[(tid + i * share) * V + k] = dg[i * V + k];
-          line[cols + (tid + i * share) * V + k] = db[i * V + k];
-        }
-      }
-  } else {
-    for (int w = 0; w < 8; ++w) {                    // warp by warp, in order
-      if ((int)(threadIdx.x >> 5) == w) {
+          for (int k = 0; k < K; ++k) {
+            float two[2][2];
+            if constexpr (W == 2) {
+              const float2 p = dg[i * K + k].both(), q = db[i * K + k].both();
+              two[0][0] = p.x, two[0][1] = p.y, two[1][0] = q.x, two[1][1] = q.y;
+            } else {
+              two[0][0] = dg[i * K + k].v, two[1][0] = db[i * K + k].v;
+            }
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (tid + i * share < units) {
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-              const int c = (tid + i * share) * V + k;
-              joined[c] = w ? joined[c] + dg[i * V + k] : dg[i * V + k];
-              joined[cols + c] = w ? joined[cols + c] + db[i * V + k] : db[i * V + k];
+            for (int e = 0; e < W; ++e) {
+              const int c = (int)col + i * 32 * V + k * W + e;
+              sums[c] = w ? sums[c] + two[0][e] : two[0][e];
+              sums[cols + c] = w ? sums[cols + c] + two[1][e] : two[1][e];
             }
           }
-      }
-      __syncthreads();
+        }
     }
-    for (int c = threadIdx.x; c < 2 * cols; c += 256) line[c] = joined[c];
+    if (t.teams > 1) __syncthreads();
   }
+  if (t.teams > 1)
+    for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) line[c] = joined[c];
 }
 
 // Rows too long for that: their sums of u and u * xhat first (one block per row), then everything else by tiles of columns,
@@ -297,25 +556,28 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) layernorm_backward_kernel(i
 template <class T, class P, int V>
 __global__ void __launch_bounds__(1024) layernorm_row_sums_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x, int64_t ldx,
                                                                   const P *gamma, const float *mean, const float *rstd, float2 *out) {
-  __shared__ float2 scratch[2][32];
+  using F = typename LnPack<T, V>::F;
+  constexpr int K = LnPack<T, V>::kParts;
+  __shared__ LnScratch scratch[2];
+  const LnTeam t(1024);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const float m = mean[row], r = rstd[row];
-    float2 s = make_float2(0.f, 0.f);
+    F s1(0.f), s2(0.f);
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
       LnPack<T, V> xv, gv;
-      float g[V];
+      F g[K];
       xv.load(x + row * ldx + i);
       gv.load(dy + row * lddy + i);
-      ln_params<P, V>(g, gamma, i, 1.f);
+      ln_params<P, V>(g, gamma, (int)i, 1.f);
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float u = gv.get(k) * g[k];
-        s.x += u;
-        s.y = fmaf(u, (xv.get(k) - m) * r, s.y);
+      for (int k = 0; k < K; ++k) {
+        const F u = gv.get(k) * g[k];
+        s1 = s1 + u;
+        s2 = ln_fma(u, (xv.get(k) + F(-m)) * F(r), s2);
       }
     }
-    s = ln_sum2<false>(s, scratch[turn]);
+    const float2 s = ln_sum2(make_float2(s1.sum(), s2.sum()), scratch[turn], t);
     if (threadIdx.x == 0) out[row] = make_float2(s.x / (float)cols, s.y / (float)cols);
   }
 }
@@ -325,8 +587,12 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(int64_t rows, in
                                                                 const float2 *row_sums, T *dx, int64_t lddx, float *partial) {
   const int64_t c = ((int64_t)blockIdx.x * 128 + threadIdx.x) * V;
   if (c >= cols) return;
-  float g[V], dg[V] = {}, db[V] = {};
-  ln_params<P, V>(g, gamma, c, 1.f);
+  using F = typename LnPack<T, V>::F;
+  constexpr int K = LnPack<T, V>::kParts, W = LnPack<T, V>::W;
+  F g[K], dg[K], db[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) dg[k] = F(0.f), db[k] = F(0.f);
+  ln_params<P, V>(g, gamma, (int)c, 1.f);
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     LnPack<T, V> xv, gv;
     xv.load_stream(x + row * ldx + c);
@@ -334,18 +600,25 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(int64_t rows, in
     const float m = mean[row], r = rstd[row];
     const float2 s = dx ? row_sums[row] : make_float2(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float d = gv.get(k), h = (xv.get(k) - m) * r;
-      dg[k] = fmaf(d, h, dg[k]);
-      db[k] += d;
-      xv.set(k, r * (d * g[k] - fmaf(h, s.y, s.x)));
+    for (int k = 0; k < K; ++k) {
+      const F d = gv.get(k), h = (xv.get(k) + F(-m)) * F(r);
+      dg[k] = ln_fma(d, h, dg[k]);
+      db[k] = db[k] + d;
+      xv.set(k, F(r) * (d * g[k] + ln_fma(h, F(-s.y), F(-s.x))));
     }
     if (dx) xv.store(dx + row * lddx + c);
   }
   if (!partial) return;
   float *line = partial + (int64_t)blockIdx.y * 2 * cols + c;
 #pragma unroll
-  for (int k = 0; k < V; ++k) line[k] = dg[k], line[cols + k] = db[k];
+  for (int k = 0; k < K; ++k) {
+    if constexpr (W == 2) {
+      const float2 p = dg[k].both(), q = db[k].both();
+      line[2 * k] = p.x, line[2 * k + 1] = p.y, line[cols + 2 * k] = q.x, line[cols + 2 * k + 1] = q.y;
+    } else {
+      line[k] = dg[k].v, line[cols + k] = db[k].v;
+    }
+  }
 }
 
 // dgamma and dbeta from the lines of partial sums: 32 columns per block, the lines shared out over 32 warps and joined in order.
@@ -375,19 +648,10 @@ __global__ void __launch_bounds__(1024) layernorm_reduce_kernel(int parts, int c
 }
 
 // ---- which form -------------------------------------------------------------------------------------
-constexpr int kLnWarpCols = 1024;       // up to here a warp takes a row; backward, where a thread holds sums too, up to
-constexpr int kLnWarpColsBackward = 512;
-constexpr int kLnParts = 296;           // most lines of partial sums: two blocks on each of 148 SMs
-// Elements of a row that a thread holds, by the width of its accesses: enough that 1024 threads take 32768 columns forward
-// and 8192 backward (there the sums over rows are held too).
-constexpr int ln_held(int v) { return v == 1 ? 16 : 32; }
-constexpr int kLnHeldBackward = 8;
-static int ln_backward_longest() { return 1024 * kLnHeldBackward; }
-
-static int64_t ln_parts(int64_t rows, int64_t cols) {
-  const int64_t blocks = cols <= kLnWarpColsBackward ? (rows + 7) / 8 : rows;
-  return blocks < kLnParts ? blocks : kLnParts;
-}
+constexpr int kLnHeldBackward = 16;       // elements per thread, backward
+constexpr int kLnLongestBackward = 8192;  // 512 threads of 16 elements, or 1024 of 8
+constexpr int kLnParts = 296;           // most blocks, and lines of partial sums: two blocks on each of 148 SMs
+static int64_t ln_parts(int64_t rows) { return rows < kLnParts ? rows : kLnParts; }
 
 // Whether every address and pitch (in bytes) is a multiple of `bytes`; NULL is.
 static bool ln_multiple(int64_t bytes, std::initializer_list<const void *> pointers, std::initializer_list<int64_t> pitches) {
@@ -397,6 +661,33 @@ static bool ln_multiple(int64_t bytes, std::initializer_list<const void *> point
     if (p % bytes) return false;
   return true;
 }
+// Accesses per thread that take `units` of them over `share` threads.
+static int ln_turns(int64_t units, int share) { return (int)((units + share - 1) / share); }
+
+// Blocks of this size that an SM holds, asked once per kernel, size and device.
+static int ln_blocks_per_sm(const void *kernel, int device, int threads, size_t smem, int *out) {
+  struct Entry {
+    const void *kernel;
+    int device, threads;
+    size_t smem;
+    int blocks;
+  };
+  static std::vector<Entry> known;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lk(mu);
+  for (const Entry &e : known)
+    if (e.kernel == kernel && e.device == device && e.threads == threads && e.smem == smem) {
+      *out = e.blocks;
+      return B2_OK;
+    }
+  int n = 0;
+  B2_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem));
+  if (n < 1) n = 1;
+  known.push_back({kernel, device, threads, smem, n});
+  *out = n;
+  return B2_OK;
+}
+
 // The widest access, in elements, for rows of `cols` elements of `tb` bytes at these places; parameters of pb bytes are read
 // as many at a time (16 bytes at most).
 static int ln_width(int64_t cols, int tb, int pb, std::initializer_list<const void *> rows, std::initializer_list<int64_t> pitches,
@@ -441,41 +732,60 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
   B2_CONTEXT(ctx, h, "b2_layernorm");
   const int width = ln_width(cols, tb, pb, {x, y}, {ldx * tb, ldy * tb}, {gamma, beta});
   cudaStream_t s = (cudaStream_t)stream;
-  auto launch = [&](auto t, auto p) {
+  auto launch = [&](auto t, auto p) -> int {
     using T = decltype(t);
     using P = decltype(p);
+    int result = B2_OK;
     ln_with_width<T>(width, [&](auto w) {
-      constexpr int V = decltype(w)::value, kMost = ln_held(V) / V, kFew = kMost >= 4 ? kMost / 4 : 1;
-      const int64_t units = cols / V;
-      auto run = [&](auto kernel, int64_t blocks, int threads) {
-        const int64_t cap = (int64_t)1 << 30;
-        kernel<<<(unsigned)(blocks < cap ? blocks : cap), threads, 0, s>>>(rows, (int)cols, eps, (const T *)x, ldx, (const P *)gamma,
-                                                                          (const P *)beta, (T *)y, ldy, mean, rstd);
+      constexpr int V = decltype(w)::value;
+      // E elements per thread, teams of threads to a row in blocks of about 256
+      auto run = [&](auto elements, auto bound) {
+        constexpr int E = decltype(elements)::value, THREADS = decltype(bound)::value;
+        const int share = (int)((cols + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns(cols / V, share);
+        const bool full = turns == E / V && cols == (int64_t)share * E;
+        const auto kernel = full ? layernorm_kernel<T, P, V, E, THREADS, true> : layernorm_kernel<T, P, V, E, THREADS, false>;
+        const int64_t fit = share <= 256 ? 256 / share : 1;
+        const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
+        const size_t row_bytes = V * sizeof(T) >= 4 ? (size_t)threads * E * sizeof(T) : 0;
+        const int ahead = (kLnAhead + 1) * row_bytes <= 112 * 1024 ? kLnAhead : 0;
+        const int64_t blocks = (rows + teams - 1) / teams;
+        const int largest = (int)(THREADS * E * sizeof(T));
+        result = ensure_func_attributes((const void *)kernel, ctx->device, largest > 112 * 1024 ? largest : 112 * 1024);
+        if (result != B2_OK) return;
+        int64_t most = (int64_t)1 << 30;      // with rows fetched ahead: the blocks that the device holds at once
+        if (ahead && row_bytes) {
+          int held = 1;
+          result = ln_blocks_per_sm((const void *)kernel, ctx->device, threads, (ahead + 1) * row_bytes, &held);
+          if (result != B2_OK) return;
+          most = (int64_t)ctx->sm_count * held;
+        }
+        kernel<<<(unsigned)(blocks < most ? blocks : most), threads, (ahead + 1) * row_bytes, s>>>(
+            rows, (int)cols, share, turns, ahead, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
       };
-      // Few rows: as many threads to each as its length allows; else each thread holds as much as it can, and more rows share an SM.
-      const bool few = rows <= 2 * ctx->sm_count;
-      if (units <= 32 * kMost && cols <= kLnWarpCols && !(few && units > 32 * kFew)) {
-        if (units <= 32 * kFew) run(layernorm_kernel<T, P, V, kFew, true>, (rows + 7) / 8, 256);
-        else run(layernorm_kernel<T, P, V, kMost, true>, (rows + 7) / 8, 256);
-      } else if (units <= 1024 * kFew && (few || units <= 128 * kFew)) {
-        run(layernorm_kernel<T, P, V, kFew, false>, rows, (int)((units + 32 * kFew - 1) / (32 * kFew)) * 32);
-      } else if (units <= 1024 * kMost) {
-        run(layernorm_kernel<T, P, V, kMost, false>, rows, (int)((units + 32 * kMost - 1) / (32 * kMost)) * 32);
-      } else {
-        run(layernorm_long_kernel<T, P, V>, rows, 1024);
-      }
+      constexpr int kFew = V == 8 ? 8 : 4, kMost = 16, kLong = V == 1 ? 16 : 32;
+      using Half = std::integral_constant<int, 512>;
+      using Full = std::integral_constant<int, 1024>;
+      // Few rows: as many threads to each as its length allows.  Else each thread takes as much as it can hold: the fewer share
+      // a sum, the less it costs.
+      if (rows <= 2 * ctx->sm_count && cols <= 1024 * kFew) run(std::integral_constant<int, kFew>(), Full());
+      else if (cols <= 512 * kMost) run(std::integral_constant<int, kMost>(), Half());
+      else if (cols <= 1024 * kLong) run(std::integral_constant<int, kLong>(), Full());
+      else
+        layernorm_long_kernel<T, P, V><<<(unsigned)(rows < 1 << 30 ? rows : 1 << 30), 1024, 0, s>>>(
+            rows, (int)cols, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
     });
-    return 0;
+    return result;
   };
-  with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
+  const int st = with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
+  if (st != B2_OK) return st;
   B2_CUDA(cudaGetLastError());
   return B2_OK;
 }
 
 size_t b2_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const size_t sums = (size_t)ln_parts(rows, cols) * 2 * (size_t)cols * sizeof(float);
-  return (sums + 15) / 16 * 16 + (cols > ln_backward_longest() ? (size_t)rows * sizeof(float2) : 0);
+  const size_t sums = (size_t)ln_parts(rows) * 2 * (size_t)cols * sizeof(float);
+  return (sums + 15) / 16 * 16 + (cols > kLnLongestBackward ? (size_t)rows * sizeof(float2) : 0);
 }
 
 int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, const void *dy, int64_t lddy, const void *x,
@@ -504,7 +814,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
   }
   B2_REQUIRE((((uintptr_t)gamma | (uintptr_t)dgamma | (uintptr_t)dbeta) & (pb - 1)) == 0, B2_ERR_INVALID_ARG,
              "b2_layernorm_backward: gamma, dgamma or dbeta is not aligned to its element type");
-  const bool is_long = cols > ln_backward_longest();
+  const bool is_long = cols > kLnLongestBackward;
   const size_t need = sums || is_long ? b2_layernorm_backward_workspace_bytes(rows, cols) : 0;
   B2_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), B2_ERR_WORKSPACE,
              "b2_layernorm_backward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
@@ -516,39 +826,48 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
     if (dbeta) B2_CUDA(cudaMemsetAsync(dbeta, 0, (size_t)cols * pb, s));
     return B2_OK;
   }
-  (void)ctx;
-  const int parts = (int)ln_parts(rows, cols);
+  int parts = (int)ln_parts(rows);
   const int width = ln_width(cols, tb, pb, {dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : 0}, {gamma});
   float *partial = sums ? (float *)workspace : nullptr;
   float2 *row_sums = is_long ? (float2 *)((char *)workspace + (need - (size_t)rows * sizeof(float2))) : nullptr;
-  auto launch = [&](auto t, auto p) {
+  auto launch = [&](auto t, auto p) -> int {
     using T = decltype(t);
     using P = decltype(p);
+    int result = B2_OK;
     ln_with_width<T>(width, [&](auto w) {
-      constexpr int V = decltype(w)::value, kCta = V >= kLnHeldBackward ? 1 : kLnHeldBackward / V, kWarp = kLnWarpColsBackward / 32 / V,
-                    kFew = kWarp >= 4 ? kWarp / 4 : 1;
-      const int64_t units = cols / V;
-      auto run = [&](auto kernel, int threads, size_t smem) {
-        kernel<<<parts, threads, smem, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, (T *)dx,
-                                            lddx, partial);
-      };
-      if (cols <= kLnWarpColsBackward) {
-        const size_t smem = (size_t)2 * cols * sizeof(float);
-        if (units <= 32 * kFew) run(layernorm_backward_kernel<T, P, V, kFew, true>, 256, smem);
-        else run(layernorm_backward_kernel<T, P, V, kWarp, true>, 256, smem);
-      } else if (!is_long) {
-        run(layernorm_backward_kernel<T, P, V, kCta, false>, (int)((units + 32 * kCta - 1) / (32 * kCta)) * 32, 0);
+      constexpr int V = decltype(w)::value;
+      if (!is_long) {
+        // E elements per thread, and teams of threads to a row in blocks of about 256
+        auto run = [&](auto elements) {
+          constexpr int E = decltype(elements)::value;
+          const int share = (int)((cols + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns(cols / V, share);
+          const bool full = turns == E / V && cols == (int64_t)share * E;
+          const auto kernel = full ? layernorm_backward_kernel<T, P, V, E, true> : layernorm_backward_kernel<T, P, V, E, false>;
+          const int64_t fit = share <= 256 ? 256 / share : 1;
+          const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
+          if ((rows + teams - 1) / teams < parts) parts = (int)((rows + teams - 1) / teams);
+          size_t smem = V * sizeof(T) >= 4 ? (size_t)(kLnAhead + 1) * 2 * E * sizeof(T) * threads : 0;
+          smem += (size_t)share * E * sizeof(float);       // gamma
+          if (teams > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
+          result = ensure_func_attributes((const void *)kernel, ctx->device, ((kLnAhead + 1) * 2 * sizeof(T) + sizeof(float)) * E * 512);
+          if (result != B2_OK) return;
+          kernel<<<parts, threads, smem, s>>>(rows, (int)cols, share, turns, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd,
+                                              (T *)dx, lddx, partial);
+        };
+        // 16-bit elements one by one: what is fetched ahead takes registers too
+        if (V == 1 && sizeof(T) == 2 && cols <= 512 * 8) run(std::integral_constant<int, (V == 1 && sizeof(T) == 2 ? 8 : kLnHeldBackward)>());
+        else run(std::integral_constant<int, kLnHeldBackward>());
       } else {
         if (dx) {
           const int64_t blocks = rows < 1 << 30 ? rows : 1 << 30;
           layernorm_row_sums_kernel<T, P, V><<<(unsigned)blocks, 1024, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx,
                                                                             (const P *)gamma, mean, rstd, row_sums);
         }
-        layernorm_columns_kernel<T, P, V><<<dim3((unsigned)((units + 127) / 128), (unsigned)parts), 128, 0, s>>>(
+        layernorm_columns_kernel<T, P, V><<<dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
       }
     });
-    if (sums) {
+    if (result == B2_OK && sums) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)((cols + 31) / 32));
       cfg.blockDim = dim3(1024);
@@ -558,11 +877,12 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
       attr[0].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      return (int)cudaLaunchKernelEx(&cfg, layernorm_reduce_kernel<P>, parts, (int)cols, (const float *)partial, (P *)dgamma, (P *)dbeta);
+      B2_CUDA(cudaLaunchKernelEx(&cfg, layernorm_reduce_kernel<P>, parts, (int)cols, (const float *)partial, (P *)dgamma, (P *)dbeta));
     }
-    return 0;
+    return result;
   };
-  with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
+  const int st = with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
+  if (st != B2_OK) return st;
   B2_CUDA(cudaGetLastError());
   return B2_OK;
 }
