@@ -195,6 +195,37 @@ __device__ __forceinline__ float ln_sum(float v, LnScratch &scratch, const LnTea
   return v;
 }
 
+// A parameter vector in FP32 in shared memory, [warp of a team][access][16 bytes of it][lane]: read from memory, two 16-byte
+// halves of every 32 bytes apart, gamma and beta together took as long as x and y.
+template <int V, int N>
+struct LnWeights {
+  static constexpr int G = V >= 4 ? 4 : V;      // elements per access
+  using Pack = LnPack<float, G>;
+  Pack *at;
+  __device__ __forceinline__ LnWeights(float *base, const LnTeam &t)
+      : at(reinterpret_cast<Pack *>(base) + (t.tid >> 5) * N * (V / G) * 32 + t.lane) {}
+  template <class P>
+  __device__ __forceinline__ void put(const P *p, int valid, float without) {
+    for (int i = 0; i < valid; ++i) {
+#pragma unroll
+      for (int q = 0; q < V / G; ++q) {
+        Pack w;
+#pragma unroll
+        for (int k = 0; k < G; ++k) w.e[k] = p ? to_f32(p[i * 32 * V + q * G + k]) : without;
+        at[(i * (V / G) + q) * 32] = w;
+      }
+    }
+  }
+  __device__ __forceinline__ void get(LnF<(V >= 2 ? 2 : 1)> (&v)[V >= 2 ? V / 2 : 1], int i) const {
+#pragma unroll
+    for (int q = 0; q < V / G; ++q) {
+      const Pack w = at[(i * (V / G) + q) * 32];
+#pragma unroll
+      for (int k = 0; k < Pack::kParts; ++k) v[q * Pack::kParts + k] = w.get(k);
+    }
+  }
+};
+
 // Rows to come are fetched by cp.async, each thread's elements into places of its own, so that no barrier guards them:
 // `kLnAhead` rows besides the one in hand, or none where a block's memory does not hold them.  (FP16 and bf16 elements that
 // must be read one by one have no cp.async of their size and go through registers.)
@@ -218,7 +249,9 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
   using Pack = LnPack<T, V>;
   using F = typename Pack::F;
   constexpr int N = E / V, K = Pack::kParts;
-  constexpr bool RING = V * sizeof(T) >= 4, HOLD = E <= 16;       // HOLD: gamma and beta stay in registers over the rows
+  constexpr bool RING = V * sizeof(T) >= 4;
+  // gamma and beta: in registers over the rows, in shared memory, or (the longest rows) read again for each row
+  constexpr bool HOLD = E <= 16, SHARED = !HOLD && THREADS <= 512;
   __shared__ LnScratch scratch[2];
   extern __shared__ __align__(16) unsigned char dynamic[];
   const LnTeam t(share);
@@ -256,6 +289,16 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
   if constexpr (RING)
     for (int i = 0; i < ahead; ++i) fetch();
   F g[HOLD ? N : 1][K], b[HOLD ? N : 1][K];
+  using Weights = LnWeights<V, N>;
+  float *const shared_params = reinterpret_cast<float *>(dynamic + (RING ? (ahead + 1) * slot * sizeof(Pack) : 0));
+  Weights weights_g(shared_params, t), weights_b(shared_params + share * E, t);
+  if constexpr (SHARED) {
+    if (t.team == 0) {
+      weights_g.template put<P>(pg, valid, 1.f);
+      weights_b.template put<P>(pb, valid, 0.f);
+    }
+    __syncthreads();
+  }
   if constexpr (HOLD) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -267,7 +310,8 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
   for (int64_t row = t.first; row < rows; row += t.step, py += y_step) {
     fetch();
     if constexpr (RING) {
-      if (ahead) ln_wait<kLnAhead>();
+      if (ahead == 2) ln_wait<2>();
+      else if (ahead == 1) ln_wait<1>();
       else ln_wait<0>();
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -310,7 +354,10 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (FULL || i < valid) {
-        if constexpr (!HOLD) {
+        if constexpr (SHARED) {
+          weights_g.get(g[0], i);
+          weights_b.get(b[0], i);
+        } else if constexpr (!HOLD) {
           ln_params<P, V>(g[0], pg, i * 32 * V, 1.f);
           ln_params<P, V>(b[0], pb, i * 32 * V, 0.f);
         }
@@ -389,12 +436,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(int64_t rows, i
   pdl_launch_dependents();
   const LnTeam t(share);
   if (FULL) turns = N;
-  // gamma in FP32, [warp of a team][access][16 bytes of it][lane]: read from memory, two 16-byte halves of every 32 bytes apart,
-  // it took as long as dy
-  constexpr int G = V >= 4 ? 4 : V;                                        // its elements per access to shared memory
-  using Gamma = LnPack<float, G>;
-  Gamma *const weights = reinterpret_cast<Gamma *>(dynamic + (RING ? (kLnAhead + 1) * 2 * N * sizeof(Pack) * blockDim.x : 0)) +
-                         (t.tid >> 5) * N * (V / G) * 32 + t.lane;
+  LnWeights<V, N> weights(reinterpret_cast<float *>(dynamic + (RING ? (kLnAhead + 1) * 2 * N * sizeof(Pack) * blockDim.x : 0)), t);
   const int valid = FULL ? N : t.valid(cols / V, turns);
   const int64_t col = (int64_t)t.unit(turns) * V;
   const float inv = 1.f / (float)cols;
@@ -434,19 +476,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(int64_t rows, i
     px += x_step;
     pg += g_step;
   };
-  if (t.team == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (FULL || i < valid) {
-#pragma unroll
-        for (int q = 0; q < V / G; ++q) {
-          Gamma w;
-#pragma unroll
-          for (int k = 0; k < G; ++k) w.e[k] = pw ? to_f32(pw[i * 32 * V + q * G + k]) : 1.f;
-          weights[(i * (V / G) + q) * 32] = w;
-        }
-      }
-  }
+  if (t.team == 0) weights.template put<P>(pw, valid, 1.f);
   __syncthreads();
   // mean and rstd of this team's next 32 rows, a row per lane
   int64_t at = t.first + t.lane * t.step;
@@ -486,12 +516,7 @@ __global__ void __launch_bounds__(512) layernorm_backward_kernel(int64_t rows, i
     for (int i = 0; i < N; ++i)
       if (FULL || i < valid) {
         F g[K];
-#pragma unroll
-        for (int q = 0; q < V / G; ++q) {
-          const Gamma w = weights[(i * (V / G) + q) * 32];
-#pragma unroll
-          for (int k = 0; k < Gamma::kParts; ++k) g[q * Gamma::kParts + k] = w.get(k);
-        }
+        weights.get(g, i);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const int q = i * K + k;
@@ -648,6 +673,7 @@ __global__ void __launch_bounds__(1024) layernorm_reduce_kernel(int parts, int c
 }
 
 // ---- which form -------------------------------------------------------------------------------------
+constexpr int kLnBlock = 384;           // threads of a block of several teams, forward
 constexpr int kLnHeldBackward = 16;       // elements per thread, backward
 constexpr int kLnLongestBackward = 8192;  // 512 threads of 16 elements, or 1024 of 8
 constexpr int kLnParts = 296;           // most blocks, and lines of partial sums: two blocks on each of 148 SMs
@@ -744,30 +770,32 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
         const int share = (int)((cols + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns(cols / V, share);
         const bool full = turns == E / V && cols == (int64_t)share * E;
         const auto kernel = full ? layernorm_kernel<T, P, V, E, THREADS, true> : layernorm_kernel<T, P, V, E, THREADS, false>;
-        const int64_t fit = share <= 256 ? 256 / share : 1;
+        const int64_t fit = share <= kLnBlock ? kLnBlock / share : 1;
         const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
         const size_t row_bytes = V * sizeof(T) >= 4 ? (size_t)threads * E * sizeof(T) : 0;
-        const int ahead = (kLnAhead + 1) * row_bytes <= 112 * 1024 ? kLnAhead : 0;
+        const size_t params = E > 16 && THREADS <= 512 ? (size_t)2 * share * E * sizeof(float) : 0;
+        // rows ahead: two, or as many as leave room for two blocks on an SM, or for one
+        int ahead = kLnAhead;
+        while (ahead > 0 && (ahead + 1) * row_bytes + params > 112 * 1024) --ahead;
+        if (ahead == 0)
+          for (ahead = kLnAhead; ahead > 0 && (ahead + 1) * row_bytes + params > 224 * 1024;) --ahead;
+        const size_t smem = (ahead + 1) * row_bytes + params;
         const int64_t blocks = (rows + teams - 1) / teams;
-        const int largest = (int)(THREADS * E * sizeof(T));
-        result = ensure_func_attributes((const void *)kernel, ctx->device, largest > 112 * 1024 ? largest : 112 * 1024);
+        result = ensure_func_attributes((const void *)kernel, ctx->device, 224 * 1024);
         if (result != B2_OK) return;
-        int64_t most = (int64_t)1 << 30;      // with rows fetched ahead: the blocks that the device holds at once
-        if (ahead && row_bytes) {
-          int held = 1;
-          result = ln_blocks_per_sm((const void *)kernel, ctx->device, threads, (ahead + 1) * row_bytes, &held);
-          if (result != B2_OK) return;
-          most = (int64_t)ctx->sm_count * held;
-        }
-        kernel<<<(unsigned)(blocks < most ? blocks : most), threads, (ahead + 1) * row_bytes, s>>>(
+        int held = 1;      // the blocks that the device holds at once walk over all rows
+        result = ln_blocks_per_sm((const void *)kernel, ctx->device, threads, smem, &held);
+        if (result != B2_OK) return;
+        const int64_t most = (int64_t)ctx->sm_count * held;
+        kernel<<<(unsigned)(blocks < most ? blocks : most), threads, smem, s>>>(
             rows, (int)cols, share, turns, ahead, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
       };
-      constexpr int kFew = V == 8 ? 8 : 4, kMost = 16, kLong = V == 1 ? 16 : 32;
+      constexpr int kFew = V == 8 ? 8 : 4, kMost = V >= 4 ? 32 : 16, kLong = V == 1 ? 16 : 32;
       using Half = std::integral_constant<int, 512>;
       using Full = std::integral_constant<int, 1024>;
-      // Few rows: as many threads to each as its length allows.  Else each thread takes as much as it can hold: the fewer share
-      // a sum, the less it costs.
-      if (rows <= 2 * ctx->sm_count && cols <= 1024 * kFew) run(std::integral_constant<int, kFew>(), Full());
+      // Few rows: as many threads to each as its length allows; rows so short that a warp has enough with a few elements per
+      // thread likewise.  Else each thread takes as much as it can hold: the fewer share a sum, the less it costs.
+      if ((rows <= 2 * ctx->sm_count && cols <= 1024 * kFew) || cols <= 32 * kFew) run(std::integral_constant<int, kFew>(), Full());
       else if (cols <= 512 * kMost) run(std::integral_constant<int, kMost>(), Half());
       else if (cols <= 1024 * kLong) run(std::integral_constant<int, kLong>(), Full());
       else
