@@ -19,13 +19,15 @@ __device__ __forceinline__ float w4_warp_max(float v) {
 
 // The integer nearest to w / s for s > 0, ties to even, as a float.  The quotient in FP32 names a candidate that is at most
 // one off; the candidate's remainder, which an FMA leaves exact near a border, says whether a neighbour is nearer.  `inv` is
-// 1 / s (finite: see w4_prescale).
-__device__ __forceinline__ float w4_nearest(float w, float s, float inv) {
-  float q = rintf(fminf(fmaxf(w * inv, -40.f), 40.f));
-  const float r = fmaf(-q, s, w), half = 0.5f * s;
-  const bool odd = ((int)q) & 1;
-  if (r > half || (r == half && odd)) q += 1.f;
-  else if (r < -half || (r == -half && odd)) q -= 1.f;
+// 1 / s (finite: see w4_prescale), `half` is s / 2.  Adding and taking away 1.5 * 2^23 rounds to an even integer as rintf does,
+// and leaves the integer's parity in the lowest bit of the sum.
+__device__ __forceinline__ float w4_nearest(float w, float s, float half, float inv) {
+  const float big = fminf(fmaxf(w * inv, -40.f), 40.f) + 12582912.f;
+  const float q = big - 12582912.f, r = fmaf(-q, s, w);
+  if (fabsf(r) < half) return q;
+  const bool odd = __float_as_uint(big) & 1u;
+  if (r > half || (r == half && odd)) return q + 1.f;
+  if (r < -half || (r == -half && odd)) return q - 1.f;
   return q;
 }
 // A power of two that keeps the reciprocal of a tiny scale finite and its half exact; weights of such a group are at most
@@ -60,65 +62,192 @@ __device__ __forceinline__ S w4_scale(float lo, float hi, bool with_zeros) {
   return from_f32<S>(fminf(s, w4_largest<S>()));
 }
 
-// One warp per group, a byte (two codes) per lane and turn.
-template <class T, class S>
-__global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, int group, const T *W, int64_t ldw, uint8_t *codes,
-                                                          int64_t ldq, S *scales, uint8_t *zeros) {
-  const int64_t groups = (K + group - 1) / group;
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t at = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); at < N * groups; at += warps) {
-    const int64_t n = at / groups, k0 = (at - n * groups) * group;
-    const int len = (int)(K - k0 < group ? K - k0 : group);
-    const T *w = W + n * ldw + k0;
-    float lo = 0.f, hi = 0.f;
-    bool bad = false;
-    for (int i = lane; i < len; i += 32) {
-      const float v = to_f32(w[i]);
-      lo = fminf(lo, v);
-      hi = fmaxf(hi, v);
-      bad |= !isfinite(v);
-    }
-    hi = w4_warp_max(hi);
-    lo = -w4_warp_max(-lo);
-    bad = __any_sync(0xffffffffu, bad);
-    const S stored = bad ? from_f32<S>(__int_as_float(0x7fffffff)) : w4_scale<S>(lo, hi, zeros != nullptr);
-    const float scale = to_f32(stored);
-    const bool flat = !(scale > 0.f);   // 0, or NaN: every code is the zero point
-    const float f = w4_prescale(scale), s = scale * f, inv = 1.f / s;
-    float zero = 8.f;
-    if (zeros && !flat) zero = fminf(fmaxf(w4_nearest(-lo * f, s, inv), 0.f), 15.f);
-    const float lowest = zeros ? 0.f : 1.f;
-    if (lane == 0) {
-      scales[at] = stored;
-      if (zeros) zeros[at] = (uint8_t)zero;
-    }
-    for (int b = lane; 2 * b < len; b += 32) {
-      int c[2] = {(int)zero, 2 * b + 1 < len ? (int)zero : 0};
+// V elements in order as FP32 (V a multiple of 2; one access of 16 bytes per 16 / sizeof(T) of them).
+template <class T, int V>
+__device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
+  constexpr int PER = 16 / (int)sizeof(T);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (!flat && 2 * b + e < len)
-          c[e] = (int)fminf(fmaxf(w4_nearest(to_f32(w[2 * b + e]) * f, s, inv) + zero, lowest), 15.f);
-      codes[n * ldq + (k0 >> 1) + b] = (uint8_t)(c[0] | (c[1] << 4));
+  for (int i = 0; i < V; i += PER) {
+    union {
+      uint4 q;
+      T e[PER];
+    } u;
+    u.q = __ldcs(reinterpret_cast<const uint4 *>(p + i));
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[i + k] = to_f32(u.e[k]);
+  }
+}
+
+// Quantising is bound by reading W.  group / 16 lanes share a group, 16 elements (8 bytes of codes) each: a group's extremes take
+// log2(group / 16) shuffles, and a warp reads 512 elements in a row.  Without a place to start on 16 bytes (VEC = false: odd
+// pitches, shifted bases) the elements come one by one, and the codes of 8 bytes go out as bytes.
+template <class T, class S, bool VEC>
+__global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, int group_shift, const T *W, int64_t ldw, uint8_t *codes,
+                                                          int64_t ldq, S *scales, uint8_t *zeros) {
+  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
+  const int lanes = 1 << (group_shift - 4);                               // of a group: 2, 4, 8, 16
+  const int64_t row_units = groups << (group_shift - 4);                  // units of 16 elements, whole groups
+  // blockDim.x threads to a row (a power of two, not less than a group's lanes), blockDim.y rows to a block; all threads of a
+  // block take every turn, so that shuffles see every lane
+  for (int64_t nb = (int64_t)blockIdx.y * blockDim.y; nb < N; nb += (int64_t)gridDim.y * blockDim.y) {
+    const int64_t n = nb + threadIdx.y;
+    for (int64_t ub = (int64_t)blockIdx.x * blockDim.x; ub < row_units; ub += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t u = ub + threadIdx.x, k0 = u * 16;
+      const int64_t left = n < N ? K - k0 : 0;
+      const int len = left >= 16 ? 16 : left > 0 ? (int)left : 0;
+      const T *w = W + n * ldw + k0;
+      float v[16];
+      if (VEC && len == 16) {
+        w4_load<T, 16>(v, w);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = i < len ? to_f32(w[i]) : 0.f;
+      }
+      float lo = 0.f, hi = 0.f, sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        lo = fminf(lo, v[i]);
+        hi = fmaxf(hi, v[i]);
+        sum += v[i] * 0.f;                                                // 0, or NaN from an infinity or a NaN
+      }
+      for (int o = 1; o < lanes; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      if (len <= 0) continue;                                             // nothing to write; a group's first lane has elements
+      const bool bad = sum != 0.f;                                        // true for NaN
+      const S stored = bad ? from_f32<S>(__int_as_float(0x7fffffff)) : w4_scale<S>(lo, hi, zeros != nullptr);
+      const float scale = to_f32(stored);
+      const bool flat = !(scale > 0.f);                                   // 0, or NaN: every code is the zero point
+      const float f = w4_prescale(scale), s = scale * f, inv = 1.f / s, half = 0.5f * s;
+      float zero = 8.f;
+      if (zeros && !flat) zero = fminf(fmaxf(w4_nearest(-lo * f, s, half, inv), 0.f), 15.f);
+      const float lowest = zeros ? 0.f : 1.f;
+      if ((u & (lanes - 1)) == 0) {
+        const int64_t at = n * groups + (u >> (group_shift - 4));
+        scales[at] = stored;
+        if (zeros) zeros[at] = (uint8_t)zero;
+      }
+      uint32_t out[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float c = flat ? zero : fminf(fmaxf(w4_nearest(v[i] * f, s, half, inv) + zero, lowest), 15.f);
+        // as an integer in the low bits of 2^23 + c
+        const uint32_t bits = __float_as_uint(c + 8388608.f) & 15u;
+        out[i >> 3] |= (i < len ? bits : 0u) << (4 * (i & 7));
+      }
+      uint8_t *to = codes + n * ldq + (k0 >> 1);
+      if (VEC && len == 16) {
+        *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
+      } else {
+        for (int i = 0; 2 * i < len; ++i) to[i] = (uint8_t)(out[i >> 2] >> (8 * (i & 3)));
+      }
     }
   }
 }
 
 __device__ __forceinline__ float w4_zero(const uint8_t *zeros, int64_t at) { return zeros ? (float)(zeros[at] & 15) : 8.f; }
 
-// One thread per element, in the order of the output.
-template <class T, class S>
-__global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K, int group, const uint8_t *codes, int64_t ldq,
-                                                            const S *scales, const uint8_t *zeros, T *W, int64_t ldw,
-                                                            int transpose) {
-  const int64_t groups = (K + group - 1) / group;
-  const int64_t step = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < N * K; i += step) {
-    const int64_t a = transpose ? i / N : i / K, b = i - a * (transpose ? N : K);
-    const int64_t n = transpose ? b : a, k = transpose ? a : b;
-    const int c = (codes[n * ldq + (k >> 1)] >> (4 * (k & 1))) & 15;
-    const int64_t g = n * groups + k / group;
-    W[a * ldw + b] = from_f32<T>(((float)c - w4_zero(zeros, g)) * to_f32(scales[g]));
+// 8 codes of a word, times (scale) after the zero point is taken off, as 8 elements of T.
+template <class T>
+struct W4Out {
+  T e[8];
+};
+template <class T>
+__device__ __forceinline__ void w4_expand(W4Out<T> &out, uint32_t word, float scale, float zero) {
+  // a code in the low bits of 2^23 reads 2^23 + c; the difference with 2^23 + z is exact
+  const float base = 8388608.f + zero;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    out.e[i] = from_f32<T>((__uint_as_float(((word >> (4 * i)) & 15u) | 0x4b000000u) - base) * scale);
+}
+
+// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements; VEC where words of codes
+// and 16 bytes of W start on their own size.
+template <class T, class S, bool VEC>
+__global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
+                                                            const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
+  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift, units = (K + 7) >> 3;
+  for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
+    for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t k0 = u * 8, g = n * groups + (k0 >> group_shift);
+      const int len = K - k0 < 8 ? (int)(K - k0) : 8;
+      const uint8_t *from = codes + n * ldq + 4 * u;
+      uint32_t word = 0;
+      if (VEC && len == 8) {
+        word = __ldcs(reinterpret_cast<const uint32_t *>(from));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (2 * i < len) word |= (uint32_t)from[i] << (8 * i);
+      }
+      W4Out<T> out;
+      w4_expand(out, word, to_f32(scales[g]), w4_zero(zeros, g));
+      T *to = W + n * ldw + k0;
+      if (VEC && len == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4 *>(to) + i, reinterpret_cast<const uint4 *>(out.e)[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < len) to[i] = out.e[i];
+      }
+    }
+  }
+}
+
+// Transposed: tiles of 64 rows n x 64 of k through shared memory, so that codes are read along k and W is written along n.
+// A thread expands 16 codes (8 bytes) of one row into a column of the tile; a row of the tile goes out as 64 elements along n.
+// The tile's rows are 65 words apart (FP32; two 16-bit elements share a word in pairs of rows otherwise wasted): threads of a
+// warp that write 16 different rows of one k meet in different banks.
+template <class T, class S, bool VEC>
+__global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
+                                                           const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
+  __shared__ float tile[64][65];                // [k][n]
+  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
+  const int64_t k_tiles = (K + 63) >> 6, n_tiles = (N + 63) >> 6;
+  for (int64_t at = blockIdx.x; at < k_tiles * n_tiles; at += gridDim.x) {
+    const int64_t n0 = (at % n_tiles) * 64, k0 = (at / n_tiles) * 64;
+    {
+      // thread: row threadIdx.x / 4, 16 codes from (threadIdx.x % 4) * 16 on
+      const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+      const int64_t n = n0 + r, k = k0 + c;
+      uint32_t word[2] = {0, 0};
+      float scale = 0.f, zero = 0.f;
+      if (n < N && k < K) {
+        const uint8_t *from = codes + n * ldq + (k >> 1);
+        if (VEC && k + 16 <= K) {
+          const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(from));
+          word[0] = v.x, word[1] = v.y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (k + 2 * i < K) word[i >> 2] |= (uint32_t)from[i] << (8 * (i & 3));
+        }
+        const int64_t g = n * groups + (k >> group_shift);
+        scale = to_f32(scales[g]);
+        zero = w4_zero(zeros, g);
+      }
+      const float base = 8388608.f + zero;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        tile[c + i][r] = (__uint_as_float(((word[i >> 3] >> (4 * (i & 7))) & 15u) | 0x4b000000u) - base) * scale;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t k = k0 + warp * 8 + i;
+      if (k < K) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t n = n0 + h * 32 + lane;
+          if (n < N) W[k * ldw + n] = from_f32<T>(tile[warp * 8 + i][h * 32 + lane]);
+        }
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -788,6 +917,21 @@ static int w4_check(const char *who, int64_t N, int64_t K, int group, int type, 
   return B2_OK;
 }
 
+static int w4_group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8; }
+
+// Blocks of 256 threads over `units` of a row (x) and the rows (y): as many threads to a row, in powers of two, as it has units
+// (at least `least`), the others to further rows.
+struct W4Grid {
+  dim3 grid, block;
+  W4Grid(int64_t units, int64_t rows, int least) {
+    int x = least;
+    while (x < 256 && x < units) x *= 2;
+    block = dim3(x, 256 / x);
+    const int64_t gx = (units + x - 1) / x, gy = (rows + block.y - 1) / block.y;
+    grid = dim3((unsigned)(gx < 1 << 20 ? gx : 1 << 20), (unsigned)(gy < 65535 ? gy : 65535));
+  }
+};
+
 template <class F>
 static void w4_with_types(int type, int scale_type, F &&f) {
   with_type(type, [&](auto t) { return with_type(scale_type, [&](auto s) { f(t, s); return 0; }); });
@@ -810,12 +954,16 @@ int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const
   B2_REQUIRE(!matrices_overlap(W, N, K * tb, ldw * tb, codes, N, (K + 1) / 2, ldq), B2_ERR_INVALID_ARG,
              "b2_w4_quantize: codes overlap W");
   B2_CONTEXT(ctx, h, "b2_w4_quantize");
-  const int64_t need = (N * ((K + group - 1) / group) + 7) / 8, cap = (int64_t)ctx->sm_count * 16;
-  const int grid = (int)(need < cap ? need : cap);
+  (void)ctx;
+  const int shift = w4_group_shift(group);
+  const int64_t units = ((K + group - 1) / group) * (group / 16);
+  const W4Grid g(units, N, group / 16);
+  const bool vec = (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0 && (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
-    w4_quantize_kernel<T, S><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, group, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
+    if (vec) w4_quantize_kernel<T, S, true><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
+    else w4_quantize_kernel<T, S, false><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
   });
   B2_CUDA(cudaGetLastError());
   return B2_OK;
@@ -833,13 +981,22 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
   B2_REQUIRE(!matrices_overlap(W, transpose ? K : N, (transpose ? N : K) * tb, ldw * tb, codes, N, (K + 1) / 2, ldq), B2_ERR_INVALID_ARG,
              "b2_w4_dequantize: W overlaps the codes");
   B2_CONTEXT(ctx, h, "b2_w4_dequantize");
-  const int64_t need = (N * K + 255) / 256, cap = (int64_t)ctx->sm_count * 32;
-  const int grid = (int)(need < cap ? need : cap);
+  const int shift = w4_group_shift(group);
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
-    w4_dequantize_kernel<T, S><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, group, codes, ldq, (const S *)scales, zeros, (T *)W, ldw,
-                                                                      transpose);
+    if (transpose) {
+      const int64_t tiles = ((N + 63) / 64) * ((K + 63) / 64), most = (int64_t)ctx->sm_count * 64;
+      const unsigned grid = (unsigned)(tiles < most ? tiles : most);
+      const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
+      if (vec) w4_transpose_kernel<T, S, true><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      else w4_transpose_kernel<T, S, false><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+    } else {
+      const W4Grid g((K + 7) / 8, N, 1);
+      const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 3) == 0 && (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0;
+      if (vec) w4_dequantize_kernel<T, S, true><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      else w4_dequantize_kernel<T, S, false><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+    }
   });
   B2_CUDA(cudaGetLastError());
   return B2_OK;
@@ -874,7 +1031,7 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   MvArgs a = {};
   a.N = N, a.K = alpha != 0.f ? K : 0, a.ldx = ldx, a.ldq = ldq, a.ldy = ldy, a.groups = (K + group - 1) / group;
   a.M = (int)M, a.type = type, a.scale_type = scale_type, a.alpha = alpha, a.beta = beta;
-  a.group_shift = group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : 8;
+  a.group_shift = w4_group_shift(group);
   a.x = x, a.codes = codes, a.zeros = zeros, a.scales = scales, a.y = y;
   const int nb = mv_blocks(M, type);
   a.parts = mv_parts(type);
