@@ -16,6 +16,43 @@ __device__ __forceinline__ float w4_warp_max(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
+// The larger and the smaller of two, NaN if either is.
+__device__ __forceinline__ float w4_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float w4_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// Two FP32 values to an instruction.
+__device__ __forceinline__ uint64_t w4_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 w4_both(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t w4_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t w4_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t w4_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
 // The integer nearest to w / s for s > 0, ties to even, as a float.  The quotient in FP32 names a candidate that is at most
 // one off; the candidate's remainder, which an FMA leaves exact near a border, says whether a neighbour is nearer.  `inv` is
@@ -78,10 +115,13 @@ __device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
   }
 }
 
-// Quantising is bound by reading W.  group / 16 lanes share a group, 16 elements (8 bytes of codes) each: a group's extremes take
-// log2(group / 16) shuffles, and a warp reads 512 elements in a row.  Without a place to start on 16 bytes (VEC = false: odd
-// pitches, shifted bases) the elements come one by one, and the codes of 8 bytes go out as bytes.
-template <class T, class S, bool VEC>
+// Quantising should be bound by reading W; at 8 instructions per element it nearly is.  group / 16 lanes share a group, 16
+// elements (8 bytes of codes) each: a group's extremes take log2(group / 16) shuffles.  Nearly every element's code is what the
+// magic addition in w4_nearest gives at once: w / s + 1.5 * 2^23 holds it in its low bits.  Elements that are not nearer than
+// s / 2 to their codes' values (with 16-bit weights a third of the warps meet one that is exactly s / 2 away), and all of a group
+// that needs more care (a scale that is 0, tiny or clamped), are given to w4_nearest, one by one.  Without a place to start on 16 bytes (VEC = false: odd pitches, shifted bases) the elements come
+// one by one and the codes go out as bytes.
+template <class T, class S, bool ZEROS, bool VEC>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, int group_shift, const T *W, int64_t ldw, uint8_t *codes,
                                                           int64_t ldq, S *scales, uint8_t *zeros) {
   const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
@@ -103,44 +143,64 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = i < len ? to_f32(w[i]) : 0.f;
       }
-      float lo = 0.f, hi = 0.f, sum = 0.f;
+      float lo = 0.f, hi = 0.f;                                           // without zeros: hi = largest magnitude
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        lo = fminf(lo, v[i]);
-        hi = fmaxf(hi, v[i]);
-        sum += v[i] * 0.f;                                                // 0, or NaN from an infinity or a NaN
+        hi = w4_max_nan(hi, ZEROS ? v[i] : fabsf(v[i]));
+        if (ZEROS) lo = w4_min_nan(lo, v[i]);
       }
       for (int o = 1; o < lanes; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        hi = w4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       }
       if (len <= 0) continue;                                             // nothing to write; a group's first lane has elements
-      const bool bad = sum != 0.f;                                        // true for NaN
-      const S stored = bad ? from_f32<S>(__int_as_float(0x7fffffff)) : w4_scale<S>(lo, hi, zeros != nullptr);
+      const bool bad = !isfinite(hi) || (ZEROS && !isfinite(lo));
+      const S stored = bad ? from_f32<S>(__int_as_float(0x7fffffff)) : w4_scale<S>(lo, hi, ZEROS);
       const float scale = to_f32(stored);
       const bool flat = !(scale > 0.f);                                   // 0, or NaN: every code is the zero point
       const float f = w4_prescale(scale), s = scale * f, inv = 1.f / s, half = 0.5f * s;
       float zero = 8.f;
-      if (zeros && !flat) zero = fminf(fmaxf(w4_nearest(-lo * f, s, half, inv), 0.f), 15.f);
-      const float lowest = zeros ? 0.f : 1.f;
+      if (ZEROS && !flat) zero = fminf(fmaxf(w4_nearest(-lo * f, s, half, inv), 0.f), 15.f);
       if ((u & (lanes - 1)) == 0) {
         const int64_t at = n * groups + (u >> (group_shift - 4));
         scales[at] = stored;
-        if (zeros) zeros[at] = (uint8_t)zero;
+        if (ZEROS) zeros[at] = (uint8_t)zero;
       }
       uint32_t out[2] = {0, 0};
+      // the quick way: 1.5 * 2^23 + zero - 8 is even or odd as zero is, which only ties would tell apart
+      uint32_t unsure = !flat && f == 1.f && (ZEROS || hi * inv < 7.4f) ? 0u : 0xffffu;
+      const float magic = 12582912.f;
+      const uint64_t inv2 = w4_two(inv, inv), magic2 = w4_two(magic, magic), minus2 = w4_two(-magic, -magic), s2 = w4_two(-s, -s);
+      const float least = magic - zero, most = magic + 15.f - zero;
+      const uint32_t base = __float_as_uint(magic) - (uint32_t)(int)zero;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float c = flat ? zero : fminf(fmaxf(w4_nearest(v[i] * f, s, half, inv) + zero, lowest), 15.f);
-        // as an integer in the low bits of 2^23 + c
-        const uint32_t bits = __float_as_uint(c + 8388608.f) & 15u;
-        out[i >> 3] |= (i < len ? bits : 0u) << (4 * (i & 7));
+      for (int i = 0; i < 16; i += 2) {
+        const uint64_t x = w4_two(v[i], v[i + 1]);
+        const uint64_t big = w4_fma(x, inv2, magic2);                     // rounded once, to an integer
+        const float2 r = w4_both(w4_fma(w4_add(big, minus2), s2, x));
+        if (!(fabsf(r.x) < half)) unsure |= 1u << i;
+        if (!(fabsf(r.y) < half)) unsure |= 2u << i;
+        float2 b = w4_both(big);
+        if (ZEROS) b = make_float2(fminf(fmaxf(b.x, least), most), fminf(fmaxf(b.y, least), most));
+        // (where the quick way is not taken at all these bits are nonsense, and every code is set below)
+        out[i >> 3] += ((__float_as_uint(b.x) - base) << (4 * (i & 7))) + ((__float_as_uint(b.y) - base) << (4 * (i & 7) + 4));
+      }
+      while (unsure) {
+        const int i = __ffs((int)unsure) - 1;
+        unsure &= unsure - 1;
+        float e = v[0];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) e = i == k ? v[k] : e;
+        const float c = flat ? zero : fminf(fmaxf(w4_nearest(e * f, s, half, inv) + zero, ZEROS ? 0.f : 1.f), 15.f);
+        const uint32_t shift = 4 * (i & 7), fresh = (uint32_t)c << shift, keep = ~(15u << shift);
+        if (i < 8) out[0] = (out[0] & keep) | fresh;
+        else out[1] = (out[1] & keep) | fresh;
       }
       uint8_t *to = codes + n * ldq + (k0 >> 1);
       if (VEC && len == 16) {
         *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
       } else {
+        if (len & 1) out[len >> 3] &= ~(0xf0u << (8 * ((len >> 1) & 3)));   // the half byte behind an odd row is 0
         for (int i = 0; 2 * i < len; ++i) to[i] = (uint8_t)(out[i >> 2] >> (8 * (i & 3)));
       }
     }
@@ -149,59 +209,82 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
 
 __device__ __forceinline__ float w4_zero(const uint8_t *zeros, int64_t at) { return zeros ? (float)(zeros[at] & 15) : 8.f; }
 
-// 8 codes of a word, times (scale) after the zero point is taken off, as 8 elements of T.
-template <class T>
-struct W4Out {
-  T e[8];
-};
-template <class T>
-__device__ __forceinline__ void w4_expand(W4Out<T> &out, uint32_t word, float scale, float zero) {
-  // a code in the low bits of 2^23 reads 2^23 + c; the difference with 2^23 + z is exact
-  const float base = 8388608.f + zero;
+// 8 codes of a word as FP32: (c - z) * scale, in order.  The even codes are masked out as bytes, the odd ones likewise after a
+// shift; a byte under 2^23's upper three reads 2^23 + c, and the difference with 2^23 + z is exact.
+__device__ __forceinline__ void w4_expand(float (&v)[8], uint32_t word, float scale, float zero) {
+  const uint32_t even = word & 0x0f0f0f0fu, odd = (word >> 4) & 0x0f0f0f0fu;
+  const uint64_t less = w4_two(-8388608.f - zero, -8388608.f - zero), by = w4_two(scale, scale);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    out.e[i] = from_f32<T>((__uint_as_float(((word >> (4 * i)) & 15u) | 0x4b000000u) - base) * scale);
+  for (int i = 0; i < 4; ++i) {
+    const float a = __uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + i)), b = __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + i));
+    const float2 r = w4_both(w4_mul(w4_add(w4_two(a, b), less), by));
+    v[2 * i] = r.x, v[2 * i + 1] = r.y;
+  }
 }
 
-// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements; VEC where words of codes
-// and 16 bytes of W start on their own size.
+// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight;
+// VEC where words of codes and 16 bytes of W start on their own size.
 template <class T, class S, bool VEC>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
                                                             const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
-  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift, units = (K + 7) >> 3;
+  constexpr int kFlight = 4;
+  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
+  const int units = (int)((K + 7) >> 3), step = (int)(gridDim.x * blockDim.x);
   for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
-    for (int64_t u = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; u < units; u += (int64_t)gridDim.x * blockDim.x) {
-      const int64_t k0 = u * 8, g = n * groups + (k0 >> group_shift);
-      const int len = K - k0 < 8 ? (int)(K - k0) : 8;
-      const uint8_t *from = codes + n * ldq + 4 * u;
-      uint32_t word = 0;
-      if (VEC && len == 8) {
-        word = __ldcs(reinterpret_cast<const uint32_t *>(from));
-      } else {
+    const uint8_t *row = codes + n * ldq;
+    const S *scale_row = scales + n * groups;
+    const uint8_t *zero_row = zeros ? zeros + n * groups : nullptr;
+    T *out = W + n * ldw;
+    for (int64_t u0 = blockIdx.x * blockDim.x + threadIdx.x; u0 < units; u0 += (int64_t)kFlight * step) {
+      uint32_t word[kFlight];
+      float scale[kFlight], zero[kFlight];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (2 * i < len) word |= (uint32_t)from[i] << (8 * i);
+      for (int i = 0; i < kFlight; ++i) {
+        const int64_t u = u0 + (int64_t)i * step;
+        word[i] = 0;
+        if (u < units) {
+          if (VEC && 8 * u + 8 <= K) {
+            word[i] = __ldcs(reinterpret_cast<const uint32_t *>(row + 4 * u));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (8 * u + 2 * q < K) word[i] |= (uint32_t)row[4 * u + q] << (8 * q);
+          }
+          scale[i] = to_f32(scale_row[(8 * u) >> group_shift]);
+          zero[i] = zero_row ? (float)(zero_row[(8 * u) >> group_shift] & 15) : 8.f;
+        }
       }
-      W4Out<T> out;
-      w4_expand(out, word, to_f32(scales[g]), w4_zero(zeros, g));
-      T *to = W + n * ldw + k0;
-      if (VEC && len == 8) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4 *>(to) + i, reinterpret_cast<const uint4 *>(out.e)[i]);
-      } else {
+      for (int i = 0; i < kFlight; ++i) {
+        const int64_t u = u0 + (int64_t)i * step;
+        if (u < units) {
+          float v[8];
+          w4_expand(v, word[i], scale[i], zero[i]);
+          union {
+            T e[8];
+            uint4 q[sizeof(T) / 2];
+          } o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < len) to[i] = out.e[i];
+          for (int k = 0; k < 8; ++k) o.e[k] = from_f32<T>(v[k]);
+          T *to = out + 8 * u;
+          if (VEC && 8 * u + 8 <= K) {
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4 *>(to) + q, o.q[q]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (8 * u + k < K) to[k] = o.e[k];
+          }
+        }
       }
     }
   }
 }
 
 // Transposed: tiles of 64 rows n x 64 of k through shared memory, so that codes are read along k and W is written along n.
-// A thread expands 16 codes (8 bytes) of one row into a column of the tile; a row of the tile goes out as 64 elements along n.
-// The tile's rows are 65 words apart (FP32; two 16-bit elements share a word in pairs of rows otherwise wasted): threads of a
-// warp that write 16 different rows of one k meet in different banks.
-template <class T, class S, bool VEC>
+// A thread expands 16 codes (8 bytes) of one row into a column of the tile; a row of the tile goes out as 64 elements along n,
+// two of 16 bits to an access where W allows (PAIR).
+template <class T, class S, bool VEC, bool PAIR>
 __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
                                                            const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
   __shared__ float tile[64][65];                // [k][n]
@@ -229,10 +312,13 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
         scale = to_f32(scales[g]);
         zero = w4_zero(zeros, g);
       }
-      const float base = 8388608.f + zero;
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        tile[c + i][r] = (__uint_as_float(((word[i >> 3] >> (4 * (i & 7))) & 15u) | 0x4b000000u) - base) * scale;
+      for (int h = 0; h < 2; ++h) {
+        float v[8];
+        w4_expand(v, word[h], scale, zero);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) tile[c + 8 * h + i][r] = v[i];
+      }
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -240,10 +326,22 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
     for (int i = 0; i < 8; ++i) {
       const int64_t k = k0 + warp * 8 + i;
       if (k < K) {
+        if constexpr (PAIR) {
+          const int64_t n = n0 + 2 * lane;
+          union {
+            T e[2];
+            uint32_t w;
+          } o;
+          o.e[0] = from_f32<T>(tile[warp * 8 + i][2 * lane]);
+          o.e[1] = from_f32<T>(tile[warp * 8 + i][2 * lane + 1]);
+          if (n + 1 < N) *reinterpret_cast<uint32_t *>(W + k * ldw + n) = o.w;
+          else if (n < N) W[k * ldw + n] = o.e[0];
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int64_t n = n0 + h * 32 + lane;
-          if (n < N) W[k * ldw + n] = from_f32<T>(tile[warp * 8 + i][h * 32 + lane]);
+          for (int h = 0; h < 2; ++h) {
+            const int64_t n = n0 + h * 32 + lane;
+            if (n < N) W[k * ldw + n] = from_f32<T>(tile[warp * 8 + i][h * 32 + lane]);
+          }
         }
       }
     }
@@ -962,8 +1060,9 @@ int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
-    if (vec) w4_quantize_kernel<T, S, true><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
-    else w4_quantize_kernel<T, S, false><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
+    const auto kernel = zeros ? (vec ? w4_quantize_kernel<T, S, true, true> : w4_quantize_kernel<T, S, true, false>)
+                              : (vec ? w4_quantize_kernel<T, S, false, true> : w4_quantize_kernel<T, S, false, false>);
+    kernel<<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
   });
   B2_CUDA(cudaGetLastError());
   return B2_OK;
@@ -989,10 +1088,13 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
       const int64_t tiles = ((N + 63) / 64) * ((K + 63) / 64), most = (int64_t)ctx->sm_count * 64;
       const unsigned grid = (unsigned)(tiles < most ? tiles : most);
       const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
-      if (vec) w4_transpose_kernel<T, S, true><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
-      else w4_transpose_kernel<T, S, false><<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      constexpr bool kPair = sizeof(T) == 2;
+      const bool pair = kPair && (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 3) == 0;
+      const auto kernel = pair ? (vec ? w4_transpose_kernel<T, S, true, kPair> : w4_transpose_kernel<T, S, false, kPair>)
+                               : (vec ? w4_transpose_kernel<T, S, true, false> : w4_transpose_kernel<T, S, false, false>);
+      kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
     } else {
-      const W4Grid g((K + 7) / 8, N, 1);
+      const W4Grid g((K + 31) / 32, N, 1);      // four units of 8 to a thread
       const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 3) == 0 && (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0;
       if (vec) w4_dequantize_kernel<T, S, true><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
       else w4_dequantize_kernel<T, S, false><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
