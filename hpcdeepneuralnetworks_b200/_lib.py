@@ -90,7 +90,7 @@ def load() -> C.CDLL:
     L.b2_w4_quantize.argtypes = [vp, i64, i64, i32, i32, vp, i64, vp, i64, i32, vp, vp, vp]
     L.b2_w4_dequantize.argtypes = [vp, i64, i64, i32, vp, i64, i32, vp, vp, i32, vp, i64, i32, vp]
     L.b2_w4_matvec_workspace_bytes.restype = C.c_size_t
-    L.b2_w4_matvec_workspace_bytes.argtypes = [i64, i64, i32]
+    L.b2_w4_matvec_workspace_bytes.argtypes = [i64, i64, i64, i32]
     L.b2_w4_matvec.argtypes = [vp, i64, i64, i64, i32, f32, i32, vp, i64, vp, i64, i32, vp, vp, f32, vp, i64, vp, C.c_size_t, vp]
     L.b2_fill_uniform.argtypes = [vp, i64, u64, vp]
     L.b2_fill_uniform_host.argtypes = [vp, i64, u64]

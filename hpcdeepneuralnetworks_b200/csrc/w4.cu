@@ -377,13 +377,13 @@ constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2, kMvCode
 constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns of a warp's store in 32 banks
 constexpr int kMvWindow = 1024;             // scales and zero points held together: 8 groups of each row, the group / 32 chunks
 constexpr int kMvWindows = 2;               // they span
-constexpr int kMvMaxStages = 8, kMvBarrierBytes = 256 + 1024;   // barriers, and room to align
+constexpr int kMvMaxStages = 8, kMvBarrierBytes = 512 + 1024;   // barriers and flags, and room to align
 constexpr int kMvXThreads = 512;
 
-template <int NB>
+template <int NB, bool RESIDENT>
 struct MvTile {
   static constexpr int kXBytes = NB * (kMvChunk * 8 * 2 + 256);     // x of one chunk: fragments, then sums [part of a group][8 NB]
-  static constexpr int kStage = (kMvCodeBytes + kXBytes + 1023) / 1024 * 1024;
+  static constexpr int kStage = RESIDENT ? kMvCodeBytes : (kMvCodeBytes + kXBytes + 1023) / 1024 * 1024;
   static constexpr int kSumBytes = 2 * 8 * NB * kMvPitch * 4;
   static constexpr int kCtasPerSm = NB <= 2 ? 2 : 1;
   static constexpr int kSmem = kCtasPerSm == 2 ? 115712 : 232448;   // what a CTA may have
@@ -393,17 +393,27 @@ struct MvTile {
 static int mv_parts(int type) { return type == B2_F32 ? 3 : 1; }
 static int mv_blocks(int64_t M, int type) { return M * mv_parts(type) <= 8 ? 1 : M * mv_parts(type) <= 16 ? 2 : 4; }
 static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
+// Whether a product's CTAs lay x out themselves (RESIDENT): each keeps its part of k, cut over clusters of up to 8, in shared
+// memory.  That saves a kernel and a workspace, and costs the same work in every row block's CTAs.
+constexpr int kMvResidentBytes = 35 * 1024;
+constexpr int64_t kMvResidentWork = 4096;      // row blocks x chunks x column blocks
+static bool mv_resident(int64_t M, int64_t N, int64_t K, int type) {
+  const int nb = mv_blocks(M, type);
+  const int64_t chunks = (K + kMvChunk - 1) / kMvChunk, per_cta = (chunks + 7) / 8;
+  const int64_t blocks = (N + kMvRows - 1) / kMvRows;
+  return nb <= 2 && per_cta * nb * (kMvChunk * 8 * 2 + 256) <= kMvResidentBytes && blocks * chunks * nb <= kMvResidentWork;
+}
 
 struct MvArgs {
   int64_t N, K, ldx, ldq, ldy, groups;
   int M, rows_per_item, parts, type, group_shift, scale_type;
-  int stages, items, row_blocks, chunks, chunks_per_cta;
+  int stages, items, row_blocks, chunks, chunks_per_cta, vec;
   float alpha, beta;
   const void *x;
   const uint8_t *codes, *zeros;
   const void *scales;
   void *y;
-  const unsigned char *image;      // [item's rows][chunk][kXBytes]
+  const unsigned char *image;      // [item's rows][chunk][kXBytes], unless the CTAs lay x out themselves
   const int2 *row_info;            // of each row of x: the power of two it was scaled by, and whether it holds an infinity or NaN
   int *status;
   unsigned int seq;
@@ -456,9 +466,56 @@ __device__ __forceinline__ void mv_load_x(float (&v)[8], const T *row, int64_t k
   }
 }
 
-// One block per row of x: its largest finite element, then the scaled, paired FP16 terms and the sums over parts of groups
-// (1 << part_log elements: a group, or the 128 of a longer one that a warp multiplies).  Four units of 8 elements per thread are
-// kept between the two passes; a longer row is read again.
+// The power of two that brings `largest` to [2^14, 2^15), as an exponent, and as two factors (it may pass FP32's range).
+__device__ __forceinline__ int mv_exponent(float largest) {
+  int q = 0;
+  if (largest > 0.f) frexpf(largest, &q), q = 15 - q;
+  return q;
+}
+// Looks at 8 elements: the largest finite magnitude, and whether one is not finite.
+__device__ __forceinline__ void mv_look(const float (&e)[8], float &top, bool &bad) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (isfinite(e[i])) top = fmaxf(top, fabsf(e[i]));
+    else bad = true;
+  }
+}
+// Lays one unit (8 elements, the `u`-th of its chunk, a lane per unit) of columns col0.. out in a chunk's image: scaled by
+// f1 * f2, cut into `parts` FP16 terms, paired, and summed over parts of groups (1 << part_log elements: a group, or the 128 of
+// a longer one that a warp multiplies).
+__device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8], int u, int nb, int col0, int parts, int part_log, float f1,
+                                       float f2) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) ? 0.0625f : 1.f) : 0.f;
+  for (int p = 0; p < parts; ++p) {
+    const int col = col0 + p;
+    __half h[8];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      h[i] = __float2half_rn(r[i]);
+      const float back = __half2float(h[i]);
+      sum += (i & 1) ? 16.f * back : back;
+      r[i] = (r[i] - back) * 2048.f;       // what the term left, 11 bits up, for the next
+    }
+    union {
+      __half2 h2[4];
+      uint4 q;
+    } out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.h2[i] = __halves2half2(h[i], h[i + 4]);
+    reinterpret_cast<uint4 *>(chunk)[(((u >> 2) * nb + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = out.q;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1)
+      if (o < (1 << (part_log - 3))) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((u & ((1 << (part_log - 3)) - 1)) == 0)
+      reinterpret_cast<float *>(chunk + nb * (kMvChunk * 8 * 2))[(u >> (part_log - 3)) * 8 * nb + col] = sum * 0x1p-24f;
+  }
+}
+
+// One block per row of x: its largest finite element, then its image.  Four units per thread are kept between the two passes; a
+// longer row is read again.
 template <class T>
 __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ldx, int vec, const T *x, int chunks, int nb, int rows_per_item,
                                                            int part_log, unsigned char *image, int2 *row_info) {
@@ -473,23 +530,16 @@ __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ld
   float v[kKept][8];
   float top = 0.f;
   bool bad = false;
-  auto look = [&](const float (&e)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (isfinite(e[i])) top = fmaxf(top, fabsf(e[i]));
-      else bad = true;
-    }
-  };
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
     if (tid + i * kMvXThreads < units) mv_load_x<T>(v[i], row, 8 * (int64_t)(tid + i * kMvXThreads), K, vec != 0);
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) look(v[i]);
+    if (tid + i * kMvXThreads < units) mv_look(v[i], top, bad);
   for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
     float e[8];
     mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
-    look(e);
+    mv_look(e, top, bad);
   }
   top = w4_warp_max(top);
   const bool any = __any_sync(0xffffffffu, bad);
@@ -497,43 +547,12 @@ __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ld
   __syncthreads();
   top = w4_warp_max(lane < kMvXThreads / 32 ? largest[lane] : 0.f);
   bad = __any_sync(0xffffffffu, lane < kMvXThreads / 32 && odd[lane]);
-  int q = 0;
-  if (top > 0.f) frexpf(top, &q), q = 15 - q;       // top * 2^q in [2^14, 2^15)
+  const int q = mv_exponent(top);
   if (tid == 0) row_info[m] = make_int2(q, bad);
-  const int q1 = q / 2, q2 = q - q1;               // 2^q itself may pass FP32's range
-  const float f1 = ldexpf(1.f, q1), f2 = ldexpf(1.f, q2);
-
+  const float f1 = ldexpf(1.f, q / 2), f2 = ldexpf(1.f, q - q / 2);
   const int chunk_bytes = nb * (kMvChunk * 8 * 2 + 256);
   auto put = [&](const float (&e)[8], int u) {
-    unsigned char *chunk = image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes;
-    float r[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) ? 0.0625f : 1.f) : 0.f;
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) {
-      const int col = col0 + p;
-      __half h[8];
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        h[i] = __float2half_rn(r[i]);
-        const float back = __half2float(h[i]);
-        sum += (i & 1) ? 16.f * back : back;
-        r[i] = (r[i] - back) * 2048.f;       // what the term left, 11 bits up, for the next
-      }
-      union {
-        __half2 h2[4];
-        uint4 q;
-      } out;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out.h2[i] = __halves2half2(h[i], h[i + 4]);
-      reinterpret_cast<uint4 *>(chunk)[((((u >> 2) & 7) * nb + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = out.q;
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1)
-        if (o < (1 << (part_log - 3))) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((u & ((1 << (part_log - 3)) - 1)) == 0)
-        reinterpret_cast<float *>(chunk + nb * (kMvChunk * 8 * 2))[((u & 31) >> (part_log - 3)) * 8 * nb + col] = sum * 0x1p-24f;
-    }
+    mv_put(image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes, e, u & 31, nb, col0, kParts, part_log, f1, f2);
   };
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
@@ -629,10 +648,10 @@ __device__ __forceinline__ float mv_load_any_type(const void *p, int type, int64
   return to_f32(((const __half *)p)[at]);
 }
 
-// What the infinities and NaN of row m of x add to output n.
-__device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n) {
+// What the infinities and NaN of row m of x, elements k0 to k1, add to output n.
+__device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, int64_t k0, int64_t k1) {
   float v = 0.f;
-  for (int64_t k = 0; k < a.K; ++k) {
+  for (int64_t k = k0; k < k1; ++k) {
     const float e = mv_load_any_type(a.x, a.type, m * a.ldx + k);
     if (isfinite(e)) continue;
     const int c = (a.codes[n * a.ldq + (k >> 1)] >> (4 * (k & 1))) & 15;
@@ -643,10 +662,11 @@ __device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n) {
 }
 
 // ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
-template <int NB, bool ALIGNED>
-__global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
+// RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
+template <int NB, bool ALIGNED, bool RESIDENT>
+__global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
-  using Tile = MvTile<NB>;
+  using Tile = MvTile<NB, RESIDENT>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle is one of addresses
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -656,15 +676,17 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
   chunks = chunks < 0 ? 0 : chunks < a.chunks_per_cta ? chunks : a.chunks_per_cta;
   const int window_log = a.group_shift - 5;                                // chunks of a window: group / 32
   float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, zero point
-  float *const sums = reinterpret_cast<float *>(windows + kMvWindows * kMvWindow);       // [2][8 NB][kMvPitch]
+  unsigned char *const xs = reinterpret_cast<unsigned char *>(windows + kMvWindows * kMvWindow);   // RESIDENT: [chunk][kXBytes]
+  float *const sums = reinterpret_cast<float *>(xs + (RESIDENT ? a.chunks_per_cta * Tile::kXBytes : 0));   // [2][8 NB][kMvPitch]
   uint64_t *const full = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sums) + Tile::kSumBytes);
   uint64_t *const empty = full + kMvMaxStages, *const wfull = empty + kMvMaxStages, *const wempty = wfull + kMvWindows;
   uint64_t *const ready = wempty + kMvWindows, *const done = ready + 1;
+  int *const largest = reinterpret_cast<int *>(done + 1), *const odd = largest + 16;      // RESIDENT: of each row of x (at most 16)
   constexpr int kFillers = kMvProducers - 32;     // threads that write shared memory themselves
 
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&full[s], ALIGNED ? 1 : 1 + kFillers);
+      mbar_init(&full[s], (ALIGNED || !RESIDENT ? 1 : 0) + (ALIGNED ? 0 : kFillers));
       mbar_init(&empty[s], kMvConsumers / 32);
     }
     for (int s = 0; s < kMvWindows; ++s) {
@@ -682,7 +704,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
   if (warp >= kMvConsumers / 32) {
     if (warp == kMvConsumers / 32) {
       if (lane == 0) {
-        // Weights may be read at once: the kernel in front of this one, w4_x_kernel, began after all earlier work had ended.
+        // (RESIDENT: an ordinary launch, and codes alone.)  Weights may be read at once: the kernel in front of this one, w4_x_kernel, began after all earlier work had ended.
         // Its own results, x, have to be waited for; the ring is filled with codes first.
         MvRing ring(a.stages);
         uint32_t sent = 0;
@@ -697,9 +719,10 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
           for (int c = 0; c < chunks; ++c, ring.next(), image += Tile::kXBytes) {
             if (sent >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
             if (!wait.alive) continue;
-            mbar_expect_tx(&full[ring.at], (ALIGNED ? kMvCodeBytes : 0) + Tile::kXBytes);
+            if (ALIGNED || !RESIDENT) mbar_expect_tx(&full[ring.at], (ALIGNED ? kMvCodeBytes : 0) + (RESIDENT ? 0 : Tile::kXBytes));
             if (ALIGNED) tma_load_2d(smem + ring.at * Tile::kStage, &code_map, &full[ring.at], (first + c) * kMvRowBytes, row);
-            if (waited) {
+            if (RESIDENT) {
+            } else if (waited) {
               send_x(ring.at, image);
             } else {
               late[sent] = image;
@@ -777,6 +800,38 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
     const int parts_log = a.group_shift < 7 ? a.group_shift - 5 : 2;      // blocks of 32 in a part of a group
     uint32_t turn = 0;
     MvRing ring(a.stages), window(kMvWindows);
+    if constexpr (RESIDENT) {
+      // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8.  Each
+      // row is scaled by its largest element here; the sums are scaled back before they leave the CTA.
+      if (tid < 16) largest[tid] = 0, odd[tid] = 0;
+      mv_consumers_sync();
+      for (int pass = 0; pass < 2; ++pass) {
+        for (int at = warp; at < a.M * chunks; at += kMvConsumers / 32) {
+          const int m = at / chunks, c = at - m * chunks;
+          const int64_t k = (int64_t)(first + c) * kMvChunk + 8 * lane;
+          float e[8];
+          if (a.type == B2_F32) mv_load_x(e, (const float *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+          else if (a.type == B2_BF16) mv_load_x(e, (const __nv_bfloat16 *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+          else mv_load_x(e, (const __half *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+          if (pass == 0) {
+            float top = 0.f;
+            bool bad = false;
+            mv_look(e, top, bad);
+            top = w4_warp_max(top);
+            bad = __any_sync(0xffffffffu, bad);
+            if (lane == 0) {
+              atomicMax(&largest[m], __float_as_int(top));      // not negative: ordered as integers
+              if (bad) atomicOr(&odd[m], 1);
+            }
+          } else {
+            const int q = mv_exponent(__int_as_float(largest[m]));
+            mv_put(xs + c * Tile::kXBytes, e, lane, NB, m * a.parts, a.parts, a.group_shift < 7 ? a.group_shift : 7, ldexpf(1.f, q / 2),
+                   ldexpf(1.f, q - q / 2));
+          }
+        }
+        mv_consumers_sync();
+      }
+    }
     for (int item = blockIdx.x; item < a.items; item += gridDim.x, ++turn) {
       const int mc = item / a.row_blocks;
       float total[2][NB][4] = {};
@@ -786,8 +841,9 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
         wait(&full[ring.at], ring.phase);
         const unsigned char *const stage = smem + ring.at * Tile::kStage;
         const unsigned char *codes = stage + (wn * 32 + g) * kMvRowBytes + 4 * t;
-        const uint4 *xf = reinterpret_cast<const uint4 *>(stage + kMvCodeBytes) + wk * 4 * NB * 32 + lane;
-        const float *xsum = reinterpret_cast<const float *>(stage + kMvCodeBytes + NB * (kMvChunk * 8 * 2)) + 2 * t;
+        const unsigned char *const image = RESIDENT ? xs + c * Tile::kXBytes : stage + kMvCodeBytes;
+        const uint4 *xf = reinterpret_cast<const uint4 *>(image) + wk * 4 * NB * 32 + lane;
+        const float *xsum = reinterpret_cast<const float *>(image + NB * (kMvChunk * 8 * 2)) + 2 * t;
         const float2 *sz = windows + window.at * kMvWindow + ((wn * 32 + g) << 3);
         const int block0 = in_window * 8 + wk * 4;                    // this warp's first block of 32 k within the window
         // the warp's 128 k in straight-line code, BLOCKS blocks of 32 to a group (or to the warp's part of one)
@@ -849,26 +905,46 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
       if (turn == 0) cluster_wait();                                // every CTA's barriers are set up
       else if (ctas > 1) wait.cluster(done, (turn - 1) & 1);        // every CTA has read the sums of the block before
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt)
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        for (int i = 0; i < 2; ++i) {
+          const int col = nb * 8 + 2 * t + i, m = col / a.parts;
+          // RESIDENT: the codes' 2^-24, this CTA's scale of the row and the term's
+          const int up = RESIDENT && m < a.M ? 24 - 11 * (col - m * a.parts) - mv_exponent(__int_as_float(largest[m])) : 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            sums[(wk * 8 * NB + nb * 8 + 2 * t + (i & 1)) * kMvPitch + wn * 32 + rt * 16 + g + (i >> 1) * 8] = total[rt][nb][i];
+          for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float v = total[rt][nb][i + 2 * h];
+              sums[(wk * 8 * NB + col) * kMvPitch + wn * 32 + rt * 16 + g + h * 8] = RESIDENT ? ldexpf(v, up) : v;
+            }
+        }
       mv_consumers_sync();
+      if constexpr (RESIDENT) {
+        bool any = false;
+        for (int m = 0; m < a.M; ++m) any |= odd[m] != 0;
+        if (any && chunks > 0) {
+          const int64_t n0 = (int64_t)item * kMvRows, k0 = (int64_t)first * kMvChunk, k1 = k0 + (int64_t)chunks * kMvChunk;
+          for (int i = tid; i < a.M * kMvRows; i += kMvConsumers) {
+            const int m = i / kMvRows, r = i % kMvRows;
+            if (odd[m] && n0 + r < a.N) sums[m * a.parts * kMvPitch + r] += mv_not_finite(a, m, n0 + r, k0, k1 < a.K ? k1 : a.K);
+          }
+          mv_consumers_sync();
+        }
+      }
       if (ctas > 1) {
         if (tid < ctas) mbar_arrive_cluster(mapa_u32(smem_u32(ready), (uint32_t)tid));
         wait.cluster(ready, turn & 1);
       }
       const int m0 = mc * a.rows_per_item, mm = a.M - m0 < a.rows_per_item ? a.M - m0 : a.rows_per_item;
       const int64_t n0 = (int64_t)(item - mc * a.row_blocks) * kMvRows;
-      if (turn == 0) pdl_wait();                                    // row_info is w4_x_kernel's
+      if (!RESIDENT && turn == 0) pdl_wait();                       // row_info is w4_x_kernel's
       for (int i = tid + rank * kMvConsumers; i < mm * kMvRows; i += kMvConsumers * ctas) {
         const int m = i / kMvRows, r = i % kMvRows;
         if (n0 + r >= a.N) continue;
         float v = 0.f;
         if (a.chunks > 0) {
-          const int2 info = a.row_info[m0 + m];
+          const int2 info = RESIDENT ? make_int2(0, 0) : a.row_info[m0 + m];
           for (int p = 0; p < a.parts; ++p) {
             const float *at = sums + (m * a.parts + p) * kMvPitch + r;
             float s = 0.f;
@@ -880,9 +956,9 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB>::kCtasPerSm)
             } else {
               s = at[0] + at[8 * NB * kMvPitch];
             }
-            v += ldexpf(s, 24 - 11 * p - info.x);                   // the codes' 2^-24, the row's scale and the term's
+            v += RESIDENT ? s : ldexpf(s, 24 - 11 * p - info.x);    // the codes' 2^-24, the row's scale and the term's
           }
-          if (info.y) v += mv_not_finite(a, m0 + m, n0 + r);
+          if (info.y) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
         }
         v *= a.alpha;
         const int64_t to = (int64_t)(m0 + m) * a.ldy + n0 + r;
@@ -931,10 +1007,10 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   return B2_OK;
 }
 
-template <int NB, bool ALIGNED>
+template <int NB, bool ALIGNED, bool RESIDENT>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
-  using Tile = MvTile<NB>;
-  const auto kernel = w4_matvec_kernel<NB, ALIGNED>;
+  using Tile = MvTile<NB, RESIDENT>;
+  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
   const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows;
@@ -947,15 +1023,17 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   int ctas = 1, clusters = 1;
   int64_t shortest = INT64_MAX;
   for (int n = 1; n <= 8 && (n == 1 || n <= a.chunks); n *= 2) {
+    const int64_t each = (a.chunks + n - 1) / n;
+    if (RESIDENT && n < 8 && 2 * n <= a.chunks && each * Tile::kXBytes > kMvResidentBytes) continue;      // x would not fit
     int held = 1;
     const int e = mv_clusters((const void *)kernel, ctx->device, n, Tile::kSmem, &held);
     if (e != B2_OK) return e;
     if (held > a.items) held = a.items;
-    const int64_t length = (int64_t)((a.items + held - 1) / held) * ((a.chunks + n - 1) / n + 1);
+    const int64_t length = (int64_t)((a.items + held - 1) / held) * (each + 1) + (RESIDENT ? each : 0);
     if (length < shortest) shortest = length, ctas = n, clusters = held;
   }
   a.chunks_per_cta = (a.chunks + ctas - 1) / ctas;
-  const int other = Tile::kSumBytes + kMvWindows * kMvWindow * 8 + kMvBarrierBytes;
+  const int other = Tile::kSumBytes + kMvWindows * kMvWindow * 8 + kMvBarrierBytes + (RESIDENT ? a.chunks_per_cta * Tile::kXBytes : 0);
   a.stages = (Tile::kSmem - other) / Tile::kStage;
   if (a.stages > kMvMaxStages) a.stages = kMvMaxStages;
   const int64_t per_cta = (int64_t)a.chunks_per_cta * ((a.items + clusters - 1) / clusters);
@@ -978,7 +1056,7 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = a.chunks > 0 ? 2 : 1;        // without w4_x_kernel in front there is nothing to overlap
+  cfg.numAttrs = RESIDENT || a.chunks == 0 ? 1 : 2;        // without w4_x_kernel in front there is nothing to overlap
   a.status = (int *)((char *)ctx->fixed + kFixedStatus);
   a.seq = next_launch_seq(ctx);
   B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const MvArgs)a, (const CUtensorMap)code_map));
@@ -986,10 +1064,11 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
 }
 
 template <bool ALIGNED>
-static int w4_matvec_blocks(Context *ctx, const MvArgs &a, int nb, cudaStream_t s) {
-  return nb == 1   ? w4_matvec_launch<1, ALIGNED>(ctx, a, s)
-         : nb == 2 ? w4_matvec_launch<2, ALIGNED>(ctx, a, s)
-                   : w4_matvec_launch<4, ALIGNED>(ctx, a, s);
+static int w4_matvec_blocks(Context *ctx, const MvArgs &a, int nb, bool resident, cudaStream_t s) {
+  if (resident) return nb == 1 ? w4_matvec_launch<1, ALIGNED, true>(ctx, a, s) : w4_matvec_launch<2, ALIGNED, true>(ctx, a, s);
+  return nb == 1   ? w4_matvec_launch<1, ALIGNED, false>(ctx, a, s)
+         : nb == 2 ? w4_matvec_launch<2, ALIGNED, false>(ctx, a, s)
+                   : w4_matvec_launch<4, ALIGNED, false>(ctx, a, s);
 }
 
 // The workspace of a product: the image of x, then row_info.
@@ -1104,8 +1183,9 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
   return B2_OK;
 }
 
-size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t K, int type) {
-  if (M <= 0 || M > kW4MaxRows || K <= 0 || K > INT32_MAX || type_bytes(type) == 0) return 0;
+size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t N, int64_t K, int type) {
+  if (M <= 0 || M > kW4MaxRows || N <= 0 || K <= 0 || N > INT32_MAX || K > INT32_MAX || type_bytes(type) == 0) return 0;
+  if (mv_resident(M, N, K, type)) return 0;
   return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int2);
 }
 
@@ -1124,7 +1204,7 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   B2_REQUIRE(y != nullptr && (K == 0 || x != nullptr), B2_ERR_INVALID_ARG, "b2_w4_matvec: x or y is NULL");
   B2_REQUIRE((((uintptr_t)x | (uintptr_t)y) & (tb - 1)) == 0, B2_ERR_INVALID_ARG, "b2_w4_matvec: x or y is not aligned to its type");
   B2_REQUIRE(!matrices_overlap(x, M, K * tb, ldx * tb, y, M, N * tb, ldy * tb), B2_ERR_INVALID_ARG, "b2_w4_matvec: y overlaps x");
-  const size_t need = b2_w4_matvec_workspace_bytes(M, K, type);
+  const size_t need = b2_w4_matvec_workspace_bytes(M, N, K, type);
   B2_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), B2_ERR_WORKSPACE,
              "b2_w4_matvec: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   B2_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, B2_ERR_INVALID_ARG, "b2_w4_matvec: workspace is not 16-byte aligned");
@@ -1139,21 +1219,22 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   a.parts = mv_parts(type);
   a.rows_per_item = mv_rows(nb, type);
   a.chunks = (int)((a.K + kMvChunk - 1) / kMvChunk);
-  if (a.chunks > 0) {
+  a.vec = (((uintptr_t)x | (uintptr_t)(ldx * tb)) & 15) == 0;
+  const bool resident = mv_resident(M, N, K, type);
+  if (a.chunks > 0 && !resident) {
     unsigned char *image = (unsigned char *)workspace;
     int2 *info = (int2 *)(image + mv_image_bytes(M, K, type));
     a.image = image, a.row_info = info;
-    const int vec = (((uintptr_t)x | (uintptr_t)(ldx * tb)) & 15) == 0;
     with_type(type, [&](auto t) {
       using T = decltype(t);
-      w4_x_kernel<T><<<(unsigned)M, kMvXThreads, 0, s>>>(K, ldx, vec, (const T *)x, a.chunks, nb, a.rows_per_item,
+      w4_x_kernel<T><<<(unsigned)M, kMvXThreads, 0, s>>>(K, ldx, a.vec, (const T *)x, a.chunks, nb, a.rows_per_item,
                                                          a.group_shift < 7 ? a.group_shift : 7, image, info);
       return 0;
     });
     B2_CUDA(cudaGetLastError());
   }
   const bool aligned = (((uintptr_t)codes | (uintptr_t)ldq) & 15) == 0;
-  return aligned ? w4_matvec_blocks<true>(ctx, a, nb, s) : w4_matvec_blocks<false>(ctx, a, nb, s);
+  return aligned ? w4_matvec_blocks<true>(ctx, a, nb, resident, s) : w4_matvec_blocks<false>(ctx, a, nb, resident, s);
 }
 
 }  // extern "C"

@@ -9,6 +9,8 @@ dimension given by name (in elements; ``ldq`` in bytes) takes the tensor as raw 
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -49,6 +51,8 @@ def _same_type(t, dtype, name):
 
 def _matrix(t, rows, cols, ld, name, device):
     """(address, leading dimension) of a rows x cols matrix held by ``t``."""
+    if ld is None and isinstance(t, torch.Tensor) and t.get_device() == device and t.shape == (rows, cols) and t.is_contiguous():
+        return t.data_ptr(), cols      # the usual case, first
     _tensor(t, name, device)
     if ld is None:
         if t.dim() > 1 and t.shape[-1] != cols:
@@ -71,6 +75,8 @@ def _vector(t, n, name, device, dtype=None):
     """Address of a contiguous vector of at least n elements, or None."""
     if t is None:
         return None
+    if isinstance(t, torch.Tensor) and t.get_device() == device and t.is_contiguous() and t.numel() >= n and (dtype is None or t.dtype is dtype):
+        return t.data_ptr()            # the usual case, first
     _tensor(t, name, device)
     if dtype is not None:
         _same_type(t, dtype, name)
@@ -208,16 +214,21 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
     return W
 
 
-def w4_matvec_workspace_bytes(M: int, K: int, dtype) -> int:
-    """Bytes that ``w4_matvec`` lays x out in."""
-    return int(_lib.load().b2_w4_matvec_workspace_bytes(M, K, TYPE_CODES[dtype]))
+@functools.lru_cache(maxsize=4096)
+def _w4_matvec_workspace(M, N, K, t) -> int:
+    return int(_lib.load().b2_w4_matvec_workspace_bytes(M, N, K, t))
+
+
+def w4_matvec_workspace_bytes(M: int, N: int, K: int, dtype) -> int:
+    """Bytes that ``w4_matvec`` lays x out in; 0 for smaller products."""
+    return _w4_matvec_workspace(M, N, K, TYPE_CODES[dtype])
 
 
 def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, ldx=None, ldy=None, ldq=None,
               workspace=None, handle: Handle | None = None):
     """y = alpha * x * W^T + beta * y with W (N x K) in 4-bit form, x (M x K) and y (M x N) of one type, M = 0..64 rows (more:
     ``w4_dequantize`` once and ``sgemm``).  ``y`` None: a new tensor (beta must be 0).  ``workspace``: a tensor of at least
-    ``w4_matvec_workspace_bytes(M, K, x.dtype)`` bytes that no other call uses meanwhile; None takes one from torch's allocator
+    ``w4_matvec_workspace_bytes(M, N, K, x.dtype)`` bytes that no other call uses meanwhile; None takes one from torch's allocator
     on the current stream for this call.  Returns ``y``."""
     _tensor(x, "x")
     device = torch.cuda.current_device()
@@ -230,10 +241,14 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
     py, ldy = _matrix(y, M, N, ldy, "y", device)
     _same_type(y, x.dtype, "y")
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
-    L = _lib.load()
+    ws, ws_bytes = None, 0
     if workspace is None:
-        workspace = torch.empty(L.b2_w4_matvec_workspace_bytes(M, K, t), dtype=torch.uint8, device=x.device)
-    ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
+        ws_bytes = _w4_matvec_workspace(M, N, K, t)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+            ws = workspace.data_ptr()
+    else:
+        ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
     h = handle or default_handle()
-    check(L.b2_w4_matvec(h.raw, M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
+    check(_lib.load().b2_w4_matvec(h.raw, M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
     return y

@@ -267,10 +267,10 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
  * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
  * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm.  y must not overlap x.
  * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.
- * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, K, type) bytes (16 to 272 KB for K = 4096) that no other call
- * uses meanwhile; x is laid out there for the tensor cores first.  A bounded wait that runs out on the device is left for
- * b2_check_status as for the SGEMM. */
-size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t K, int type);
+ * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, N, K, type) bytes that no other call uses meanwhile, where x is
+ * laid out for the tensor cores first; 0 (NULL will do) for smaller products, whose kernel lays it out itself.  A bounded wait
+ * that runs out on the device is left for b2_check_status as for the SGEMM. */
+size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t N, int64_t K, int type);
 int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
                  const uint8_t *codes, int64_t ldq, int scale_type, const void *scales, const uint8_t *zeros, float beta,
                  void *y, int64_t ldy, void *workspace, size_t workspace_bytes, void *stream);

@@ -103,7 +103,8 @@ def test_w4_dequantize_refuses(L, bad):
 
 
 @pytest.mark.parametrize("bad", SHARED + [dict(M=-1), dict(ldx=63), dict(ldy=3), dict(x=NULL), dict(y=NULL), dict(x=at(0x1002)),
-                                          dict(y=at(0x1000)), dict(y=at(0x1100)), dict(ws=at(0x10008))])
+                                          dict(y=at(0x1000)), dict(y=at(0x1100)),
+                                          dict(M=60, x=at(0x100000), y=at(0x200000), ws=at(0x10008))])
 def test_w4_matvec_refuses(L, bad):
     assert matvec(L, **bad) == INVALID
     assert L.b2_last_error()
@@ -116,12 +117,14 @@ def test_w4_matvec_refuses_many_rows(L):
 
 def test_w4_matvec_workspace(L):
     for type_ in (F32, BF16, F16):
-        need = L.b2_w4_matvec_workspace_bytes(2, 64, type_)
+        need = L.b2_w4_matvec_workspace_bytes(60, 4, 64, type_)
         assert need > 0
-        assert matvec(L, type_=type_, nws=need - 1) == WORKSPACE
-        assert matvec(L, type_=type_, ws=NULL) == WORKSPACE
-    assert L.b2_w4_matvec_workspace_bytes(0, 64, F32) == 0 and L.b2_w4_matvec_workspace_bytes(4, 0, F32) == 0
-    assert L.b2_w4_matvec_workspace_bytes(4, 64, 7) == 0
+        rows = dict(M=60, type_=type_, x=at(0x100000), y=at(0x200000))
+        assert matvec(L, nws=need - 1, **rows) == WORKSPACE
+        assert matvec(L, ws=NULL, **rows) == WORKSPACE
+        assert L.b2_w4_matvec_workspace_bytes(1, 4, 64, type_) == 0        # a small product needs none
+    assert L.b2_w4_matvec_workspace_bytes(0, 4, 64, F32) == 0 and L.b2_w4_matvec_workspace_bytes(60, 4, 0, F32) == 0
+    assert L.b2_w4_matvec_workspace_bytes(60, 4, 64, 7) == 0
 
 
 def test_w4_empty_calls_are_no_ops(L):
