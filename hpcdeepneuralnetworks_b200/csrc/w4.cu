@@ -396,12 +396,12 @@ static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
 // Whether a product's CTAs lay x out themselves (RESIDENT): each keeps its part of k, cut over clusters of up to 8, in shared
 // memory.  That saves a kernel and a workspace, and costs the same work in every row block's CTAs.
 constexpr int kMvResidentBytes = 35 * 1024;
-constexpr int64_t kMvResidentWork = 4096;      // row blocks x chunks x column blocks
+constexpr int64_t kMvResidentWork = 600;       // row blocks x chunks (16 KB of codes each)
 static bool mv_resident(int64_t M, int64_t N, int64_t K, int type) {
   const int nb = mv_blocks(M, type);
   const int64_t chunks = (K + kMvChunk - 1) / kMvChunk, per_cta = (chunks + 7) / 8;
   const int64_t blocks = (N + kMvRows - 1) / kMvRows;
-  return nb <= 2 && per_cta * nb * (kMvChunk * 8 * 2 + 256) <= kMvResidentBytes && blocks * chunks * nb <= kMvResidentWork;
+  return nb == 1 && per_cta * (kMvChunk * 8 * 2 + 256) <= kMvResidentBytes && blocks * chunks <= kMvResidentWork;
 }
 
 struct MvArgs {
@@ -570,6 +570,12 @@ __device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mv_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // d = a * b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // A tensor map of `rows` rows of `cols` bytes, `pitch` bytes apart, in boxes of 128 bytes x box_rows.
 static int mv_map(CUtensorMap *out, const void *base, int64_t cols, int64_t rows, int64_t pitch, int box_rows) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -603,6 +609,21 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ uint32_t ld_shared_32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 ld_shared_128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 ld_shared_f32x2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) { return __uint_as_float(ld_shared_cluster_u32(cluster_addr)); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -615,9 +636,12 @@ struct MvWait {
   unsigned int seq;
   bool alive = true;
   __device__ __forceinline__ void operator()(uint64_t *bar, uint32_t parity) {
+    if (!mbar_try_wait(bar, parity)) slow(bar, parity);
+  }
+  __device__ __noinline__ void slow(uint64_t *bar, uint32_t parity) {
     if (alive && !mbar_wait(bar, parity)) fail();
   }
-  __device__ __forceinline__ void cluster(uint64_t *bar, uint32_t parity) {
+  __device__ __noinline__ void cluster(uint64_t *bar, uint32_t parity) {
     if (!alive || mbar_try_wait_cluster(bar, parity)) return;
     const uint64_t t0 = global_timer_ns();
     for (uint32_t i = 1; i < (1u << 22); ++i) {
@@ -663,7 +687,8 @@ __device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, i
 
 // ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
 // RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
-template <int NB, bool ALIGNED, bool RESIDENT>
+// BLOCKS: blocks of 32 k in a group, or in the 128 of a longer one that a warp multiplies.
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS>
 __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
   using Tile = MvTile<NB, RESIDENT>;
@@ -747,32 +772,43 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
         const int64_t n0 = (int64_t)(item % a.row_blocks) * kMvRows, n_rows = a.N - n0;
         for (int c = 0; c < chunks; ++c) {
           if ((c & ((1 << window_log) - 1)) == 0) {
-            // scales and zero points of a window: entry e is group e & 7 of row e >> 3; all loads before the first use
-            constexpr int kTurns = (kMvWindow + kFillers - 1) / kFillers;
+            // scales and zero points of a window: entry e is group e & 7 of row e >> 3, so a thread's group stays the same and
+            // its rows lie kFillers / 8 apart; all loads before the first use
+            constexpr int kTurns = (kMvWindow + kFillers - 1) / kFillers, kRowStep = kFillers / 8;
             uint32_t scale[kTurns], zero[kTurns];
-            const int64_t q0 = ((int64_t)(first + c) * kMvChunk) >> a.group_shift;
-            const int count = a.groups - q0 < 8 ? (int)(a.groups - q0) : 8;
-            const int64_t base = n0 * a.groups + q0;
+            const int64_t q = (((int64_t)(first + c) * kMvChunk) >> a.group_shift) + (me & 7);
+            const int rows = n_rows < kMvRows ? (int)n_rows : kMvRows, mine = q < a.groups ? rows - (me >> 3) : 0;      // rows left
+            const int64_t at = (n0 + (me >> 3)) * a.groups + q, row_step = kRowStep * a.groups;
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-              const int e = me + i * kFillers, r = e >> 3, q = e & 7;
-              const bool in = e < kMvWindow && r < n_rows && q < count;
-              const int64_t at = in ? base + r * a.groups + q : 0;
-              scale[i] = a.scale_type == B2_F32 ? ((const uint32_t *)a.scales)[at] : ((const uint16_t *)a.scales)[at];
-              zero[i] = a.zeros ? a.zeros[at] : 8;
-              if (!in) scale[i] = 0;
+            for (int i = 0; i < kTurns; ++i) scale[i] = 0, zero[i] = 8;
+            if (a.scale_type == B2_F32) {
+              const uint32_t *from = (const uint32_t *)a.scales + at;
+#pragma unroll
+              for (int i = 0; i < kTurns; ++i, from += row_step)
+                if (i * kRowStep < mine) scale[i] = *from;
+            } else {
+              const uint16_t *from = (const uint16_t *)a.scales + at;
+#pragma unroll
+              for (int i = 0; i < kTurns; ++i, from += row_step)
+                if (i * kRowStep < mine) scale[i] = *from;
+            }
+            if (a.zeros) {
+              const uint8_t *from = a.zeros + at;
+#pragma unroll
+              for (int i = 0; i < kTurns; ++i, from += row_step)
+                if (i * kRowStep < mine) zero[i] = *from & 15;
             }
             if (opened >= kMvWindows) wait(&wempty[window.at], window.phase ^ 1);
             ++opened;
-            float2 *to = windows + window.at * kMvWindow;
+            float2 *to = windows + window.at * kMvWindow + me;
+            if (a.scale_type != B2_F32) {
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-              const int e = me + i * kFillers;
-              const float s = a.scale_type == B2_F32    ? __uint_as_float(scale[i])
-                              : a.scale_type == B2_BF16 ? __uint_as_float(scale[i] << 16)
-                                                        : __half2float(__ushort_as_half((unsigned short)scale[i]));
-              if (e < kMvWindow) to[e] = make_float2(s, (float)(zero[i] & 15));
+              for (int i = 0; i < kTurns; ++i)
+                scale[i] = a.scale_type == B2_BF16 ? scale[i] << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)scale[i])));
             }
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i)
+              if ((i + 1) * kFillers <= kMvWindow || me + i * kFillers < kMvWindow) to[i * kFillers] = make_float2(__uint_as_float(scale[i]), (float)zero[i]);
             mbar_arrive(&wfull[window.at]);
             window.next();
           }
@@ -797,9 +833,12 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     cluster_wait();
   } else {
     const int g = lane >> 2, t = lane & 3, wn = warp & 3, wk = warp >> 2;
-    const int parts_log = a.group_shift < 7 ? a.group_shift - 5 : 2;      // blocks of 32 in a part of a group
     uint32_t turn = 0;
     MvRing ring(a.stages), window(kMvWindows);
+    const uint32_t smem_base = smem_u32(smem), xs_base = smem_u32(xs), windows_base = smem_u32(windows + ((wn * 32 + g) << 3));
+    uint32_t place[4];        // of this thread's words of row wn * 32 + g (and, at fixed distances, g + 8, ...) in a stage
+#pragma unroll
+    for (int b4 = 0; b4 < 4; ++b4) place[b4] = (wn * 32 + g) * kMvRowBytes + (((wk * 4 + b4) ^ g) << 4) + 4 * t;
     if constexpr (RESIDENT) {
       // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8.  Each
       // row is scaled by its largest element here; the sums are scaled back before they leave the CTA.
@@ -839,46 +878,47 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
         const int in_window = c & ((1 << window_log) - 1);
         if (in_window == 0) wait(&wfull[window.at], window.phase);
         wait(&full[ring.at], ring.phase);
-        const unsigned char *const stage = smem + ring.at * Tile::kStage;
-        const unsigned char *codes = stage + (wn * 32 + g) * kMvRowBytes + 4 * t;
-        const unsigned char *const image = RESIDENT ? xs + c * Tile::kXBytes : stage + kMvCodeBytes;
-        const uint4 *xf = reinterpret_cast<const uint4 *>(image) + wk * 4 * NB * 32 + lane;
-        const float *xsum = reinterpret_cast<const float *>(image + NB * (kMvChunk * 8 * 2)) + 2 * t;
-        const float2 *sz = windows + window.at * kMvWindow + ((wn * 32 + g) << 3);
-        const int block0 = in_window * 8 + wk * 4;                    // this warp's first block of 32 k within the window
-        // the warp's 128 k in straight-line code, BLOCKS blocks of 32 to a group (or to the warp's part of one)
-        auto multiply = [&](auto blocks) {
-          constexpr int BLOCKS = decltype(blocks)::value;
+        const uint32_t stage = smem_base + ring.at * Tile::kStage;
+        const uint32_t image = RESIDENT ? xs_base + c * Tile::kXBytes : stage + kMvCodeBytes;
+        const uint32_t xf = image + (wk * 4 * NB * 32 + lane) * 16;
+        const uint32_t xsum = image + NB * (kMvChunk * 8 * 2) + t * 8 + wk * (4 / BLOCKS) * 8 * NB * 4;
+        // this warp's first group of the window
+        const uint32_t sz = windows_base + window.at * (kMvWindow * 8) + (((in_window * 8 + wk * 4) >> window_log) << 3);
+        // the warp's 128 k in straight-line code
+        {
 #pragma unroll
           for (int b0 = 0; b0 < 4; b0 += BLOCKS) {
-            float acc[2][NB][4] = {};
+            float acc[2][NB][4];
 #pragma unroll
             for (int b4 = b0; b4 < b0 + BLOCKS; ++b4) {
               uint4 xv[NB];
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) xv[nb] = xf[(b4 * NB + nb) * 32];
+              for (int nb = 0; nb < NB; ++nb) xv[nb] = ld_shared_128(xf + (b4 * NB + nb) * 512);
+              const uint32_t at = stage + place[b4];
 #pragma unroll
               for (int rt = 0; rt < 2; ++rt) {
-                const int place = ((wk * 4 + b4) ^ g) << 4;           // rows g, g + 8, ... have one place
-                const uint32_t w0 = *reinterpret_cast<const uint32_t *>(codes + (rt * 16) * kMvRowBytes + place);
-                const uint32_t w1 = *reinterpret_cast<const uint32_t *>(codes + (rt * 16 + 8) * kMvRowBytes + place);
+                const uint32_t w0 = ld_shared_32(at + rt * 16 * kMvRowBytes), w1 = ld_shared_32(at + (rt * 16 + 8) * kMvRowBytes);
                 const uint32_t f[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                for (int nb = 0; nb < NB; ++nb) {
+                  if (b4 == b0) mv_mma_first(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                  else mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                }
                 const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
                 const uint32_t h[4] = {v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], h, xv[nb].z, xv[nb].w);
               }
             }
-            const float2 *from = sz + ((block0 + b0) >> window_log);
-            const float *xs = xsum + ((wk * 4 + b0) >> parts_log) * 8 * NB;
+            float2 group[4];                                          // scale and zero point of rows g + 8 r
+#pragma unroll
+            for (int r = 0; r < 4; ++r) group[r] = ld_shared_f32x2(sz + (b0 / BLOCKS) * 8 + r * 8 * 64);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              const float2 x2 = *reinterpret_cast<const float2 *>(xs + nb * 8);
+              const float2 x2 = ld_shared_f32x2(xsum + (b0 / BLOCKS) * 8 * NB * 4 + nb * 32);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
-                const float2 v = from[(8 * r) << 3];                  // scale and zero point of row g + 8 r
+                const float2 v = group[r];
                 float(&tot)[4] = total[r >> 1][nb];
                 const float(&ac)[4] = acc[r >> 1][nb];
                 tot[2 * (r & 1)] = fmaf(v.x, fmaf(-v.y, x2.x, ac[2 * (r & 1)]), tot[2 * (r & 1)]);
@@ -886,10 +926,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
               }
             }
           }
-        };
-        if (a.group_shift >= 7) multiply(std::integral_constant<int, 4>());
-        else if (a.group_shift == 6) multiply(std::integral_constant<int, 2>());
-        else multiply(std::integral_constant<int, 1>());
+        }
         const bool window_ends = in_window == (1 << window_log) - 1 || c + 1 == chunks;
         __syncwarp();
         if (lane == 0) {
@@ -1007,10 +1044,10 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   return B2_OK;
 }
 
-template <int NB, bool ALIGNED, bool RESIDENT>
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   using Tile = MvTile<NB, RESIDENT>;
-  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT>;
+  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
   const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows;
@@ -1063,12 +1100,21 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   return B2_OK;
 }
 
-template <bool ALIGNED>
-static int w4_matvec_blocks(Context *ctx, const MvArgs &a, int nb, bool resident, cudaStream_t s) {
-  if (resident) return nb == 1 ? w4_matvec_launch<1, ALIGNED, true>(ctx, a, s) : w4_matvec_launch<2, ALIGNED, true>(ctx, a, s);
-  return nb == 1   ? w4_matvec_launch<1, ALIGNED, false>(ctx, a, s)
-         : nb == 2 ? w4_matvec_launch<2, ALIGNED, false>(ctx, a, s)
-                   : w4_matvec_launch<4, ALIGNED, false>(ctx, a, s);
+template <int NB, bool RESIDENT>
+static int w4_matvec_groups(Context *ctx, const MvArgs &a, bool aligned, cudaStream_t s) {
+  if (aligned)
+    return a.group_shift == 5   ? w4_matvec_launch<NB, true, RESIDENT, 1>(ctx, a, s)
+           : a.group_shift == 6 ? w4_matvec_launch<NB, true, RESIDENT, 2>(ctx, a, s)
+                                : w4_matvec_launch<NB, true, RESIDENT, 4>(ctx, a, s);
+  return a.group_shift == 5   ? w4_matvec_launch<NB, false, RESIDENT, 1>(ctx, a, s)
+         : a.group_shift == 6 ? w4_matvec_launch<NB, false, RESIDENT, 2>(ctx, a, s)
+                              : w4_matvec_launch<NB, false, RESIDENT, 4>(ctx, a, s);
+}
+static int w4_matvec_run(Context *ctx, const MvArgs &a, int nb, bool resident, bool aligned, cudaStream_t s) {
+  if (resident) return w4_matvec_groups<1, true>(ctx, a, aligned, s);
+  return nb == 1   ? w4_matvec_groups<1, false>(ctx, a, aligned, s)
+         : nb == 2 ? w4_matvec_groups<2, false>(ctx, a, aligned, s)
+                   : w4_matvec_groups<4, false>(ctx, a, aligned, s);
 }
 
 // The workspace of a product: the image of x, then row_info.
@@ -1234,7 +1280,7 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
     B2_CUDA(cudaGetLastError());
   }
   const bool aligned = (((uintptr_t)codes | (uintptr_t)ldq) & 15) == 0;
-  return aligned ? w4_matvec_blocks<true>(ctx, a, nb, resident, s) : w4_matvec_blocks<false>(ctx, a, nb, resident, s);
+  return w4_matvec_run(ctx, a, nb, resident, aligned, s);
 }
 
 }  // extern "C"
