@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .blas import Handle, default_handle
+from .blas import Handle, _default, default_handle
 
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 W4_GROUPS = (32, 64, 128, 256)
@@ -89,15 +89,21 @@ def _params_type(x, params, names):
     """The common element type of the layer norm's parameter tensors that are given: float32 or x's."""
     dtype = None
     for t, name in zip(params, names):
-        if t is None:
+        if t is None or (dtype is not None and isinstance(t, torch.Tensor) and t.dtype is dtype):
             continue
         _tensor(t, name)
         if t.dtype is not torch.float32 and t.dtype is not x.dtype:
             raise TypeError(f"{name}: {t.dtype} is neither float32 nor x's {x.dtype}")
-        if dtype is not None and t.dtype is not dtype:
+        if dtype is not None:
             raise TypeError(f"{name}: {t.dtype} differs from the other parameters' {dtype}")
         dtype = t.dtype
     return TYPE_CODES[dtype if dtype is not None else x.dtype]
+
+
+def _raw(handle, device):
+    """The library's handle: the caller's, or the default one of the device."""
+    h = handle or _default.get(device) or default_handle()
+    return h.raw
 
 
 # ---- layer norm ---------------------------------------------------------------------------------
@@ -114,16 +120,20 @@ def layernorm(rows, cols, eps, x, gamma, beta, y=None, *, mean=None, rstd=None, 
     py, ldy = _matrix(y, rows, cols, ldy, "y", device)
     _same_type(y, x.dtype, "y")
     pt = _params_type(x, (gamma, beta), ("gamma", "beta"))
-    h = handle or default_handle()
-    check(_lib.load().b2_layernorm(h.raw, rows, cols, eps, t, px, ldx, pt, _vector(gamma, cols, "gamma", device),
+    check(_lib.load().b2_layernorm(_raw(handle, device), rows, cols, eps, t, px, ldx, pt, _vector(gamma, cols, "gamma", device),
                                    _vector(beta, cols, "beta", device), py, ldy, _vector(mean, rows, "mean", device, torch.float32),
                                    _vector(rstd, rows, "rstd", device, torch.float32), _stream(device)))
     return y
 
 
-def layernorm_backward_workspace_bytes(rows: int, cols: int) -> int:
-    """Bytes that the sums over rows of ``layernorm_backward`` go through."""
+@functools.lru_cache(maxsize=4096)
+def _layernorm_workspace(rows, cols) -> int:
     return int(_lib.load().b2_layernorm_backward_workspace_bytes(rows, cols))
+
+
+def layernorm_backward_workspace_bytes(rows: int, cols: int) -> int:
+    """Bytes that the sums of ``layernorm_backward`` go through."""
+    return _layernorm_workspace(rows, cols)
 
 
 def layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, *, lddy=None, ldx=None, lddx=None,
@@ -143,13 +153,14 @@ def layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, 
     if dx is not None:
         _same_type(dx, x.dtype, "dx")
     pt = _params_type(x, (gamma, dgamma, dbeta), ("gamma", "dgamma", "dbeta"))
-    ws = ws_bytes = 0
-    if dgamma is not None or dbeta is not None:
-        if workspace is None:
-            workspace = torch.empty(L.b2_layernorm_backward_workspace_bytes(rows, cols), dtype=torch.uint8, device=x.device)
+    ws, ws_bytes = None, 0
+    if workspace is not None:
         ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
-    h = handle or default_handle()
-    check(L.b2_layernorm_backward(h.raw, rows, cols, t, pdy, lddy, px, ldx, pt, _vector(gamma, cols, "gamma", device),
+    elif rows > 0:
+        ws_bytes = _layernorm_workspace(rows, cols)
+        workspace = x.new_empty(-(-ws_bytes // x.element_size()))
+        ws = workspace.data_ptr()
+    check(L.b2_layernorm_backward(_raw(handle, device), rows, cols, t, pdy, lddy, px, ldx, pt, _vector(gamma, cols, "gamma", device),
                                   _vector(mean, rows, "mean", device, torch.float32), _vector(rstd, rows, "rstd", device, torch.float32),
                                   pdx, lddx, _vector(dgamma, cols, "dgamma", device), _vector(dbeta, cols, "dbeta", device),
                                   ws, ws_bytes, _stream(device)))
@@ -192,8 +203,7 @@ def w4_quantize(N, K, group, W, codes, scales, zeros=None, *, ldw=None, ldq=None
     t = _type(W, "W")
     pw, ldw = _matrix(W, N, K, ldw, "W", device)
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
-    h = handle or default_handle()
-    check(_lib.load().b2_w4_quantize(h.raw, N, K, group, t, pw, ldw, pq, ldq, st, ps, pz, _stream(device)))
+    check(_lib.load().b2_w4_quantize(_raw(handle, device), N, K, group, t, pw, ldw, pq, ldq, st, ps, pz, _stream(device)))
     return codes, scales, zeros
 
 
@@ -208,8 +218,7 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
         W = torch.empty((rows, cols), dtype=dtype, device=codes.device)
     pw, ldw = _matrix(W, rows, cols, ldw, "W", device)
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
-    h = handle or default_handle()
-    check(_lib.load().b2_w4_dequantize(h.raw, N, K, group, pq, ldq, st, ps, pz, _type(W, "W"), pw, ldw, 1 if transpose else 0,
+    check(_lib.load().b2_w4_dequantize(_raw(handle, device), N, K, group, pq, ldq, st, ps, pz, _type(W, "W"), pw, ldw, 1 if transpose else 0,
                                        _stream(device)))
     return W
 
@@ -245,10 +254,9 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
     if workspace is None:
         ws_bytes = _w4_matvec_workspace(M, N, K, t)
         if ws_bytes:
-            workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+            workspace = x.new_empty(ws_bytes // x.element_size())      # a multiple of 16 bytes
             ws = workspace.data_ptr()
     else:
         ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
-    h = handle or default_handle()
-    check(_lib.load().b2_w4_matvec(h.raw, M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
+    check(_lib.load().b2_w4_matvec(_raw(handle, device), M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
     return y
