@@ -119,11 +119,19 @@ __device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
 // elements (8 bytes of codes) each: a group's extremes take log2(group / 16) shuffles.  Nearly every element's code is what the
 // magic addition in w4_nearest gives at once: w / s + 1.5 * 2^23 holds it in its low bits.  Elements that are not nearer than
 // s / 2 to their codes' values (with 16-bit weights a third of the warps meet one that is exactly s / 2 away), and all of a group
-// that needs more care (a scale that is 0, tiny or clamped), are given to w4_nearest, one by one.  Without a place to start on 16 bytes (VEC = false: odd pitches, shifted bases) the elements come
-// one by one and the codes go out as bytes.
-template <class T, class S, bool ZEROS, bool VEC>
+// that needs more care (a scale that is 0, tiny or clamped), are given to w4_nearest, one by one.
+// ALIGN: what W's rows and pitch are a multiple of, 16, 4 or 2 bytes.  Below 16 a warp's 512 elements pass through shared memory,
+// so that its accesses lie side by side (8192 x 8190 bf16: 253 us with each lane reading its own elements); likewise its codes
+// where rows of codes do not start on 8 bytes (QVEC = false).
+template <class T, class S, bool ZEROS, int ALIGN, bool QVEC>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, int group_shift, const T *W, int64_t ldw, uint8_t *codes,
                                                           int64_t ldq, S *scales, uint8_t *zeros) {
+  constexpr int PER = ALIGN / (int)sizeof(T) < 1 ? 1 : ALIGN / (int)sizeof(T);      // elements per access of a staged row
+  constexpr int kPitch = 17;
+  __shared__ float staged[ALIGN < 16 ? 8 : 1][ALIGN < 16 ? 32 * kPitch : 1];         // [warp][lane][16]
+  __shared__ uint2 coded[QVEC ? 1 : 8][QVEC ? 1 : 32];
+  const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31, warp = (threadIdx.y * blockDim.x + threadIdx.x) >> 5;
+  const bool wide = blockDim.x >= 32;                                     // a warp's lanes lie in one row
   const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
   const int lanes = 1 << (group_shift - 4);                               // of a group: 2, 4, 8, 16
   const int64_t row_units = groups << (group_shift - 4);                  // units of 16 elements, whole groups
@@ -132,13 +140,50 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
   for (int64_t nb = (int64_t)blockIdx.y * blockDim.y; nb < N; nb += (int64_t)gridDim.y * blockDim.y) {
     const int64_t n = nb + threadIdx.y;
     for (int64_t ub = (int64_t)blockIdx.x * blockDim.x; ub < row_units; ub += (int64_t)gridDim.x * blockDim.x) {
+      if ((ALIGN < 16 || !QVEC) && wide && ub + (threadIdx.x & ~31u) >= row_units) continue;      // a whole warp behind the row
       const int64_t u = ub + threadIdx.x, k0 = u * 16;
       const int64_t left = n < N ? K - k0 : 0;
       const int len = left >= 16 ? 16 : left > 0 ? (int)left : 0;
       const T *w = W + n * ldw + k0;
       float v[16];
-      if (VEC && len == 16) {
+      if (ALIGN == 16 && len == 16) {
         w4_load<T, 16>(v, w);
+      } else if (ALIGN < 16 && wide) {
+        // the warp's elements from k0 of its first lane on
+        const int64_t from = k0 - 16 * lane, behind = n < N ? K - from : 0;
+        const T *row = W + (n < N ? n * ldw + from : 0);
+        const int end = behind > 512 ? 512 : (int)behind;
+        union Access {
+          T e[PER];
+          uint32_t word;
+        } got[16 / PER];
+        if (end == 512) {      // all loads before the first use
+#pragma unroll
+          for (int i = 0; i < 16 / PER; ++i) {
+            const T *p = row + (i * 32 + lane) * PER;
+            if (PER > 1) got[i].word = __ldcs(reinterpret_cast<const unsigned int *>(p));
+            else got[i].e[0] = *p;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 / PER; ++i)
+#pragma unroll
+            for (int q = 0; q < PER; ++q) {
+              const int e = (i * 32 + lane) * PER + q;
+              got[i].e[q] = e < end ? row[e] : from_f32<T>(0.f);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16 / PER; ++i)
+#pragma unroll
+          for (int q = 0; q < PER; ++q) {
+            const int e = (i * 32 + lane) * PER + q;
+            staged[warp][(e >> 4) * kPitch + (e & 15)] = to_f32(got[i].e[q]);
+          }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = staged[warp][lane * kPitch + i];
+        __syncwarp();
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = i < len ? to_f32(w[i]) : 0.f;
@@ -153,7 +198,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
         hi = w4_max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         if (ZEROS) lo = w4_min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       }
-      if (len <= 0) continue;                                             // nothing to write; a group's first lane has elements
+      if (len <= 0 && (QVEC || !wide)) continue;                          // nothing to write; a group's first lane has elements
       const bool bad = !isfinite(hi) || (ZEROS && !isfinite(lo));
       const S stored = bad ? from_f32<S>(__int_as_float(0x7fffffff)) : w4_scale<S>(lo, hi, ZEROS);
       const float scale = to_f32(stored);
@@ -161,7 +206,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
       const float f = w4_prescale(scale), s = scale * f, inv = 1.f / s, half = 0.5f * s;
       float zero = 8.f;
       if (ZEROS && !flat) zero = fminf(fmaxf(w4_nearest(-lo * f, s, half, inv), 0.f), 15.f);
-      if ((u & (lanes - 1)) == 0) {
+      if ((u & (lanes - 1)) == 0 && (QVEC || len > 0)) {
         const int64_t at = n * groups + (u >> (group_shift - 4));
         scales[at] = stored;
         if (ZEROS) zeros[at] = (uint8_t)zero;
@@ -169,6 +214,7 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
       uint32_t out[2] = {0, 0};
       // the quick way: 1.5 * 2^23 + zero - 8 is even or odd as zero is, which only ties would tell apart
       uint32_t unsure = !flat && f == 1.f && (ZEROS || hi * inv < 7.4f) ? 0u : 0xffffu;
+      if (!QVEC && len <= 0) unsure = 0;
       const float magic = 12582912.f;
       const uint64_t inv2 = w4_two(inv, inv), magic2 = w4_two(magic, magic), minus2 = w4_two(-magic, -magic), s2 = w4_two(-s, -s);
       const float least = magic - zero, most = magic + 15.f - zero;
@@ -178,8 +224,8 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
         const uint64_t x = w4_two(v[i], v[i + 1]);
         const uint64_t big = w4_fma(x, inv2, magic2);                     // rounded once, to an integer
         const float2 r = w4_both(w4_fma(w4_add(big, minus2), s2, x));
-        if (!(fabsf(r.x) < half)) unsure |= 1u << i;
-        if (!(fabsf(r.y) < half)) unsure |= 2u << i;
+        if (!(fabsf(r.x) < half) && (QVEC || len > 0)) unsure |= 1u << i;
+        if (!(fabsf(r.y) < half) && (QVEC || len > 0)) unsure |= 2u << i;
         float2 b = w4_both(big);
         if (ZEROS) b = make_float2(fminf(fmaxf(b.x, least), most), fminf(fmaxf(b.y, least), most));
         // (where the quick way is not taken at all these bits are nonsense, and every code is set below)
@@ -197,10 +243,23 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(int64_t N, int64_t K, 
         else out[1] = (out[1] & keep) | fresh;
       }
       uint8_t *to = codes + n * ldq + (k0 >> 1);
-      if (VEC && len == 16) {
+      if (QVEC && len == 16) {
         *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1]);
+        continue;
+      }
+      if (len & 1) out[len >> 3] &= ~(0xf0u << (8 * ((len >> 1) & 3)));     // the half byte behind an odd row is 0
+      if (!QVEC && wide) {
+        coded[warp][lane] = make_uint2(out[0], out[1]);
+        __syncwarp();
+        const unsigned char *bytes = reinterpret_cast<const unsigned char *>(coded[warp]);
+        const int64_t from = (k0 - 16 * lane) >> 1, behind = n < N ? ((K + 1) >> 1) - from : 0;
+        uint8_t *const first = codes + n * ldq + from + lane;
+        const int end = (behind > 256 ? 256 : (int)behind) - lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i * 32 < end) first[i * 32] = bytes[i * 32 + lane];
+        __syncwarp();
       } else {
-        if (len & 1) out[len >> 3] &= ~(0xf0u << (8 * ((len >> 1) & 3)));   // the half byte behind an odd row is 0
         for (int i = 0; 2 * i < len; ++i) to[i] = (uint8_t)(out[i >> 2] >> (8 * (i & 3)));
       }
     }
@@ -222,59 +281,92 @@ __device__ __forceinline__ void w4_expand(float (&v)[8], uint32_t word, float sc
   }
 }
 
-// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight;
-// VEC where words of codes and 16 bytes of W start on their own size.
-template <class T, class S, bool VEC>
+// Four bytes at an offset of a row of `width` bytes that may start anywhere, zero behind its end; no byte outside is touched.
+__device__ __forceinline__ uint32_t w4_word(const uint8_t *row, int64_t at, int64_t width) {
+  const uint8_t *p = row + at;
+  const int skew = (int)((uintptr_t)p & 3);
+  if (at >= 4 && at + 8 <= width) {
+    const uint32_t *q = reinterpret_cast<const uint32_t *>(p - skew);
+    return __funnelshift_r(q[0], q[1], 8 * skew);
+  }
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < width) word |= (uint32_t)p[i] << (8 * i);
+  return word;
+}
+
+// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight.
+// CVEC: words of codes start on 4 bytes.  WVEC: 16 bytes of W start on 16; otherwise a warp's 256 elements pass through shared
+// memory, so that its stores lie side by side (8192 x 8190 bf16: 171 us with each lane writing its own elements).
+template <class T, class S, bool CVEC, bool WVEC>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
                                                             const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
   constexpr int kFlight = 4;
-  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
+  struct alignas(16) Eight {
+    T e[8];
+  };
+  __shared__ Eight staged[WVEC ? 1 : 8][WVEC ? 1 : 32];
+  const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift, width = (K + 1) >> 1;
   const int units = (int)((K + 7) >> 3), step = (int)(gridDim.x * blockDim.x);
-  for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
+  const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31, warp = (threadIdx.y * blockDim.x + threadIdx.x) >> 5;
+  const bool wide = blockDim.x >= 32;                                     // a warp's lanes lie in one row
+  // every thread takes every turn: warps work together
+  for (int64_t nb = (int64_t)blockIdx.y * blockDim.y; nb < N; nb += (int64_t)gridDim.y * blockDim.y) {
+    const int64_t n = nb + threadIdx.y;
+    const int mine = n < N ? units : 0;
     const uint8_t *row = codes + n * ldq;
     const S *scale_row = scales + n * groups;
     const uint8_t *zero_row = zeros ? zeros + n * groups : nullptr;
     T *out = W + n * ldw;
-    for (int64_t u0 = blockIdx.x * blockDim.x + threadIdx.x; u0 < units; u0 += (int64_t)kFlight * step) {
+    for (int64_t ub = (int64_t)blockIdx.x * blockDim.x; ub < units; ub += (int64_t)kFlight * step) {
       uint32_t word[kFlight];
       float scale[kFlight], zero[kFlight];
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
-        const int64_t u = u0 + (int64_t)i * step;
+        const int64_t u = ub + threadIdx.x + (int64_t)i * step;
         word[i] = 0;
-        if (u < units) {
-          if (VEC && 8 * u + 8 <= K) {
-            word[i] = __ldcs(reinterpret_cast<const uint32_t *>(row + 4 * u));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (8 * u + 2 * q < K) word[i] |= (uint32_t)row[4 * u + q] << (8 * q);
-          }
+        scale[i] = zero[i] = 0.f;
+        if (u < mine) {
+          if (CVEC && 8 * u + 8 <= K) word[i] = __ldcs(reinterpret_cast<const unsigned int *>(row + 4 * u));
+          else word[i] = w4_word(row, 4 * u, width);
           scale[i] = to_f32(scale_row[(8 * u) >> group_shift]);
           zero[i] = zero_row ? (float)(zero_row[(8 * u) >> group_shift] & 15) : 8.f;
         }
       }
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
-        const int64_t u = u0 + (int64_t)i * step;
-        if (u < units) {
-          float v[8];
-          w4_expand(v, word[i], scale[i], zero[i]);
-          union {
-            T e[8];
-            uint4 q[sizeof(T) / 2];
-          } o;
+        const int64_t u = ub + threadIdx.x + (int64_t)i * step;
+        if (ub + (int64_t)i * step >= units) break;                       // for the whole block
+        float v[8];
+        w4_expand(v, word[i], scale[i], zero[i]);
+        union {
+          Eight all;
+          uint4 q[sizeof(T) / 2];
+        } o;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o.e[k] = from_f32<T>(v[k]);
-          T *to = out + 8 * u;
-          if (VEC && 8 * u + 8 <= K) {
+        for (int k = 0; k < 8; ++k) o.all.e[k] = from_f32<T>(v[k]);
+        T *to = out + 8 * u;
+        if (WVEC && 8 * u + 8 <= K) {
+          if (u < mine) {
 #pragma unroll
             for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4 *>(to) + q, o.q[q]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (8 * u + k < K) to[k] = o.e[k];
           }
+        } else if (!WVEC && wide) {
+          staged[warp][lane] = o.all;
+          __syncwarp();
+          const T *flat = reinterpret_cast<const T *>(staged[warp]);
+          const int64_t from = 8 * (u - lane), behind = n < N ? K - from : 0;
+          T *const first = out + from + lane;
+          const int end = (behind > 256 ? 256 : (int)behind) - lane;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k * 32 < end) first[k * 32] = flat[k * 32 + lane];
+          __syncwarp();
+        } else if (u < mine) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (8 * u + k < K) to[k] = o.all.e[k];
         }
       }
     }
@@ -418,35 +510,6 @@ struct MvArgs {
   int *status;
   unsigned int seq;
 };
-
-// Bytes [at, at + 16) of a row of `width` bytes that may start anywhere, zero behind its end, without touching a byte outside.
-__device__ __forceinline__ uint4 mv_load_any(const uint8_t *row, int64_t at, int64_t width) {
-  union {
-    uint32_t w[4];
-    uint4 v;
-  } out;
-  const uint8_t *p = row + at;
-  const int skew = (int)((uintptr_t)p & 3);
-  if (at >= 4 && at + 20 <= width) {
-    const uint32_t *q = reinterpret_cast<const uint32_t *>(p - skew);
-    uint32_t prev = q[0];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t next = q[i + 1];
-      out.w[i] = __funnelshift_r(prev, next, 8 * skew);
-      prev = next;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      out.w[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (at + 4 * i + j < width) out.w[i] |= (uint32_t)p[4 * i + j] << (8 * j);
-    }
-  }
-  return out.v;
-}
 
 // x[k .. k + 8) of a row in FP32, zero behind K.
 template <class T>
@@ -817,11 +880,40 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             ++filled;
             unsigned char *stage = smem + ring.at * Tile::kStage;
             const int64_t at = (int64_t)(first + c) * kMvRowBytes, width = (a.K + 1) >> 1;
-            for (int u = me; u < kMvCodeBytes / 16; u += kFillers) {
-              const int r = u >> 3, cc = u & 7;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (r < n_rows && at + 16 * cc < width) v = mv_load_any(a.codes + (n0 + r) * a.ldq, at + 16 * cc, width);
-              *reinterpret_cast<uint4 *>(stage + r * kMvRowBytes + ((cc ^ (r & 7)) << 4)) = v;
+            // 16-byte units, a thread's of one column and rows kFillers / 8 apart, four in flight; five words each inside a row
+            constexpr int kFlight = 4, kTurns = (kMvRows * 8 + kFillers - 1) / kFillers;
+            const int cc = me & 7;
+            const int64_t byte = at + 16 * cc;
+            const bool inside = byte >= 4 && byte + 20 <= width;
+            const int rows = byte < width ? (n_rows < kMvRows ? (int)n_rows : kMvRows) : 0;
+            for (int i0 = 0; i0 < kTurns; i0 += kFlight) {
+              uint32_t w[kFlight][5];
+#pragma unroll
+              for (int i = 0; i < kFlight; ++i) {
+                const int r = (me >> 3) + (i0 + i) * (kFillers / 8);
+                const uint8_t *p = a.codes + (n0 + r) * a.ldq + byte;
+                if (inside && r < rows) {
+                  const uint32_t *q = reinterpret_cast<const uint32_t *>(p - ((uintptr_t)p & 3));
+#pragma unroll
+                  for (int k = 0; k < 5; ++k) w[i][k] = q[k];
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < kFlight; ++i) {
+                const int r = (me >> 3) + (i0 + i) * (kFillers / 8);
+                if (r >= kMvRows) break;
+                const uint8_t *row = a.codes + (n0 + r) * a.ldq;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < rows) {
+                  const int skew = 8 * (int)((uintptr_t)(row + byte) & 3);
+                  if (inside)
+                    v = make_uint4(__funnelshift_r(w[i][0], w[i][1], skew), __funnelshift_r(w[i][1], w[i][2], skew),
+                                   __funnelshift_r(w[i][2], w[i][3], skew), __funnelshift_r(w[i][3], w[i][4], skew));
+                  else v = make_uint4(w4_word(row, byte, width), w4_word(row, byte + 4, width), w4_word(row, byte + 8, width),
+                                      w4_word(row, byte + 12, width));
+                }
+                *reinterpret_cast<uint4 *>(stage + r * kMvRowBytes + ((cc ^ (r & 7)) << 4)) = v;
+              }
             }
             mbar_arrive(&full[ring.at]);
             ring.next();
@@ -1182,12 +1274,20 @@ int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const
   const int shift = w4_group_shift(group);
   const int64_t units = ((K + group - 1) / group) * (group / 16);
   const W4Grid g(units, N, group / 16);
-  const bool vec = (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0 && (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
+  const uintptr_t place = (uintptr_t)W | (uintptr_t)(ldw * tb);
+  const int align = (place & 15) == 0 ? 16 : (place & 3) == 0 ? 4 : 2;
+  const bool qvec = (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
-    const auto kernel = zeros ? (vec ? w4_quantize_kernel<T, S, true, true> : w4_quantize_kernel<T, S, true, false>)
-                              : (vec ? w4_quantize_kernel<T, S, false, true> : w4_quantize_kernel<T, S, false, false>);
+    constexpr int kLeast = sizeof(T) == 4 ? 4 : 2;
+    const auto pick = [&](auto z) {
+      constexpr bool Z = decltype(z)::value;
+      return align == 16  ? (qvec ? w4_quantize_kernel<T, S, Z, 16, true> : w4_quantize_kernel<T, S, Z, 16, false>)
+             : align == 4 ? (qvec ? w4_quantize_kernel<T, S, Z, 4, true> : w4_quantize_kernel<T, S, Z, 4, false>)
+                          : (qvec ? w4_quantize_kernel<T, S, Z, kLeast, true> : w4_quantize_kernel<T, S, Z, kLeast, false>);
+    };
+    const auto kernel = zeros ? pick(std::true_type()) : pick(std::false_type());
     kernel<<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
   });
   B2_CUDA(cudaGetLastError());
@@ -1221,9 +1321,10 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
       kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
     } else {
       const W4Grid g((K + 31) / 32, N, 1);      // four units of 8 to a thread
-      const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 3) == 0 && (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0;
-      if (vec) w4_dequantize_kernel<T, S, true><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
-      else w4_dequantize_kernel<T, S, false><<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      const bool cvec = (((uintptr_t)codes | (uintptr_t)ldq) & 3) == 0, wvec = (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0;
+      const auto kernel = cvec ? (wvec ? w4_dequantize_kernel<T, S, true, true> : w4_dequantize_kernel<T, S, true, false>)
+                               : (wvec ? w4_dequantize_kernel<T, S, false, true> : w4_dequantize_kernel<T, S, false, false>);
+      kernel<<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
     }
   });
   B2_CUDA(cudaGetLastError());
