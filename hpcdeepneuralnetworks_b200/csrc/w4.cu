@@ -382,37 +382,44 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
   __shared__ float tile[64][65];                // [k][n]
   const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift;
   const int64_t k_tiles = (K + 63) >> 6, n_tiles = (N + 63) >> 6;
-  for (int64_t at = blockIdx.x; at < k_tiles * n_tiles; at += gridDim.x) {
-    const int64_t n0 = (at % n_tiles) * 64, k0 = (at / n_tiles) * 64;
-    {
-      // thread: row threadIdx.x / 4, 16 codes from (threadIdx.x % 4) * 16 on
-      const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-      const int64_t n = n0 + r, k = k0 + c;
-      uint32_t word[2] = {0, 0};
-      float scale = 0.f, zero = 0.f;
-      if (n < N && k < K) {
-        const uint8_t *from = codes + n * ldq + (k >> 1);
-        if (VEC && k + 16 <= K) {
-          const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(from));
-          word[0] = v.x, word[1] = v.y;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (k + 2 * i < K) word[i >> 2] |= (uint32_t)from[i] << (8 * (i & 3));
-        }
-        const int64_t g = n * groups + (k >> group_shift);
-        scale = to_f32(scales[g]);
-        zero = w4_zero(zeros, g);
+  // thread: row threadIdx.x / 4 of a tile, 16 codes from (threadIdx.x % 4) * 16 on; the next tile's are fetched while this one's go out
+  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+  uint32_t word[2];
+  float scale, zero;
+  auto fetch = [&](int64_t n_tile, int64_t k_tile) {
+    const int64_t n = n_tile * 64 + r, k = k_tile * 64 + c;
+    word[0] = word[1] = 0;
+    scale = zero = 0.f;
+    if (n < N && k < K) {
+      const uint8_t *from = codes + n * ldq + (k >> 1);
+      if (VEC && k + 16 <= K) {
+        const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(from));
+        word[0] = v.x, word[1] = v.y;
+      } else {
+        word[0] = w4_word(codes + n * ldq, k >> 1, (K + 1) >> 1);
+        word[1] = w4_word(codes + n * ldq, (k >> 1) + 4, (K + 1) >> 1);
       }
+      const int64_t g = n * groups + (k >> group_shift);
+      scale = to_f32(scales[g]);
+      zero = w4_zero(zeros, g);
+    }
+  };
+  const int64_t n_step = gridDim.x % n_tiles, k_step = gridDim.x / n_tiles;
+  int64_t n_tile = blockIdx.x % n_tiles, k_tile = blockIdx.x / n_tiles;
+  fetch(n_tile, k_tile);
+  while (k_tile < k_tiles) {
+    const int64_t n0 = n_tile * 64, k0 = k_tile * 64;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float v[8];
-        w4_expand(v, word[h], scale, zero);
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+      w4_expand(v, word[h], scale, zero);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tile[c + 8 * h + i][r] = v[i];
-      }
+      for (int i = 0; i < 8; ++i) tile[c + 8 * h + i][r] = v[i];
     }
     __syncthreads();
+    n_tile += n_step, k_tile += k_step;
+    if (n_tile >= n_tiles) n_tile -= n_tiles, ++k_tile;
+    fetch(n_tile, k_tile);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -1311,7 +1318,7 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
     using T = decltype(t);
     using S = decltype(s);
     if (transpose) {
-      const int64_t tiles = ((N + 63) / 64) * ((K + 63) / 64), most = (int64_t)ctx->sm_count * 64;
+      const int64_t tiles = ((N + 63) / 64) * ((K + 63) / 64), most = (int64_t)ctx->sm_count * 8;
       const unsigned grid = (unsigned)(tiles < most ? tiles : most);
       const bool vec = (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
       constexpr bool kPair = sizeof(T) == 2;
