@@ -462,6 +462,10 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 // element above 2^-28 of the largest (bf16 and FP16 in one term, FP32 in three terms of 11 bits, a column of the tile each), and
 // what lies below is off by 2^-39 of the largest at most: nothing beside the FP32 sums.  All products are exact in FP32; group
 // sums, scales and zero points are FP32.  The same kernel sums x over each group.
+// sum c x is larger than sum (c - z) x, and the tensor cores cut where they add: results in 16 bits do not show it, FP32 ones
+// would (2.6e-6 of the result's norm, against 5e-7 for a product of FP32 matrices).  So for FP32 x (EXACT) the zero point is
+// taken off while unpacking, in four more instructions per word: under 1024's upper bits a code reads 1024 + c, or 1024 + 16 c,
+// and a subtraction or an FMA with 1/16 leaves c - z exactly.
 // An infinity or NaN in x would make z * sum_k x meaningless: such elements count as 0 above and are added, with their exact
 // weights, by the thread that writes the output (w4 rows flagged so are slow).
 //
@@ -555,9 +559,10 @@ __device__ __forceinline__ void mv_look(const float (&e)[8], float &top, bool &b
 // a longer one that a warp multiplies).
 __device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8], int u, int nb, int col0, int parts, int part_log, float f1,
                                        float f2) {
+  const bool exact = parts > 1;              // FP32: no division of the odd elements, no sums
   float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) ? 0.0625f : 1.f) : 0.f;
+  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) && !exact ? 0.0625f : 1.f) : 0.f;
   for (int p = 0; p < parts; ++p) {
     const int col = col0 + p;
     __half h[8];
@@ -576,6 +581,7 @@ __device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8]
 #pragma unroll
     for (int i = 0; i < 4; ++i) out.h2[i] = __halves2half2(h[i], h[i + 4]);
     reinterpret_cast<uint4 *>(chunk)[(((u >> 2) * nb + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = out.q;
+    if (exact) continue;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1)
       if (o < (1 << (part_log - 3))) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -634,10 +640,29 @@ __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ld
   }
 }
 
+// (w & mask) | bits in one instruction (left to itself the compiler makes two of it, having two constants)
+__device__ __forceinline__ uint32_t mv_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
 __device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// c - z of a word's codes 0 and 4 (even: in the lowest bits of its halves), or 1 and 5 (odd: four bits up), from 1024 + z.
+__device__ __forceinline__ uint32_t mv_even(uint32_t w, uint32_t zero) {
+  const uint32_t v = mv_and_or(w, 0x000f000fu, 0x64006400u);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&zero));
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t mv_odd(uint32_t w, uint32_t zero) {
+  const uint32_t v = mv_and_or(w, 0x00f000f0u, 0x64006400u);
+  const __half2 less = __hsub2(__float2half2_rn(960.f), *reinterpret_cast<const __half2 *>(&zero));      // -(64 + z)
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&v), __float2half2_rn(0.0625f), less);
+  return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 __device__ __forceinline__ void mv_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // d = a * b
@@ -758,7 +783,7 @@ __device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, i
 // ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
 // RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
 // BLOCKS: blocks of 32 k in a group, or in the 128 of a longer one that a warp multiplies.
-template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS>
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
 __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
   using Tile = MvTile<NB, RESIDENT>;
@@ -770,7 +795,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
   int chunks = a.chunks - first;
   chunks = chunks < 0 ? 0 : chunks < a.chunks_per_cta ? chunks : a.chunks_per_cta;
   const int window_log = a.group_shift - 5;                                // chunks of a window: group / 32
-  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, zero point
+  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, zero point (EXACT: 1024 + z, twice in FP16)
   unsigned char *const xs = reinterpret_cast<unsigned char *>(windows + kMvWindows * kMvWindow);   // RESIDENT: [chunk][kXBytes]
   float *const sums = reinterpret_cast<float *>(xs + (RESIDENT ? a.chunks_per_cta * Tile::kXBytes : 0));   // [2][8 NB][kMvPitch]
   uint64_t *const full = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sums) + Tile::kSumBytes);
@@ -878,7 +903,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             }
 #pragma unroll
             for (int i = 0; i < kTurns; ++i)
-              if ((i + 1) * kFillers <= kMvWindow || me + i * kFillers < kMvWindow) to[i * kFillers] = make_float2(__uint_as_float(scale[i]), (float)zero[i]);
+              if ((i + 1) * kFillers <= kMvWindow || me + i * kFillers < kMvWindow) to[i * kFillers] = make_float2(__uint_as_float(scale[i]), EXACT ? __uint_as_float(0x64006400u + zero[i] * 0x00010001u) : (float)zero[i]);
             mbar_arrive(&wfull[window.at]);
             window.next();
           }
@@ -973,7 +998,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     for (int item = blockIdx.x; item < a.items; item += gridDim.x, ++turn) {
       const int mc = item / a.row_blocks;
       float total[2][NB][4] = {};
-#pragma unroll 2
+#pragma unroll (EXACT ? 1 : 2)
       for (int c = 0; c < chunks; ++c) {
         const int in_window = c & ((1 << window_log) - 1);
         if (in_window == 0) wait(&wfull[window.at], window.phase);
@@ -989,6 +1014,9 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
 #pragma unroll
           for (int b0 = 0; b0 < 4; b0 += BLOCKS) {
             float acc[2][NB][4];
+            uint32_t zero[4];                                         // EXACT: of rows g + 8 r
+#pragma unroll
+            for (int r = 0; r < 4; ++r) zero[r] = EXACT ? ld_shared_32(sz + (b0 / BLOCKS) * 8 + r * 8 * 64 + 4) : 0;
 #pragma unroll
             for (int b4 = b0; b4 < b0 + BLOCKS; ++b4) {
               uint4 xv[NB];
@@ -998,14 +1026,21 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
 #pragma unroll
               for (int rt = 0; rt < 2; ++rt) {
                 const uint32_t w0 = ld_shared_32(at + rt * 16 * kMvRowBytes), w1 = ld_shared_32(at + (rt * 16 + 8) * kMvRowBytes);
-                const uint32_t f[4] = {w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u};
+                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+                uint32_t f[4], h[4];
+                if constexpr (EXACT) {
+                  const uint32_t z0 = zero[2 * rt], z1 = zero[2 * rt + 1];
+                  f[0] = mv_even(w0, z0), f[1] = mv_even(w1, z1), f[2] = mv_odd(w0, z0), f[3] = mv_odd(w1, z1);
+                  h[0] = mv_even(v0, z0), h[1] = mv_even(v1, z1), h[2] = mv_odd(v0, z0), h[3] = mv_odd(v1, z1);
+                } else {
+                  f[0] = w0 & 0x000f000fu, f[1] = w1 & 0x000f000fu, f[2] = w0 & 0x00f000f0u, f[3] = w1 & 0x00f000f0u;
+                  h[0] = v0 & 0x000f000fu, h[1] = v1 & 0x000f000fu, h[2] = v0 & 0x00f000f0u, h[3] = v1 & 0x00f000f0u;
+                }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                   if (b4 == b0) mv_mma_first(acc[rt][nb], f, xv[nb].x, xv[nb].y);
                   else mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y);
                 }
-                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-                const uint32_t h[4] = {v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], h, xv[nb].z, xv[nb].w);
               }
@@ -1015,14 +1050,17 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             for (int r = 0; r < 4; ++r) group[r] = ld_shared_f32x2(sz + (b0 / BLOCKS) * 8 + r * 8 * 64);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-              const float2 x2 = ld_shared_f32x2(xsum + (b0 / BLOCKS) * 8 * NB * 4 + nb * 32);
+              const float2 x2 = EXACT ? make_float2(0.f, 0.f) : ld_shared_f32x2(xsum + (b0 / BLOCKS) * 8 * NB * 4 + nb * 32);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const float2 v = group[r];
                 float(&tot)[4] = total[r >> 1][nb];
                 const float(&ac)[4] = acc[r >> 1][nb];
-                tot[2 * (r & 1)] = fmaf(v.x, fmaf(-v.y, x2.x, ac[2 * (r & 1)]), tot[2 * (r & 1)]);
-                tot[2 * (r & 1) + 1] = fmaf(v.x, fmaf(-v.y, x2.y, ac[2 * (r & 1) + 1]), tot[2 * (r & 1) + 1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  const float sum = EXACT ? ac[2 * (r & 1) + i] : fmaf(-v.y, i ? x2.y : x2.x, ac[2 * (r & 1) + i]);
+                  tot[2 * (r & 1) + i] = fmaf(v.x, sum, tot[2 * (r & 1) + i]);
+                }
               }
             }
           }
@@ -1047,7 +1085,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
         for (int i = 0; i < 2; ++i) {
           const int col = nb * 8 + 2 * t + i, m = col / a.parts;
           // RESIDENT: the codes' 2^-24, this CTA's scale of the row and the term's
-          const int up = RESIDENT && m < a.M ? 24 - 11 * (col - m * a.parts) - mv_exponent(__int_as_float(largest[m])) : 0;
+          const int up = RESIDENT && m < a.M ? (EXACT ? 0 : 24) - 11 * (col - m * a.parts) - mv_exponent(__int_as_float(largest[m])) : 0;
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -1093,7 +1131,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             } else {
               s = at[0] + at[8 * NB * kMvPitch];
             }
-            v += RESIDENT ? s : ldexpf(s, 24 - 11 * p - info.x);    // the codes' 2^-24, the row's scale and the term's
+            v += RESIDENT ? s : ldexpf(s, (EXACT ? 0 : 24) - 11 * p - info.x);    // the codes' 2^-24, the row's scale and the term's
           }
           if (info.y) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
         }
@@ -1144,10 +1182,10 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   return B2_OK;
 }
 
-template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS>
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   using Tile = MvTile<NB, RESIDENT>;
-  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS>;
+  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS, EXACT>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
   const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows;
@@ -1200,21 +1238,22 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   return B2_OK;
 }
 
+template <int NB, bool RESIDENT, bool ALIGNED, bool EXACT>
+static int w4_matvec_groups(Context *ctx, const MvArgs &a, cudaStream_t s) {
+  return a.group_shift == 5   ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 1, EXACT>(ctx, a, s)
+         : a.group_shift == 6 ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 2, EXACT>(ctx, a, s)
+                              : w4_matvec_launch<NB, ALIGNED, RESIDENT, 4, EXACT>(ctx, a, s);
+}
 template <int NB, bool RESIDENT>
-static int w4_matvec_groups(Context *ctx, const MvArgs &a, bool aligned, cudaStream_t s) {
-  if (aligned)
-    return a.group_shift == 5   ? w4_matvec_launch<NB, true, RESIDENT, 1>(ctx, a, s)
-           : a.group_shift == 6 ? w4_matvec_launch<NB, true, RESIDENT, 2>(ctx, a, s)
-                                : w4_matvec_launch<NB, true, RESIDENT, 4>(ctx, a, s);
-  return a.group_shift == 5   ? w4_matvec_launch<NB, false, RESIDENT, 1>(ctx, a, s)
-         : a.group_shift == 6 ? w4_matvec_launch<NB, false, RESIDENT, 2>(ctx, a, s)
-                              : w4_matvec_launch<NB, false, RESIDENT, 4>(ctx, a, s);
+static int w4_matvec_forms(Context *ctx, const MvArgs &a, bool aligned, cudaStream_t s) {
+  if (a.parts > 1) return aligned ? w4_matvec_groups<NB, RESIDENT, true, true>(ctx, a, s) : w4_matvec_groups<NB, RESIDENT, false, true>(ctx, a, s);
+  return aligned ? w4_matvec_groups<NB, RESIDENT, true, false>(ctx, a, s) : w4_matvec_groups<NB, RESIDENT, false, false>(ctx, a, s);
 }
 static int w4_matvec_run(Context *ctx, const MvArgs &a, int nb, bool resident, bool aligned, cudaStream_t s) {
-  if (resident) return w4_matvec_groups<1, true>(ctx, a, aligned, s);
-  return nb == 1   ? w4_matvec_groups<1, false>(ctx, a, aligned, s)
-         : nb == 2 ? w4_matvec_groups<2, false>(ctx, a, aligned, s)
-                   : w4_matvec_groups<4, false>(ctx, a, aligned, s);
+  if (resident) return w4_matvec_forms<1, true>(ctx, a, aligned, s);
+  return nb == 1   ? w4_matvec_forms<1, false>(ctx, a, aligned, s)
+         : nb == 2 ? w4_matvec_forms<2, false>(ctx, a, aligned, s)
+                   : w4_matvec_forms<4, false>(ctx, a, aligned, s);
 }
 
 // The workspace of a product: the image of x, then row_info.
