@@ -9,7 +9,6 @@
 #include <initializer_list>
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "types.cuh"
 
@@ -676,8 +675,14 @@ __global__ void __launch_bounds__(1024) layernorm_reduce_kernel(int parts, int c
 constexpr int kLnBlock = 384;           // threads of a block of several teams, forward
 constexpr int kLnHeldBackward = 16;       // elements per thread, backward
 constexpr int kLnLongestBackward = 8192;  // 512 threads of 16 elements, or 1024 of 8
-constexpr int kLnParts = 296;           // most blocks, and lines of partial sums: two blocks on each of 148 SMs
-static int64_t ln_parts(int64_t rows) { return rows < kLnParts ? rows : kLnParts; }
+// Most blocks, and lines of partial sums: two blocks on each of 148 SMs; the longest rows, whose lines are long and whose blocks
+// share the columns, take fewer.
+static int64_t ln_parts(int64_t rows, int64_t cols) {
+  int64_t most = 296;
+  if (cols > kLnLongestBackward) most = most * kLnLongestBackward / cols;
+  if (most < 8) most = 8;
+  return rows < most ? rows : most;
+}
 
 // Whether every address and pitch (in bytes) is a multiple of `bytes`; NULL is.
 static bool ln_multiple(int64_t bytes, std::initializer_list<const void *> pointers, std::initializer_list<int64_t> pitches) {
@@ -690,7 +695,7 @@ static bool ln_multiple(int64_t bytes, std::initializer_list<const void *> point
 // Accesses per thread that take `units` of them over `share` threads.
 static int ln_turns(int64_t units, int share) { return (int)((units + share - 1) / share); }
 
-// Blocks of this size that an SM holds, asked once per kernel, size and device.
+// Blocks of this size that an SM holds, asked once per kernel, size and device (and each time, should the table be full).
 static int ln_blocks_per_sm(const void *kernel, int device, int threads, size_t smem, int *out) {
   struct Entry {
     const void *kernel;
@@ -698,19 +703,21 @@ static int ln_blocks_per_sm(const void *kernel, int device, int threads, size_t 
     size_t smem;
     int blocks;
   };
-  static std::vector<Entry> known;
+  static Entry known[512];
+  static int count = 0;
   static std::mutex mu;
   std::lock_guard<std::mutex> lk(mu);
-  for (const Entry &e : known)
+  for (int i = 0; i < count; ++i) {
+    const Entry &e = known[i];
     if (e.kernel == kernel && e.device == device && e.threads == threads && e.smem == smem) {
       *out = e.blocks;
       return B2_OK;
     }
+  }
   int n = 0;
   B2_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem));
-  if (n < 1) n = 1;
-  known.push_back({kernel, device, threads, smem, n});
-  *out = n;
+  *out = n < 1 ? 1 : n;
+  if (count < (int)(sizeof(known) / sizeof(known[0]))) known[count++] = {kernel, device, threads, smem, *out};
   return B2_OK;
 }
 
@@ -812,7 +819,7 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
 
 size_t b2_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const size_t sums = (size_t)ln_parts(rows) * 2 * (size_t)cols * sizeof(float);
+  const size_t sums = (size_t)ln_parts(rows, cols) * 2 * (size_t)cols * sizeof(float);
   return (sums + 15) / 16 * 16 + (cols > kLnLongestBackward ? (size_t)rows * sizeof(float2) : 0);
 }
 
@@ -854,7 +861,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
     if (dbeta) B2_CUDA(cudaMemsetAsync(dbeta, 0, (size_t)cols * pb, s));
     return B2_OK;
   }
-  int parts = (int)ln_parts(rows);
+  int parts = (int)ln_parts(rows, cols);
   const int width = ln_width(cols, tb, pb, {dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : 0}, {gamma});
   float *partial = sums ? (float *)workspace : nullptr;
   float2 *row_sums = is_long ? (float2 *)((char *)workspace + (need - (size_t)rows * sizeof(float2))) : nullptr;

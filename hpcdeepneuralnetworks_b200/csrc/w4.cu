@@ -3,7 +3,6 @@
 
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "types.cuh"
 
@@ -1134,8 +1133,8 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             v += RESIDENT ? s : ldexpf(s, (EXACT ? 0 : 24) - 11 * p - info.x);    // the codes' 2^-24, the row's scale and the term's
           }
           if (info.y) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
+          v *= a.alpha;
         }
-        v *= a.alpha;
         const int64_t to = (int64_t)(m0 + m) * a.ldy + n0 + r;
         if (a.beta != 0.f) v = fmaf(a.beta, mv_load_any_type(a.y, a.type, to), v);
         if (a.type == B2_F32) ((float *)a.y)[to] = v;
@@ -1150,20 +1149,24 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
   cluster_sync_all();     // nobody leaves while its sums may still be read or its barriers reached
 }
 
-// Clusters of `ctas` CTAs with `smem` bytes each that the device holds at once, asked once per kernel, size and device.
+// Clusters of `ctas` CTAs with `smem` bytes each that the device holds at once, asked once per kernel, size and device (and
+// each time, should the table be full).
 static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *out) {
   struct Entry {
     const void *kernel;
     int device, ctas, smem, clusters;
   };
-  static std::vector<Entry> known;
+  static Entry known[512];
+  static int count = 0;
   static std::mutex mu;
   std::lock_guard<std::mutex> lk(mu);
-  for (const Entry &e : known)
+  for (int i = 0; i < count; ++i) {
+    const Entry &e = known[i];
     if (e.kernel == kernel && e.device == device && e.ctas == ctas && e.smem == smem) {
       *out = e.clusters;
       return B2_OK;
     }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1, (unsigned)ctas);
   cfg.blockDim = dim3(kMvThreads);
@@ -1177,8 +1180,8 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   cfg.numAttrs = 1;
   int n = 0;
   B2_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
-  known.push_back({kernel, device, ctas, smem, n < 1 ? 1 : n});
   *out = n < 1 ? 1 : n;
+  if (count < (int)(sizeof(known) / sizeof(known[0]))) known[count++] = {kernel, device, ctas, smem, *out};
   return B2_OK;
 }
 

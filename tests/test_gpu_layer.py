@@ -10,7 +10,8 @@ difference, the product, the FMA: |dy| <= H|y| + |gamma|*(e_m + u*(D + 8)*|xhat|
 Gradients: mean and rstd are inputs, so xhat carries 2 roundings, u*: dx <= H|dx| + u*rstd*(6|u| + (D + 4)*mean|u| +
 (D + 12)*|xhat|*mean|u xhat|); the sums over R rows D = R + 8 in whatever order.
 Products: fp32 sums of exact products in chains of at most 64 + K/16 additions, two roundings' worth each because the tensor
-cores cut instead of rounding: H|y| + 2u*(64 + K/16)*|alpha|*sum|x||w| + 4u*(|alpha*acc| + |beta*y0|).
+cores cut instead of rounding; sum (c - z) x s may be formed as sum c x s - z sum x s, so each |w| = |c - z| s counts with another
+z s:  H|y| + 2u*(64 + K/16)*|alpha|*sum|x|(|w| + z s) + 4u*(|alpha*acc| + |beta*y0|).
 """
 import pytest
 import torch
@@ -390,9 +391,9 @@ def check_matvec(b2, M, N, K, group, kind, scales, with_zeros, alpha=1.0, beta=0
     w = ref.w4_values(codes, s, z, group)
     acc, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
     want = alpha * acc + beta * y0.double()
-    # with zeros the kernel may subtract the zero point before or after the sums: the magnitudes of both forms
+    # the kernel may take the zero point off before or after the sums: the magnitudes of both forms, |c - z| + z at most
     at = torch.arange(K) // group
-    size = size + x.double().abs() @ (8.0 * s.double()[:, at]).t()
+    size = size + x.double().abs() @ ((8.0 if z is None else z.double()[:, at]) * s.double()[:, at]).t()
     tol = ref.half_step(y.dtype) * want.abs() + 2 * U * (64 + K / 16) * abs(alpha) * size
     tol = tol + 4 * U * ((alpha * acc).abs() + (beta * y0.double()).abs()) + (2.0 ** -25 if kind == "f16" else 0.0)
     within(y, want, tol, "y")
@@ -477,6 +478,78 @@ def test_w4_matvec_f32_keeps_large_small_and_not_finite_values(b2):
     hit = codes[:, 7] != 8
     assert bool((y[4][hit] == torch.where(codes[:, 7] > 8, 1.0, -1.0)[hit] * float("inf")).all()) and bool(y[4][~hit].isnan().all())
     assert bool(y[5].isnan().all())
+
+
+@pytest.mark.parametrize("M,N,K", [(4, 200, 2304), (1, 40, 700), (16, 300, 2304), (40, 150, 1000), (8, 2500, 8200)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_w4_matvec_infinities_and_nan_anywhere(b2, M, N, K, kind):
+    """Elements that are not finite, in one row or several and at both ends of K, meet their exact weights: their row's outputs
+    are +-inf by the sign of the weight, NaN where it is 0 or two infinities differ; the other rows keep their bound."""
+    dtype, group = TYPES[kind], 64
+    codes, s, z, dev = held(N, K, group, torch.float32, True, M + K)
+    w = ref.w4_values(codes, s, z, group)
+    x = torch.randn(M, K, generator=gen(M)).to(dtype)
+    x[0, K - 1] = float("inf")
+    if M > 3:
+        x[2, 0], x[2, K // 2] = -float("inf"), float("inf")
+        x[3, K // 3] = float("nan")
+    y = b2.w4_matvec(M, N, K, group, 1.0, x.cuda(), *dev, 0.0).cpu().double()
+    want = x.double() @ w.t()                   # 0 * inf and inf - inf are NaN here too
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y == float("inf"), want == float("inf"))
+    assert torch.equal(y == -float("inf"), want == -float("inf"))
+    fine = torch.isfinite(want).all(1)
+    assert int(fine.sum()) == M - (3 if M > 3 else 1)
+    at = torch.arange(K) // group
+    size = x[fine].double().abs() @ (w.abs() + 16.0 * s.double()[:, at]).t()
+    tol = ref.half_step(dtype) * want[fine].abs() + 2 * U * (64 + K / 16) * size + (2.0 ** -25 if kind == "f16" else 0.0)
+    within(y[fine], want[fine], tol, "the other rows")
+
+
+@pytest.mark.parametrize("M", [3, 12])
+def test_w4_matvec_rows_of_very_different_size(b2, M):
+    """Each row is scaled by itself: rows of 1e-30, 1 and 1e30 in one product, and elements 2^-20 of their row's largest."""
+    N, K, group = 60, 1600, 128
+    codes, s, z, dev = held(N, K, group, torch.bfloat16, False, 8)
+    w = ref.w4_values(codes, s, z, group)
+    x = torch.randn(M, K, generator=gen(5))
+    x[:, 5::7] *= 2.0 ** -20
+    x = (x * torch.tensor([1e-30, 1.0, 1e30])[torch.arange(M) % 3][:, None]).to(torch.bfloat16)
+    y = b2.w4_matvec(M, N, K, group, 1.0, x.cuda(), *dev, 0.0)
+    want = x.double() @ w.t()
+    size = x.double().abs() @ (w.abs() + 8.0 * s.double()[:, torch.arange(K) // group]).t()
+    within(y, want, ref.half_step(torch.bfloat16) * want.abs() + 2 * U * (64 + K / 16) * size, "y")
+    # a row whose elements are all tiny but one: the tiny ones still count
+    one = torch.full((1, K), 2.0 ** -16, dtype=torch.bfloat16)
+    one[0, 0] = 1024.0
+    y = b2.w4_matvec(1, N, K, group, 1.0, one.cuda(), *dev, 0.0)
+    want = one.double() @ w.t()
+    size = one.double() @ (w.abs() + 8.0 * s.double()[:, torch.arange(K) // group]).t()
+    within(y, want, ref.half_step(torch.bfloat16) * want.abs() + 2 * U * (64 + K / 16) * size, "y")
+
+
+@pytest.mark.parametrize("M", [1, 20])
+def test_w4_a_bad_weight_shows_in_its_output_alone(b2, M):
+    N, K, group = 50, 640, 128
+    W = weights(N, K, 3)
+    W[7, 200], W[30, 639] = float("nan"), float("inf")
+    codes, s, z = b2.w4_empty(N, K, group, torch.bfloat16)
+    b2.w4_quantize(N, K, group, W.cuda(), codes, s, z)
+    y = b2.w4_matvec(M, N, K, group, 1.0, torch.randn(M, K, generator=gen(1)).cuda(), codes, s, z, 0.0).cpu()
+    bad = torch.zeros(N, dtype=torch.bool)
+    bad[[7, 30]] = True
+    assert bool(y[:, bad].isnan().all()) and bool(torch.isfinite(y[:, ~bad]).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 9000), (5, 100000), (700, 8200), (3, 8193)])
+def test_layernorm_backward_of_the_longest_rows(b2, rows, cols):
+    x, gamma, _, dy = norm_inputs(rows, cols, torch.bfloat16, torch.float32, rows)
+    mean, rstd = statistics(x)
+    dx, dg, db = torch.zeros_like(x).cuda(), torch.zeros(cols, device="cuda"), torch.zeros(cols, device="cuda")
+    b2.layernorm_backward(rows, cols, dy.cuda(), x.cuda(), gamma.cuda(), mean.cuda(), rstd.cuda(), dx, dg, db)
+    check_backward(dy, x, gamma, mean, rstd, dx, dg, db)
+    dx2 = torch.zeros_like(dx)
+    b2.layernorm_backward(rows, cols, dy.cuda(), x.cuda(), gamma.cuda(), mean.cuda(), rstd.cuda(), dx2, None, None)
+    assert torch.equal(dx, dx2)
 
 
 def test_w4_matvec_short_cuts(b2):
