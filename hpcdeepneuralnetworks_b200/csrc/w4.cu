@@ -475,17 +475,19 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 // than CTAs, the k range is cut over the CTAs of a cluster, whose sums meet over distributed shared memory in the order of the
 // ranks: no atomics.
 constexpr int kMvConsumers = 256, kMvProducers = 128, kMvThreads = kMvConsumers + kMvProducers;
-constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2, kMvCodeBytes = kMvRows * kMvRowBytes;
+constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2;
 constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns of a warp's store in 32 banks
 constexpr int kMvWindow = 1024;             // scales and zero points held together: 8 groups of each row, the group / 32 chunks
 constexpr int kMvWindows = 2;               // they span
 constexpr int kMvMaxStages = 8, kMvBarrierBytes = 512 + 1024;   // barriers and flags, and room to align
 constexpr int kMvXThreads = 512;
 
-template <int NB, bool RESIDENT>
+template <int NB, bool RESIDENT, bool ALIGNED>
 struct MvTile {
+  // rows of codes that start anywhere are held from the 16-byte boundary in front of them on, 9 units of 16 bytes
+  static constexpr int kRowPitch = ALIGNED ? kMvRowBytes : kMvRowBytes + 16, kCodeBytes = kMvRows * kRowPitch;
   static constexpr int kXBytes = NB * (kMvChunk * 8 * 2 + 256);     // x of one chunk: fragments, then sums [part of a group][8 NB]
-  static constexpr int kStage = RESIDENT ? kMvCodeBytes : (kMvCodeBytes + kXBytes + 1023) / 1024 * 1024;
+  static constexpr int kStage = RESIDENT ? kCodeBytes : (kCodeBytes + kXBytes + 1023) / 1024 * 1024;
   static constexpr int kSumBytes = 2 * 8 * NB * kMvPitch * 4;
   static constexpr int kCtasPerSm = NB <= 2 ? 2 : 1;
   static constexpr int kSmem = kCtasPerSm == 2 ? 115712 : 232448;   // what a CTA may have
@@ -689,6 +691,17 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *global, ui
                "l"(global), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// One access of the old kind of asynchronous copy, the thread's arrival at a barrier once all its copies have landed, and the wait
+// for them.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *smem_dst, const void *global) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_dst)), "l"(global) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy_arrive(uint64_t *bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
@@ -783,9 +796,9 @@ __device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, i
 // RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
 // BLOCKS: blocks of 32 k in a group, or in the 128 of a longer one that a warp multiplies.
 template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
-__global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
+__global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCtasPerSm)
     w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
-  using Tile = MvTile<NB, RESIDENT>;
+  using Tile = MvTile<NB, RESIDENT, ALIGNED>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the swizzle is one of addresses
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -805,7 +818,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
 
   if (tid == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      mbar_init(&full[s], (ALIGNED || !RESIDENT ? 1 : 0) + (ALIGNED ? 0 : kFillers));
+      mbar_init(&full[s], (ALIGNED || !RESIDENT ? 1 : 0) + (ALIGNED ? 0 : 2 * kFillers));
       mbar_init(&empty[s], kMvConsumers / 32);
     }
     for (int s = 0; s < kMvWindows; ++s) {
@@ -830,7 +843,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
         const unsigned char *late[kMvMaxStages];
         bool waited = false;
         auto send_x = [&](int s, const unsigned char *from) {
-          bulk_load(smem + s * Tile::kStage + kMvCodeBytes, from, Tile::kXBytes, &full[s]);
+          bulk_load(smem + s * Tile::kStage + Tile::kCodeBytes, from, Tile::kXBytes, &full[s]);
         };
         for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
           const int mc = item / a.row_blocks, row = (item - mc * a.row_blocks) * kMvRows;
@@ -838,7 +851,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
           for (int c = 0; c < chunks; ++c, ring.next(), image += Tile::kXBytes) {
             if (sent >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
             if (!wait.alive) continue;
-            if (ALIGNED || !RESIDENT) mbar_expect_tx(&full[ring.at], (ALIGNED ? kMvCodeBytes : 0) + (RESIDENT ? 0 : Tile::kXBytes));
+            if (ALIGNED || !RESIDENT) mbar_expect_tx(&full[ring.at], (ALIGNED ? Tile::kCodeBytes : 0) + (RESIDENT ? 0 : Tile::kXBytes));
             if (ALIGNED) tma_load_2d(smem + ring.at * Tile::kStage, &code_map, &full[ring.at], (first + c) * kMvRowBytes, row);
             if (RESIDENT) {
             } else if (waited) {
@@ -863,13 +876,14 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
       MvRing ring(a.stages), window(kMvWindows);
       uint32_t filled = 0, opened = 0;
       for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-        const int64_t n0 = (int64_t)(item % a.row_blocks) * kMvRows, n_rows = a.N - n0;
+        const int64_t n0 = (int64_t)(item % a.row_blocks) * kMvRows, n_rows = a.N - n0, width = (a.K + 1) >> 1;
         for (int c = 0; c < chunks; ++c) {
-          if ((c & ((1 << window_log) - 1)) == 0) {
+          const bool opens = (c & ((1 << window_log) - 1)) == 0;
+          constexpr int kTurns = (kMvWindow + kFillers - 1) / kFillers, kRowStep = kFillers / 8;
+          uint32_t scale[kTurns], zero[kTurns];
+          if (opens) {
             // scales and zero points of a window: entry e is group e & 7 of row e >> 3, so a thread's group stays the same and
             // its rows lie kFillers / 8 apart; all loads before the first use
-            constexpr int kTurns = (kMvWindow + kFillers - 1) / kFillers, kRowStep = kFillers / 8;
-            uint32_t scale[kTurns], zero[kTurns];
             const int64_t q = (((int64_t)(first + c) * kMvChunk) >> a.group_shift) + (me & 7);
             const int rows = n_rows < kMvRows ? (int)n_rows : kMvRows, mine = q < a.groups ? rows - (me >> 3) : 0;      // rows left
             const int64_t at = (n0 + (me >> 3)) * a.groups + q, row_step = kRowStep * a.groups;
@@ -892,6 +906,55 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
               for (int i = 0; i < kTurns; ++i, from += row_step)
                 if (i * kRowStep < mine) zero[i] = *from & 15;
             }
+          }
+          if (!ALIGNED) {
+            // 16-byte units that lie within their row go to shared memory by themselves (cp.async, which arrives at the barrier
+            // when they have landed); what a row's first and last unit share with its neighbours is read by words and bytes.
+            // Units behind a row, and rows behind N, are left: x is 0 there, or nothing is written.
+            if (filled >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
+            ++filled;
+            unsigned char *const stage = smem + ring.at * Tile::kStage;
+            const int64_t at = (int64_t)(first + c) * kMvRowBytes;
+            const int rows = n_rows < kMvRows ? (int)n_rows : kMvRows, left = width - at < kMvRowBytes ? (int)(width - at) : kMvRowBytes;
+            const uint8_t *const tile = a.codes + n0 * a.ldq + at;
+            constexpr int kUnits = Tile::kRowPitch / 16;
+#pragma unroll 4
+            for (int e = me; e < rows * kUnits; e += kFillers) {
+              const int r = e / kUnits, u = e - r * kUnits;
+              const uint8_t *const row = tile + r * a.ldq;
+              const int skew = (int)((uintptr_t)row & 15), from = 16 * u - skew;      // the unit's first byte, from the tile's
+              if ((from >= 0 || at > 0) && from + 16 <= width - at && from < kMvRowBytes)
+                copy_async<16>(stage + r * Tile::kRowPitch + 16 * u, row + from);
+            }
+            if (at == 0 || at + kMvRowBytes + 16 > width) {
+              for (int e = me; e < 2 * rows; e += kFillers) {
+                const uint8_t *const row = tile + (e >> 1) * a.ldq;
+                const int skew = (int)((uintptr_t)row & 15);
+                // the first unit, where the row starts in its middle, or the one that the row ends in (if they are one: once)
+                const int last = (left + skew - 1) >> 4, u = (e & 1) ? last : 0;
+                const int from = 16 * u - skew;
+                if ((from >= 0 || at > 0) && from + 16 <= width - at) continue;      // whole
+                if ((e & 1) && last == 0) continue;
+                unsigned char *const to = stage + (e >> 1) * Tile::kRowPitch + 16 * u;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int b = from + 4 * k;
+                  if ((b >= 0 || at > 0) && b + 4 <= width - at) copy_async<4>(to + 4 * k, row + b);
+                  else {
+                    uint32_t word = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      if ((b + i >= 0 || at > 0) && b + i < width - at) word |= (uint32_t)row[b + i] << (8 * i);
+                    *reinterpret_cast<uint32_t *>(to + 4 * k) = word;
+                  }
+                }
+              }
+            }
+            copy_arrive(&full[ring.at]);
+            mbar_arrive(&full[ring.at]);      // for what was stored
+            ring.next();
+          }
+          if (opens) {
             if (opened >= kMvWindows) wait(&wempty[window.at], window.phase ^ 1);
             ++opened;
             float2 *to = windows + window.at * kMvWindow + me;
@@ -906,52 +969,10 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
             mbar_arrive(&wfull[window.at]);
             window.next();
           }
-          if (!ALIGNED) {
-            if (filled >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
-            ++filled;
-            unsigned char *stage = smem + ring.at * Tile::kStage;
-            const int64_t at = (int64_t)(first + c) * kMvRowBytes, width = (a.K + 1) >> 1;
-            // 16-byte units, a thread's of one column and rows kFillers / 8 apart, four in flight; five words each inside a row
-            constexpr int kFlight = 4, kTurns = (kMvRows * 8 + kFillers - 1) / kFillers;
-            const int cc = me & 7;
-            const int64_t byte = at + 16 * cc;
-            const bool inside = byte >= 4 && byte + 20 <= width;
-            const int rows = byte < width ? (n_rows < kMvRows ? (int)n_rows : kMvRows) : 0;
-            for (int i0 = 0; i0 < kTurns; i0 += kFlight) {
-              uint32_t w[kFlight][5];
-#pragma unroll
-              for (int i = 0; i < kFlight; ++i) {
-                const int r = (me >> 3) + (i0 + i) * (kFillers / 8);
-                const uint8_t *p = a.codes + (n0 + r) * a.ldq + byte;
-                if (inside && r < rows) {
-                  const uint32_t *q = reinterpret_cast<const uint32_t *>(p - ((uintptr_t)p & 3));
-#pragma unroll
-                  for (int k = 0; k < 5; ++k) w[i][k] = q[k];
-                }
-              }
-#pragma unroll
-              for (int i = 0; i < kFlight; ++i) {
-                const int r = (me >> 3) + (i0 + i) * (kFillers / 8);
-                if (r >= kMvRows) break;
-                const uint8_t *row = a.codes + (n0 + r) * a.ldq;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < rows) {
-                  const int skew = 8 * (int)((uintptr_t)(row + byte) & 3);
-                  if (inside)
-                    v = make_uint4(__funnelshift_r(w[i][0], w[i][1], skew), __funnelshift_r(w[i][1], w[i][2], skew),
-                                   __funnelshift_r(w[i][2], w[i][3], skew), __funnelshift_r(w[i][3], w[i][4], skew));
-                  else v = make_uint4(w4_word(row, byte, width), w4_word(row, byte + 4, width), w4_word(row, byte + 8, width),
-                                      w4_word(row, byte + 12, width));
-                }
-                *reinterpret_cast<uint4 *>(stage + r * kMvRowBytes + ((cc ^ (r & 7)) << 4)) = v;
-              }
-            }
-            mbar_arrive(&full[ring.at]);
-            ring.next();
-          }
         }
       }
     }
+    if (!ALIGNED) copy_wait_all();
     __syncwarp();
     cluster_wait();
   } else {
@@ -959,9 +980,13 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     uint32_t turn = 0;
     MvRing ring(a.stages), window(kMvWindows);
     const uint32_t smem_base = smem_u32(smem), xs_base = smem_u32(xs), windows_base = smem_u32(windows + ((wn * 32 + g) << 3));
-    uint32_t place[4];        // of this thread's words of row wn * 32 + g (and, at fixed distances, g + 8, ...) in a stage
+    // ALIGNED: of this thread's words of row wn * 32 + g (and, at fixed distances, g + 8, ...) in a stage.  Otherwise of the first
+    // of its words of rows g + 8 r, and by how many bits that word is off, set for each row block.
+    uint32_t place[4], off[ALIGNED ? 1 : 4];
+    if constexpr (ALIGNED) {
 #pragma unroll
-    for (int b4 = 0; b4 < 4; ++b4) place[b4] = (wn * 32 + g) * kMvRowBytes + (((wk * 4 + b4) ^ g) << 4) + 4 * t;
+      for (int b4 = 0; b4 < 4; ++b4) place[b4] = (wn * 32 + g) * kMvRowBytes + (((wk * 4 + b4) ^ g) << 4) + 4 * t;
+    }
     if constexpr (RESIDENT) {
       // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8.  Each
       // row is scaled by its largest element here; the sums are scaled back before they leave the CTA.
@@ -997,13 +1022,22 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
     for (int item = blockIdx.x; item < a.items; item += gridDim.x, ++turn) {
       const int mc = item / a.row_blocks;
       float total[2][NB][4] = {};
+      if constexpr (!ALIGNED) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = wn * 32 + g + 8 * r;
+          const uint32_t skew = (uint32_t)(uintptr_t)(a.codes + ((int64_t)(item - mc * a.row_blocks) * kMvRows + row) * a.ldq) & 15u;
+          place[r] = row * Tile::kRowPitch + wk * (kMvRowBytes / 2) + 4 * t + (skew & 12u);
+          off[r] = 8 * (skew & 3u);
+        }
+      }
 #pragma unroll (EXACT ? 1 : 2)
       for (int c = 0; c < chunks; ++c) {
         const int in_window = c & ((1 << window_log) - 1);
         if (in_window == 0) wait(&wfull[window.at], window.phase);
         wait(&full[ring.at], ring.phase);
         const uint32_t stage = smem_base + ring.at * Tile::kStage;
-        const uint32_t image = RESIDENT ? xs_base + c * Tile::kXBytes : stage + kMvCodeBytes;
+        const uint32_t image = RESIDENT ? xs_base + c * Tile::kXBytes : stage + Tile::kCodeBytes;
         const uint32_t xf = image + (wk * 4 * NB * 32 + lane) * 16;
         const uint32_t xsum = image + NB * (kMvChunk * 8 * 2) + t * 8 + wk * (4 / BLOCKS) * 8 * NB * 4;
         // this warp's first group of the window
@@ -1021,10 +1055,17 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT>::kCtasPerSm)
               uint4 xv[NB];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) xv[nb] = ld_shared_128(xf + (b4 * NB + nb) * 512);
-              const uint32_t at = stage + place[b4];
 #pragma unroll
               for (int rt = 0; rt < 2; ++rt) {
-                const uint32_t w0 = ld_shared_32(at + rt * 16 * kMvRowBytes), w1 = ld_shared_32(at + (rt * 16 + 8) * kMvRowBytes);
+                uint32_t w0, w1;
+                if constexpr (ALIGNED) {
+                  const uint32_t at = stage + place[b4];
+                  w0 = ld_shared_32(at + rt * 16 * kMvRowBytes), w1 = ld_shared_32(at + (rt * 16 + 8) * kMvRowBytes);
+                } else {
+                  const uint32_t at0 = stage + place[2 * rt] + 16 * b4, at1 = stage + place[2 * rt + 1] + 16 * b4;
+                  w0 = __funnelshift_r(ld_shared_32(at0), ld_shared_32(at0 + 4), off[2 * rt]);
+                  w1 = __funnelshift_r(ld_shared_32(at1), ld_shared_32(at1 + 4), off[2 * rt + 1]);
+                }
                 const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
                 uint32_t f[4], h[4];
                 if constexpr (EXACT) {
@@ -1187,7 +1228,7 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
 
 template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
-  using Tile = MvTile<NB, RESIDENT>;
+  using Tile = MvTile<NB, RESIDENT, ALIGNED>;
   const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS, EXACT>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
