@@ -691,12 +691,10 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *global, ui
                "l"(global), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-// One access of the old kind of asynchronous copy, the thread's arrival at a barrier once all its copies have landed, and the wait
-// for them.
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void *smem_dst, const void *global) {
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem_dst)), "l"(global) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(global) : "memory");
+// 16 bytes by cp.async, the first `bytes` of them read and the others 0; the thread's arrival at a barrier once all its copies have
+// landed; and the wait for them.
+__device__ __forceinline__ void copy_async_16(void *smem_dst, const void *global, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem_dst)), "l"(global), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -908,46 +906,33 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
             }
           }
           if (!ALIGNED) {
-            // 16-byte units that lie within their row go to shared memory by themselves (cp.async, which arrives at the barrier
-            // when they have landed); what a row's first and last unit share with its neighbours is read by words and bytes.
-            // Units behind a row, and rows behind N, are left: x is 0 there, or nothing is written.
+            // 16 bytes at a time by cp.async, which arrives at the barrier when they have landed, cut off where the row ends.  In
+            // front of a row a unit may bring bytes of the row before it along, but nothing from in front of the matrix.  Units
+            // behind a row, and rows behind N, are left: x is 0 there, or nothing is written.
             if (filled >= (uint32_t)a.stages) wait(&empty[ring.at], ring.phase ^ 1);
             ++filled;
             unsigned char *const stage = smem + ring.at * Tile::kStage;
-            const int64_t at = (int64_t)(first + c) * kMvRowBytes;
-            const int rows = n_rows < kMvRows ? (int)n_rows : kMvRows, left = width - at < kMvRowBytes ? (int)(width - at) : kMvRowBytes;
-            const uint8_t *const tile = a.codes + n0 * a.ldq + at;
-            constexpr int kUnits = Tile::kRowPitch / 16;
-#pragma unroll 4
-            for (int e = me; e < rows * kUnits; e += kFillers) {
-              const int r = e / kUnits, u = e - r * kUnits;
-              const uint8_t *const row = tile + r * a.ldq;
-              const int skew = (int)((uintptr_t)row & 15), from = 16 * u - skew;      // the unit's first byte, from the tile's
-              if ((from >= 0 || at > 0) && from + 16 <= width - at && from < kMvRowBytes)
-                copy_async<16>(stage + r * Tile::kRowPitch + 16 * u, row + from);
-            }
-            if (at == 0 || at + kMvRowBytes + 16 > width) {
-              for (int e = me; e < 2 * rows; e += kFillers) {
-                const uint8_t *const row = tile + (e >> 1) * a.ldq;
-                const int skew = (int)((uintptr_t)row & 15);
-                // the first unit, where the row starts in its middle, or the one that the row ends in (if they are one: once)
-                const int last = (left + skew - 1) >> 4, u = (e & 1) ? last : 0;
-                const int from = 16 * u - skew;
-                if ((from >= 0 || at > 0) && from + 16 <= width - at) continue;      // whole
-                if ((e & 1) && last == 0) continue;
-                unsigned char *const to = stage + (e >> 1) * Tile::kRowPitch + 16 * u;
+            const int64_t at = (int64_t)(first + c) * kMvRowBytes, before = n0 * a.ldq + at;      // bytes of the matrix in front of the tile
+            const int rows = n_rows < kMvRows ? (int)n_rows : kMvRows, left = width - at < 256 ? (int)(width - at) : 256;
+            const uint8_t *const tile = a.codes + before;
+            auto unit = [&](const uint8_t *row, int r, int u) {
+              const int from = 16 * u - (int)((uintptr_t)row & 15), bytes = left - from < 16 ? left - from : 16;      // from the tile's
+              if (r < rows && bytes > 0 && (r >= 16 || row + from >= a.codes))
+                copy_async_16(stage + r * Tile::kRowPitch + 16 * u, row + from, bytes);
+            };
+            // a thread's units are of one column and rows kFillers / 8 apart (known distances: the addresses are most of the work)
+            const uint8_t *row = tile + (me >> 3) * a.ldq;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int b = from + 4 * k;
-                  if ((b >= 0 || at > 0) && b + 4 <= width - at) copy_async<4>(to + 4 * k, row + b);
-                  else {
-                    uint32_t word = 0;
+            for (int i = 0; i < (kMvRows * 8 + kFillers - 1) / kFillers; ++i, row += (kFillers / 8) * a.ldq) unit(row, (me >> 3) + i * (kFillers / 8), me & 7);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                      if ((b + i >= 0 || at > 0) && b + i < width - at) word |= (uint32_t)row[b + i] << (8 * i);
-                    *reinterpret_cast<uint32_t *>(to + 4 * k) = word;
-                  }
-                }
+            for (int r = me; r < kMvRows; r += kFillers)      // the ninth, of rows that do not start on 16 bytes
+              if ((uintptr_t)(tile + r * a.ldq) & 15) unit(tile + r * a.ldq, r, 8);
+            if (before < 16) {      // the first rows (of 1 byte, 16 of them) byte by byte
+#pragma unroll
+              for (int i = 0; i < (256 + kFillers - 1) / kFillers; ++i) {
+                const int r = (me + i * kFillers) >> 4, b = (me + i * kFillers) & 15, skew = (int)((uintptr_t)(tile + r * a.ldq) & 15);
+                if (r < 16 && r < rows && before + r * a.ldq < skew && b >= skew && b - skew < left)
+                  stage[r * Tile::kRowPitch + b] = tile[r * a.ldq + b - skew];
               }
             }
             copy_arrive(&full[ring.at]);
