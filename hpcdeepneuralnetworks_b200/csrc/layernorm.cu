@@ -1,9 +1,14 @@
 // Layer norm, forward and backward: both are bound by memory (the forward pass reads x and writes y, the backward pass reads x
 // and dy and writes dx), so every row is read once and kept in registers while its sums are formed.
 //
-// A row belongs to a warp (up to 1024 columns; 512 backward) or to a block; a thread holds up to kHeld elements of it, V neighbouring ones to
-// an access.  V is the widest access that every row pointer, the pitches and cols allow (16 bytes, 4 bytes, one element), so that
-// no row needs a head or a tail.  Longer rows are read again instead of held.
+// A row belongs to a team of warps, a thread holds up to 32 elements of it (16 backward), V neighbouring ones to an access.  V is
+// the widest access that every row pointer, the pitches and cols allow (16 bytes, 4 bytes, one element); rows that fit none but
+// are off by the same amount in all matrices are taken in 16 bytes with their ends masked (PHASED).  Longer rows are read again
+// instead of held.
+// Measured, device time: forward 16384 x 4096 bf16 47.7 us (5.6 TB/s of the 268 MB it must move, 0.87 of a copy), 8192 x 4095
+// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 75 us (5.4 TB/s, 0.83), 8192 x 4095 73 us, 5003 x 1027 FP32
+// 22 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
+// latency of a row's two sums, with 10 to 16 warps to an SM.
 #include <math.h>
 
 #include <initializer_list>
@@ -203,14 +208,20 @@ struct LnWeights {
   Pack *at;
   __device__ __forceinline__ LnWeights(float *base, const LnTeam &t)
       : at(reinterpret_cast<Pack *>(base) + (t.tid >> 5) * N * (V / G) * 32 + t.lane) {}
-  template <class P>
-  __device__ __forceinline__ void put(const P *p, int valid, float without) {
-    for (int i = 0; i < valid; ++i) {
+  // p: of the thread's first column; CUT: which of the columns lie in the row is to be looked at (others read some parameter)
+  template <class P, bool CUT>
+  __device__ __forceinline__ void put(const P *p, int col, int cols, int valid, float without) {
+    for (int i = 0; i < N; ++i) {
+      if (i >= valid && !CUT) break;
 #pragma unroll
       for (int q = 0; q < V / G; ++q) {
         Pack w;
 #pragma unroll
-        for (int k = 0; k < G; ++k) w.e[k] = p ? to_f32(p[i * 32 * V + q * G + k]) : without;
+        for (int k = 0; k < G; ++k) {
+          int c = i * 32 * V + q * G + k;
+          if (CUT) c = min(max(c, -col), cols - 1 - col);
+          w.e[k] = p ? to_f32(p[c]) : without;
+        }
         at[(i * (V / G) + q) * 32] = w;
       }
     }
@@ -233,30 +244,93 @@ __device__ __forceinline__ void ln_copy_async(void *smem, const void *global, in
   if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(global) : "memory");
 }
+__device__ __forceinline__ void ln_copy_async_16(void *smem, const void *global, int bytes) {      // the first `bytes`, and 0 behind them
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(global), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void ln_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
 __device__ __forceinline__ void ln_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 
+// Clears the places of a thread's accesses outside the row, once: nothing is ever fetched there, and the loops over a row need no
+// conditions (with one around each access: 16384 x 2052 FP32 backward 152 us instead of 86).
+template <class Pack>
+__device__ __forceinline__ void ln_clear(Pack *at, int slot, int slots, int valid, int accesses) {
+  for (int s = 0; s < slots; ++s)
+    for (int i = valid; i < accesses; ++i) {
+      Pack zero;
+      memset(&zero, 0, sizeof(zero));
+      at[s * slot + i * 32] = zero;
+    }
+}
+
+// PHASED: rows that start anywhere, in accesses of 16 bytes all the same.  The rows of all matrices start equally far behind a
+// 16-byte boundary, a team's rows do so too (its step is a multiple of V rows), and a thread's accesses lie on the boundaries: a
+// thread's columns stay the same from row to row.  A row's first access may begin with elements of the row before it, which
+// count as 0, and its last is cut off where the row ends (0 again); both are written element by element.
+template <int V>
+struct LnPhase {
+  int col, cols, shift;     // column of a thread's first element (in front of the row if negative); columns; V - 1 or less
+  bool front, edge;         // the thread has the row's first access, and it is such a one; has the first or the last
+  __device__ __forceinline__ LnPhase(int shift, int col, int cols, int valid) : col(col), cols(cols), shift(shift) {
+    front = valid > 0 && col < 0;
+    edge = front || (valid > 0 && col + (valid - 1) * 32 * V + V > cols);
+  }
+  __device__ __forceinline__ bool inside(int i, int e) const { return (unsigned)(col + i * 32 * V + e) < (unsigned)cols; }
+  template <class T>
+  __device__ __forceinline__ void fetch(void *smem, const T *from, int i) const {
+    const int left = cols - (col + i * 32 * V);
+    ln_copy_async_16(smem, from, left < V ? left * (int)sizeof(T) : 16);
+  }
+  // Parameters of access i; outside the row, some others (all loads at once, without conditions).
+  template <class P>
+  __device__ __forceinline__ void params(LnF<2> (&v)[V / 2 + (V == 1)], const P *p, int i, float without) const {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      const int c = col + i * 32 * V + 2 * k, c0 = min(max(c, 0), cols - 1), c1 = min(max(c + 1, 0), cols - 1);
+      v[k] = p ? LnF<2>(to_f32(p[c0]), to_f32(p[c1])) : LnF<2>(without);
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void clear_front(LnPack<T, V> &p) const {
+    if (front) {
+#pragma unroll
+      for (int e = 0; e < V - 1; ++e)
+        if (e < shift) p.e[e] = from_f32<T>(0.f);
+    }
+  }
+  template <class T>
+  __device__ __forceinline__ void store(const LnPack<T, V> &out, T *to, int i) const {
+    if (!edge) out.store(to);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (inside(i, e)) to[e] = out.e[e];
+    }
+  }
+};
+
 // y = (x - mean) * rstd * gamma + beta, E elements of the row per thread.  The variance is that of the distances from a first
 // mean, and what the first mean was off by (the mean of those distances) is taken out of both: a large mean costs no digits.
-template <class T, class P, int V, int E, int THREADS, bool FULL>
+template <class T, class P, int V, int E, int THREADS, bool FULL, bool PHASED>
 __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int cols, int share, int turns, int ahead, float eps, const T *x,
                                                             int64_t ldx, const P *gamma, const P *beta, T *y, int64_t ldy, float *mean,
                                                             float *rstd) {
   using Pack = LnPack<T, V>;
   using F = typename Pack::F;
   constexpr int N = E / V, K = Pack::kParts;
-  constexpr bool RING = V * sizeof(T) >= 4;
+  constexpr bool RING = V * sizeof(T) >= 4, ALL = FULL || RING;      // ALL: accesses outside the row read zeros
   // gamma and beta: in registers over the rows, in shared memory, or (the longest rows) read again for each row
   constexpr bool HOLD = E <= 16, SHARED = !HOLD && THREADS <= 512;
   __shared__ LnScratch scratch[2];
   extern __shared__ __align__(16) unsigned char dynamic[];
   const LnTeam t(share);
   if (FULL) turns = N;
-  const int valid = FULL ? N : t.valid(cols / V, turns);
-  const int64_t col = (int64_t)t.unit(turns) * V;
+  const int shift = PHASED ? (int)((uintptr_t)(x + t.first * ldx) & 15) / (int)sizeof(T) : 0;
+  const int valid = FULL ? N : t.valid((cols + shift + V - 1) / V, turns);
+  const int64_t col = (int64_t)t.unit(turns) * V - shift;
+  const LnPhase<V> phase(shift, (int)col, cols, PHASED ? valid : 0);
   const float inv = 1.f / (float)cols;
   const T *px = x + t.first * ldx + col;                    // the next row to fetch
   T *py = y + t.first * ldy + col;
@@ -268,12 +342,14 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
   const int slot = (int)blockDim.x * N;
   Pack *fetched = ring, *in_hand = ring, *const ring_end = ring + (ahead + 1) * slot;
   Pack v[N];
+  if constexpr (RING && !FULL) ln_clear(ring, slot, ahead + 1, valid, N);
   auto fetch = [&]() {
     if (next < rows) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (FULL || i < valid) {
-          if constexpr (RING) ln_copy_async(fetched + i * 32, px + i * 32 * V, V * sizeof(T));
+          if constexpr (PHASED) phase.fetch(fetched + i * 32, px + i * 32 * V, i);
+          else if constexpr (RING) ln_copy_async(fetched + i * 32, px + i * 32 * V, V * sizeof(T));
           else v[i].load_stream(px + i * 32 * V);
         }
     }
@@ -290,11 +366,11 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
   F g[HOLD ? N : 1][K], b[HOLD ? N : 1][K];
   using Weights = LnWeights<V, N>;
   float *const shared_params = reinterpret_cast<float *>(dynamic + (RING ? (ahead + 1) * slot * sizeof(Pack) : 0));
-  Weights weights_g(shared_params, t), weights_b(shared_params + share * E, t);
+  Weights weights_g(shared_params + (PHASED ? 2 * t.team * share * E : 0), t), weights_b(shared_params + (PHASED ? 2 * t.team + 1 : 1) * share * E, t);
   if constexpr (SHARED) {
-    if (t.team == 0) {
-      weights_g.template put<P>(pg, valid, 1.f);
-      weights_b.template put<P>(pb, valid, 0.f);
+    if (PHASED || t.team == 0) {
+      weights_g.template put<P, PHASED>(pg, (int)col, cols, valid, 1.f);
+      weights_b.template put<P, PHASED>(pb, (int)col, cols, valid, 0.f);
     }
     __syncthreads();
   }
@@ -302,8 +378,13 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (FULL || i < valid) {
-        ln_params<P, V>(g[i], pg, i * 32 * V, 1.f);
-        ln_params<P, V>(b[i], pb, i * 32 * V, 0.f);
+        if constexpr (PHASED) {
+          phase.params(g[i], gamma, i, 1.f);
+          phase.params(b[i], beta, i, 0.f);
+        } else {
+          ln_params<P, V>(g[i], pg, i * 32 * V, 1.f);
+          ln_params<P, V>(b[i], pb, i * 32 * V, 0.f);
+        }
       }
   }
   for (int64_t row = t.first; row < rows; row += t.step, py += y_step) {
@@ -314,14 +395,15 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
       else ln_wait<0>();
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (FULL || i < valid) v[i] = in_hand[i * 32];
+        v[i] = in_hand[i * 32];
       in_hand += slot;
       if (in_hand == ring_end) in_hand = ring;
     }
+    if constexpr (PHASED) phase.clear_front(v[0]);
     F f[N * K], s(0.f);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (FULL || i < valid) {
+      if (ALL || i < valid) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           f[i * K + k] = v[i].get(k);
@@ -330,10 +412,25 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
       }
     float m = ln_sum(s.sum(), scratch[0], t) * inv;
     F d1(0.f), d2(0.f);
+    if constexpr (ALL && !FULL) {
+      if (valid < N || (PHASED && phase.edge)) {      // what is outside the row lies at the mean
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            if constexpr (PHASED) {
+              const float2 r = f[i * K + k].both();
+              f[i * K + k] = F(i < valid && phase.inside(i, 2 * k) ? r.x : m, i < valid && phase.inside(i, 2 * k + 1) ? r.y : m);
+            } else if (i >= valid) {
+              f[i * K + k] = F(m);
+            }
+          }
+      }
+    }
     const F less(-m);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (FULL || i < valid) {
+      if (ALL || i < valid) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const F e = f[i * K + k] + less;
@@ -352,18 +449,23 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
     const F minus(-m), by(r);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (FULL || i < valid) {
+      if (ALL || i < valid) {
         if constexpr (SHARED) {
           weights_g.get(g[0], i);
           weights_b.get(b[0], i);
         } else if constexpr (!HOLD) {
-          ln_params<P, V>(g[0], pg, i * 32 * V, 1.f);
-          ln_params<P, V>(b[0], pb, i * 32 * V, 0.f);
+          if (FULL || i < valid) {
+            ln_params<P, V>(g[0], pg, i * 32 * V, 1.f);
+            ln_params<P, V>(b[0], pb, i * 32 * V, 0.f);
+          }
         }
         Pack out;
 #pragma unroll
         for (int k = 0; k < K; ++k) out.set(k, ln_fma((f[i * K + k] + minus) * by, g[HOLD ? i : 0][k], b[HOLD ? i : 0][k]));
-        out.store(py + i * 32 * V);
+        if (FULL || i < valid) {
+          if constexpr (PHASED) phase.store(out, py + i * 32 * V, i);
+          else out.store(py + i * 32 * V);
+        }
       }
   }
 }
@@ -421,23 +523,25 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(int64_t rows, int 
 // teams' sums end as one line of `partial` per block.
 //   xhat = (x - mean) * rstd,  u = dy * gamma,  dx = rstd * (u - sum(u) / n - xhat * sum(u * xhat) / n)
 // dx may be dy: a thread writes only what it has read.
-template <class T, class P, int V, int E, bool FULL>
+template <class T, class P, int V, int E, bool FULL, bool PHASED>
 __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows, int cols, int share, int turns, const T *dy, int64_t lddy,
                                                                  const T *x, int64_t ldx, const P *gamma, const float *mean,
                                                                  const float *rstd, T *dx, int64_t lddx, float *partial) {
   using Pack = LnPack<T, V>;
   using F = typename Pack::F;
   constexpr int N = E / V, K = Pack::kParts, W = Pack::W;
-  constexpr bool RING = V * sizeof(T) >= 4;
+  constexpr bool RING = V * sizeof(T) >= 4, ALL = FULL || RING;      // ALL: accesses outside the row read zeros
   __shared__ LnScratch scratch[2];
   extern __shared__ __align__(16) unsigned char dynamic[];
   float *const joined = reinterpret_cast<float *>(dynamic);                // at the end, with several teams: [2][cols]
   pdl_launch_dependents();
   const LnTeam t(share);
   if (FULL) turns = N;
-  LnWeights<V, N> weights(reinterpret_cast<float *>(dynamic + (RING ? (kLnAhead + 1) * 2 * N * sizeof(Pack) * blockDim.x : 0)), t);
-  const int valid = FULL ? N : t.valid(cols / V, turns);
-  const int64_t col = (int64_t)t.unit(turns) * V;
+  LnWeights<V, N> weights(reinterpret_cast<float *>(dynamic + (RING ? (kLnAhead + 1) * 2 * N * sizeof(Pack) * blockDim.x : 0)) + (PHASED ? t.team * share * E : 0), t);
+  const int shift = PHASED ? (int)((uintptr_t)(x + t.first * ldx) & 15) / (int)sizeof(T) : 0;
+  const int valid = FULL ? N : t.valid((cols + shift + V - 1) / V, turns);
+  const int64_t col = (int64_t)t.unit(turns) * V - shift;
+  const LnPhase<V> phase(shift, (int)col, cols, PHASED ? valid : 0);
   const float inv = 1.f / (float)cols;
   F dg[N * K], db[N * K];
 #pragma unroll
@@ -451,13 +555,20 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
   Pack *const ring = reinterpret_cast<Pack *>(dynamic) + (threadIdx.x >> 5) * 64 * N + t.lane;
   const int slot = (int)blockDim.x * 2 * N;
   Pack *fetched = ring, *in_hand = ring, *const ring_end = ring + (kLnAhead + 1) * slot;
+  if constexpr (RING && !FULL) {
+    ln_clear(ring, slot, kLnAhead + 1, valid, N);
+    ln_clear(ring + N * 32, slot, kLnAhead + 1, valid, N);
+  }
   Pack xn[RING ? 1 : N], gn[RING ? 1 : N];
   auto fetch = [&]() {
     if (next < rows) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
         if (FULL || i < valid) {
-          if constexpr (RING) {
+          if constexpr (PHASED) {
+            phase.fetch(fetched + i * 32, px + i * 32 * V, i);
+            phase.fetch(fetched + (N + i) * 32, pg + i * 32 * V, i);
+          } else if constexpr (RING) {
             ln_copy_async(fetched + i * 32, px + i * 32 * V, V * sizeof(T));
             ln_copy_async(fetched + (N + i) * 32, pg + i * 32 * V, V * sizeof(T));
           } else {
@@ -475,7 +586,7 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
     px += x_step;
     pg += g_step;
   };
-  if (t.team == 0) weights.template put<P>(pw, valid, 1.f);
+  if (PHASED || t.team == 0) weights.template put<P, ALL && !FULL>(pw, (int)col, cols, valid, 1.f);
   __syncthreads();
   // mean and rstd of this team's next 32 rows, a row per lane
   int64_t at = t.first + t.lane * t.step;
@@ -497,10 +608,7 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
       ln_wait<kLnAhead>();
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (FULL || i < valid) {
-          xc[i] = in_hand[i * 32];
-          gc[i] = in_hand[(N + i) * 32];
-        }
+        xc[i] = in_hand[i * 32], gc[i] = in_hand[(N + i) * 32];
       in_hand += slot;
       if (in_hand == ring_end) in_hand = ring;
     } else {
@@ -509,11 +617,12 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
       fetch();
     }
     // with c = x - mean:  sum(u * xhat) = rstd * sum(u * c),  dx = u * rstd + (c * (-rstd^2 * sum(u * xhat) / n) - rstd * sum(u) / n)
+    if constexpr (PHASED) phase.clear_front(xc[0]), phase.clear_front(gc[0]);
     F c[N * K], u[N * K], s1(0.f), s2(0.f);
     const F minus(-m), by(r);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (FULL || i < valid) {
+      if (ALL || i < valid) {
         F g[K];
         weights.get(g, i);
 #pragma unroll
@@ -533,11 +642,14 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
       const F a(-r * (s.x * inv)), b(-(r * r) * (r * s.y * inv));
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (FULL || i < valid) {
+        if (ALL || i < valid) {
           Pack out;
 #pragma unroll
           for (int k = 0; k < K; ++k) out.set(k, ln_fma(u[i * K + k], by, ln_fma(c[i * K + k], b, a)));
-          out.store(to + i * 32 * V);
+          if (FULL || i < valid) {
+            if constexpr (PHASED) phase.store(out, to + i * 32 * V, i);
+            else out.store(to + i * 32 * V);
+          }
         }
     }
   }
@@ -563,6 +675,7 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
 #pragma unroll
             for (int e = 0; e < W; ++e) {
               const int c = (int)col + i * 32 * V + k * W + e;
+              if (PHASED && !phase.inside(i, k * W + e)) continue;
               sums[c] = w ? sums[c] + two[0][e] : two[0][e];
               sums[cols + c] = w ? sums[cols + c] + two[1][e] : two[1][e];
             }
@@ -731,6 +844,13 @@ static int ln_width(int64_t cols, int tb, int pb, std::initializer_list<const vo
   }
   return 1;
 }
+// Whether rows that are not multiples of 16 bytes can be taken as PHASED does: the matrices start on 16 bytes (so that what is
+// in front of a row is the matrix's own) and their pitches are off by as much.
+static bool ln_phased(std::initializer_list<const void *> matrices, std::initializer_list<int64_t> pitches) {
+  for (int64_t p : pitches)
+    if ((p - *pitches.begin()) % 16) return false;
+  return ln_multiple(16, matrices, {});
+}
 template <class T, class F>
 static void ln_with_width(int v, F &&f) {
   if (v == 16 / (int)sizeof(T)) f(std::integral_constant<int, 16 / (int)sizeof(T)>());
@@ -763,7 +883,9 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
   B2_REQUIRE((x == y && ldx == ldy) || !matrices_overlap(x, rows, cols * tb, ldx * tb, y, rows, cols * tb, ldy * tb),
              B2_ERR_INVALID_ARG, "b2_layernorm: y overlaps x (only y == x with ldy == ldx may share memory)");
   B2_CONTEXT(ctx, h, "b2_layernorm");
-  const int width = ln_width(cols, tb, pb, {x, y}, {ldx * tb, ldy * tb}, {gamma, beta});
+  int width = ln_width(cols, tb, pb, {x, y}, {ldx * tb, ldy * tb}, {gamma, beta});
+  const bool phased = width * tb < 16 && rows > 2 * ctx->sm_count && cols >= 128 && cols + 16 <= 512 * 32 && ln_phased({x, y}, {ldx * tb, ldy * tb});
+  if (phased) width = 16 / tb;
   cudaStream_t s = (cudaStream_t)stream;
   auto launch = [&](auto t, auto p) -> int {
     using T = decltype(t);
@@ -772,15 +894,17 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
     ln_with_width<T>(width, [&](auto w) {
       constexpr int V = decltype(w)::value;
       // E elements per thread, teams of threads to a row in blocks of about 256
-      auto run = [&](auto elements, auto bound) {
+      auto run = [&](auto elements, auto bound, auto off) {
         constexpr int E = decltype(elements)::value, THREADS = decltype(bound)::value;
-        const int share = (int)((cols + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns(cols / V, share);
-        const bool full = turns == E / V && cols == (int64_t)share * E;
-        const auto kernel = full ? layernorm_kernel<T, P, V, E, THREADS, true> : layernorm_kernel<T, P, V, E, THREADS, false>;
-        const int64_t fit = share <= kLnBlock ? kLnBlock / share : 1;
+        constexpr bool PHASED = decltype(off)::value;
+        const int64_t span = cols + (PHASED ? V - 1 : 0);
+        const int share = (int)((span + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns((span + V - 1) / V, share);
+        const bool full = !PHASED && turns == E / V && cols == (int64_t)share * E;
+        const auto kernel = full ? layernorm_kernel<T, P, V, E, THREADS, !PHASED, PHASED> : layernorm_kernel<T, P, V, E, THREADS, false, PHASED>;
+        const int64_t fit = share <= (PHASED ? 192 : kLnBlock) ? (PHASED ? 192 : kLnBlock) / share : 1;
         const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
         const size_t row_bytes = V * sizeof(T) >= 4 ? (size_t)threads * E * sizeof(T) : 0;
-        const size_t params = E > 16 && THREADS <= 512 ? (size_t)2 * share * E * sizeof(float) : 0;
+        const size_t params = E > 16 && THREADS <= 512 ? (size_t)2 * (PHASED ? threads : share) * E * sizeof(float) : 0;
         // rows ahead: two, or as many as leave room for two blocks on an SM, or for one
         int ahead = kLnAhead;
         while (ahead > 0 && (ahead + 1) * row_bytes + params > 112 * 1024) --ahead;
@@ -793,18 +917,30 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
         int held = 1;      // the blocks that the device holds at once walk over all rows
         result = ln_blocks_per_sm((const void *)kernel, ctx->device, threads, smem, &held);
         if (result != B2_OK) return;
-        const int64_t most = (int64_t)ctx->sm_count * held;
+        int64_t most = (int64_t)ctx->sm_count * held;
+        if (PHASED && blocks > most) most = most / V * V;
         kernel<<<(unsigned)(blocks < most ? blocks : most), threads, smem, s>>>(
             rows, (int)cols, share, turns, ahead, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
       };
       constexpr int kFew = V == 8 ? 8 : 4, kMost = V >= 4 ? 32 : 16, kLong = V == 1 ? 16 : 32;
       using Half = std::integral_constant<int, 512>;
       using Full = std::integral_constant<int, 1024>;
+      using Even = std::false_type;
+      if constexpr (V == 16 / (int)sizeof(T)) {
+        if (phased) {
+          // 16 bytes against the widest access that fits: 8192 x 4095 bf16 62 -> 43 us (16 elements per thread: 80), 16384 x 2050
+          // 70 -> 51, 8192 x 8001 FP32 127 -> 103, 40000 x 131 FP16 25.6 -> 16.2 (32 elements per thread: 29.8).  Shorter rows lose
+          // (4000 x 67: 3.2 -> 4.7), and so do few rows, which the parameters' odd places delay (11 x 4097: 3.1 -> 4.9).
+          if (cols + V <= 32 * V) run(std::integral_constant<int, V>(), Half(), std::true_type());      // a warp, one access each
+          else run(std::integral_constant<int, 32>(), Half(), std::true_type());
+          return;
+        }
+      }
       // Few rows: as many threads to each as its length allows; rows so short that a warp has enough with a few elements per
       // thread likewise.  Else each thread takes as much as it can hold: the fewer share a sum, the less it costs.
-      if ((rows <= 2 * ctx->sm_count && cols <= 1024 * kFew) || cols <= 32 * kFew) run(std::integral_constant<int, kFew>(), Full());
-      else if (cols <= 512 * kMost) run(std::integral_constant<int, kMost>(), Half());
-      else if (cols <= 1024 * kLong) run(std::integral_constant<int, kLong>(), Full());
+      if ((rows <= 2 * ctx->sm_count && cols <= 1024 * kFew) || cols <= 32 * kFew) run(std::integral_constant<int, kFew>(), Full(), Even());
+      else if (cols <= 512 * kMost) run(std::integral_constant<int, kMost>(), Half(), Even());
+      else if (cols <= 1024 * kLong) run(std::integral_constant<int, kLong>(), Full(), Even());
       else
         layernorm_long_kernel<T, P, V><<<(unsigned)(rows < 1 << 30 ? rows : 1 << 30), 1024, 0, s>>>(
             rows, (int)cols, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
@@ -862,7 +998,9 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
     return B2_OK;
   }
   int parts = (int)ln_parts(rows, cols);
-  const int width = ln_width(cols, tb, pb, {dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : 0}, {gamma});
+  int width = ln_width(cols, tb, pb, {dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : 0}, {gamma});
+  const bool phased = width * tb < 16 && cols + 16 <= kLnLongestBackward && ln_phased({dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : ldx * tb});
+  if (phased) width = 16 / tb;
   float *partial = sums ? (float *)workspace : nullptr;
   float2 *row_sums = is_long ? (float2 *)((char *)workspace + (need - (size_t)rows * sizeof(float2))) : nullptr;
   auto launch = [&](auto t, auto p) -> int {
@@ -873,16 +1011,18 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
       constexpr int V = decltype(w)::value;
       if (!is_long) {
         // E elements per thread, and teams of threads to a row in blocks of about 256
-        auto run = [&](auto elements) {
+        auto run = [&](auto elements, auto off) {
           constexpr int E = decltype(elements)::value;
-          const int share = (int)((cols + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns(cols / V, share);
-          const bool full = turns == E / V && cols == (int64_t)share * E;
-          const auto kernel = full ? layernorm_backward_kernel<T, P, V, E, true> : layernorm_backward_kernel<T, P, V, E, false>;
+          constexpr bool PHASED = decltype(off)::value;
+          const int64_t span = cols + (PHASED ? V - 1 : 0);
+          const int share = (int)((span + 32 * E - 1) / (32 * E)) * 32, turns = ln_turns((span + V - 1) / V, share);
+          const bool full = !PHASED && turns == E / V && cols == (int64_t)share * E;
+          const auto kernel = full ? layernorm_backward_kernel<T, P, V, E, !PHASED, PHASED> : layernorm_backward_kernel<T, P, V, E, false, PHASED>;
           const int64_t fit = share <= 256 ? 256 / share : 1;
           const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
           if ((rows + teams - 1) / teams < parts) parts = (int)((rows + teams - 1) / teams);
           size_t smem = V * sizeof(T) >= 4 ? (size_t)(kLnAhead + 1) * 2 * E * sizeof(T) * threads : 0;
-          smem += (size_t)share * E * sizeof(float);       // gamma
+          smem += (size_t)(PHASED ? threads : share) * E * sizeof(float);       // gamma
           if (teams > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
           result = ensure_func_attributes((const void *)kernel, ctx->device, ((kLnAhead + 1) * 2 * sizeof(T) + sizeof(float)) * E * 512);
           if (result != B2_OK) return;
@@ -890,8 +1030,17 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
                                               (T *)dx, lddx, partial);
         };
         // Elements one by one take more registers and instructions each: fewer of them, in more threads (5003 x 1027 FP32: 35 -> 23 us)
-        if (V == 1 && cols <= 512 * 8) run(std::integral_constant<int, (V == 1 ? 8 : kLnHeldBackward)>());
-        else run(std::integral_constant<int, kLnHeldBackward>());
+        if constexpr (V == 16 / (int)sizeof(T)) {
+          if (phased) {
+            // 16 bytes against the widest access that fits: 8192 x 4095 bf16 257 -> 73 us, 16384 x 2050 84 -> 63 (8 elements per thread:
+            // 93), 5003 x 1027 FP32 23.4 -> 21.9 (16 elements: 30.5), 40000 x 517 FP32 64 -> 59 (16: 108), 40000 x 131 FP16 47 -> 26.5 (16: 31)
+            if (cols + V <= (V == 4 ? 512 : 32) * 8) run(std::integral_constant<int, 8>(), std::true_type());
+            else run(std::integral_constant<int, kLnHeldBackward>(), std::true_type());
+            return;
+          }
+        }
+        if (V == 1 && cols <= 512 * 8) run(std::integral_constant<int, (V == 1 ? 8 : kLnHeldBackward)>(), std::false_type());
+        else run(std::integral_constant<int, kLnHeldBackward>(), std::false_type());
       } else {
         if (dx) {
           const int64_t blocks = rows < 1 << 30 ? rows : 1 << 30;

@@ -207,6 +207,54 @@ def test_layernorm_backward(b2, rows, cols, kind, params):
     check_backward(dy, x, gamma, mean, rstd, dx, dgamma, dbeta)
 
 
+@pytest.mark.parametrize("cols", [128, 129, 131, 242, 255, 257, 515, 1027, 2050, 2053, 4095, 5121, 8170, 8183, 16366, 16383])
+@pytest.mark.parametrize("kind,params", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("pads", [(0, 0), (3, 3), (5, 13), (1, 4)])
+def test_layernorm_rows_that_start_anywhere(b2, cols, kind, params, pads):
+    """Many rows of lengths and pitches off the 16-byte boundaries, alike (mod 8 elements) or not between input and output, with NaN
+    between the input's rows and in one of them: nothing of a row's neighbours counts or is written."""
+    if cols > 5121 and pads != (0, 0):
+        pytest.skip("the longest rows are taken without padding alone")
+    rows, dtype = 601, TYPES[kind]
+    x, gamma, beta, dy = norm_inputs(rows, cols, dtype, TYPES[params], 3 * cols + pads[0])
+    hole = 77
+    mean, rstd = statistics(x)
+
+    def laid(values, pad, between):
+        base = torch.full((rows * (cols + pad),), between, dtype=dtype, device="cuda")
+        view = base.view(rows, cols + pad)[:, :cols]
+        if values is not None:
+            view.copy_(values.cuda())
+            view[hole] = float("nan")
+        return base, view
+    others = [r for r in range(rows) if r != hole]
+    _, xv = laid(x, pads[0], float("nan"))
+    base, yv = laid(None, pads[1], 3.0)
+    m, r = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    b2.layernorm(rows, cols, 1e-5, xv, gamma.cuda(), beta.cuda(), yv, mean=m, rstd=r)
+    assert bool(torch.isnan(yv[hole]).all())
+    check_forward(x[others], gamma, beta, 1e-5, yv[others], m[others], r[others], cols)
+    _, gv = laid(dy, pads[0], float("nan"))
+    for inplace in (False, True):
+        dbase, dv = (None, gv) if inplace else laid(None, pads[1], 3.0)
+        gm = torch.zeros(cols, dtype=gamma.dtype, device="cuda")
+        if not inplace:      # the columns' sums need a row that is finite
+            gv[hole], xv[hole] = dy[hole].cuda(), x[hole].cuda()
+            dbeta = torch.zeros_like(gm)
+            b2.layernorm_backward(rows, cols, gv, xv, gamma.cuda(), mean.cuda(), rstd.cuda(), dv, gm, dbeta)
+            check_backward(dy, x, gamma, mean, rstd, dv, gm, dbeta)
+            gv[hole] = float("nan")
+        b2.layernorm_backward(rows, cols, gv, xv, gamma.cuda(), mean.cuda(), rstd.cuda(), dv, None, None)
+        check_backward(dy[others], x[others], gamma, mean[others], rstd[others], dv[others], None, None)
+        if dbase is not None:
+            dv.fill_(3.0)
+            assert bool((dbase == 3.0).all()), "something outside the rows was written"
+    yv.fill_(3.0)
+    assert bool((base == 3.0).all()), "something outside the rows was written"
+    b2.layernorm(rows, cols, 1e-5, xv, gamma.cuda(), None, xv)
+    check_forward(x, gamma, None, 1e-5, xv, None, None, cols)
+
+
 @pytest.mark.parametrize("cols", [64, 1000, 5000])
 @pytest.mark.parametrize("parts", ["dx", "dgamma", "dbeta", "sums", "dx+dbeta", "no gamma"])
 def test_layernorm_backward_in_parts(b2, cols, parts):
