@@ -689,19 +689,24 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
 }
 
 // Rows too long for that: their sums of u and u * xhat first (one block per row), then everything else by tiles of columns,
-// each thread walking down V columns.
+// each thread walking down V columns.  x and dy are read twice: 4096 x 16384 bf16 takes 125 us, 5.4 TB/s of that traffic and 2.0
+// times what one reading would take (158 us with 1024 threads to a row and a line of sums for every 28 rows).  Going over the rows
+// by panels that fit L2, both kernels for each, was slower: 191 us for panels of 48 MB, 164 for 80 MB; the kernels' ends cost more
+// than the second reading.
+constexpr int kLnSumThreads = 512;
 template <class T, class P, int V>
-__global__ void __launch_bounds__(1024) layernorm_row_sums_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x, int64_t ldx,
+__global__ void __launch_bounds__(kLnSumThreads) layernorm_row_sums_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x, int64_t ldx,
                                                                   const P *gamma, const float *mean, const float *rstd, float2 *out) {
   using F = typename LnPack<T, V>::F;
   constexpr int K = LnPack<T, V>::kParts;
   __shared__ LnScratch scratch[2];
-  const LnTeam t(1024);
+  const LnTeam t(kLnSumThreads);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const float m = mean[row], r = rstd[row];
     F s1(0.f), s2(0.f);
-    for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
+#pragma unroll 4
+    for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += kLnSumThreads * V) {
       LnPack<T, V> xv, gv;
       F g[K];
       xv.load(x + row * ldx + i);
@@ -730,6 +735,7 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(int64_t rows, in
 #pragma unroll
   for (int k = 0; k < K; ++k) dg[k] = F(0.f), db[k] = F(0.f);
   ln_params<P, V>(g, gamma, (int)c, 1.f);
+#pragma unroll 2
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     LnPack<T, V> xv, gv;
     xv.load_stream(x + row * ldx + c);
@@ -789,11 +795,14 @@ constexpr int kLnBlock = 384;           // threads of a block of several teams, 
 constexpr int kLnHeldBackward = 16;       // elements per thread, backward
 constexpr int kLnLongestBackward = 8192;  // 512 threads of 16 elements, or 1024 of 8
 // Most blocks, and lines of partial sums: two blocks on each of 148 SMs; the longest rows, whose lines are long and whose blocks
-// share the columns, take fewer.
+// share the columns, take about 1184 blocks of 1024 columns and give each 8 rows at least (300 x 16384 bf16: 34 -> 18 us).
 static int64_t ln_parts(int64_t rows, int64_t cols) {
   int64_t most = 296;
-  if (cols > kLnLongestBackward) most = most * kLnLongestBackward / cols;
-  if (most < 8) most = 8;
+  if (cols > kLnLongestBackward) {
+    most = 1184 * 1024 / cols;
+    if (most > rows / 8) most = rows / 8;
+    if (most < 8) most = 8;
+  }
   return rows < most ? rows : most;
 }
 
@@ -1042,11 +1051,9 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
         if (V == 1 && cols <= 512 * 8) run(std::integral_constant<int, (V == 1 ? 8 : kLnHeldBackward)>(), std::false_type());
         else run(std::integral_constant<int, kLnHeldBackward>(), std::false_type());
       } else {
-        if (dx) {
-          const int64_t blocks = rows < 1 << 30 ? rows : 1 << 30;
-          layernorm_row_sums_kernel<T, P, V><<<(unsigned)blocks, 1024, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx,
-                                                                            (const P *)gamma, mean, rstd, row_sums);
-        }
+        if (dx)
+          layernorm_row_sums_kernel<T, P, V><<<(unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s>>>(
+              rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums);
         layernorm_columns_kernel<T, P, V><<<dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
       }
