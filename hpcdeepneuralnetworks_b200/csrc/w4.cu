@@ -114,7 +114,8 @@ __device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
   }
 }
 
-// Quantising should be bound by reading W; at 8 instructions per element it nearly is.  group / 16 lanes share a group, 16
+// Quantising should be bound by reading W; at 8 instructions per element it nearly is (8192 x 8192 bf16: 43 us, 3.9 TB/s; a copy
+// of those bytes takes 26).  group / 16 lanes share a group, 16
 // elements (8 bytes of codes) each: a group's extremes take log2(group / 16) shuffles.  Nearly every element's code is what the
 // magic addition in w4_nearest gives at once: w / s + 1.5 * 2^23 holds it in its low bits.  Elements that are not nearer than
 // s / 2 to their codes' values (with 16-bit weights a third of the warps meet one that is exactly s / 2 away), and all of a group
@@ -295,7 +296,7 @@ __device__ __forceinline__ uint32_t w4_word(const uint8_t *row, int64_t at, int6
   return word;
 }
 
-// Expanding is bound by writing W.  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight.
+// Expanding is bound by writing W (8192 x 8192 to bf16: 38 us, 4.5 TB/s, of a copy's 6.5).  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight.
 // CVEC: words of codes start on 4 bytes.  WVEC: 16 bytes of W start on 16; otherwise a warp's 256 elements pass through shared
 // memory, so that its stores lie side by side (8192 x 8190 bf16: 171 us with each lane writing its own elements).
 template <class T, class S, bool CVEC, bool WVEC>
@@ -374,7 +375,8 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
 
 // Transposed: tiles of 64 rows n x 64 of k through shared memory, so that codes are read along k and W is written along n.
 // A thread expands 16 codes (8 bytes) of one row into a column of the tile; a row of the tile goes out as 64 elements along n,
-// two of 16 bits to an access where W allows (PAIR).
+// two of 16 bits to an access where W allows (PAIR).  6144 x 6144 to FP32: 37 us, 4.6 TB/s; 8192 x 8192 to bf16, whose rows of a tile
+// are 128 bytes: 56 us.
 template <class T, class S, bool VEC, bool PAIR>
 __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
                                                            const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 // taken off while unpacking, in four more instructions per word: under 1024's upper bits a code reads 1024 + c, or 1024 + 16 c,
 // and a subtraction or an FMA with 1/16 leaves c - z exactly.
 // An infinity or NaN in x would make z * sum_k x meaningless: such elements count as 0 above and are added, with their exact
-// weights, by the thread that writes the output (w4 rows flagged so are slow).
+// weights, by the thread that writes the output, which walks through its whole row for that.
 //
 // A CTA streams tiles of 128 rows x 256 k (16 KB of codes and x of those k) through a ring of shared-memory stages.  Four
 // producer warps fill it: one thread issues the TMA loads (codes with the 128-byte swizzle: the 16-byte unit u of row r lies at
@@ -474,6 +476,8 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 // each row at a time.  Eight consumer warps, 4 (rows) x 2 (k), multiply 32 rows x 128 k each.  Where there are fewer row blocks
 // than CTAs, the k range is cut over the CTAs of a cluster, whose sums meet over distributed shared memory in the order of the
 // ranks: no atomics.
+// Measured on the device: 1 x 4096^2 bf16 8.4 us and 1 x 8192^2 13.9, latency; 16 x 32768 x 8192 45 us = 3.1 TB/s (30 us with
+// the loads alone, 43 with the codes in L2: unpacking and the waits around it decide); 3 x 6144^2 FP32 16.5 us.
 constexpr int kMvConsumers = 256, kMvProducers = 128, kMvThreads = kMvConsumers + kMvProducers;
 constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2;
 constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns of a warp's store in 32 banks
@@ -499,6 +503,8 @@ static int mv_blocks(int64_t M, int type) { return M * mv_parts(type) <= 8 ? 1 :
 static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
 // Whether a product's CTAs lay x out themselves (RESIDENT): each keeps its part of k, cut over clusters of up to 8, in shared
 // memory.  That saves a kernel and a workspace, and costs the same work in every row block's CTAs.
+// (1 token, device time and the host's share of a call: 4096^2, 512 units, 8.4 us and 9 against 7.4 and 14 through w4_x_kernel;
+// 8192^2, 2048 units, 18 against 14 us on the device.)
 constexpr int kMvResidentBytes = 35 * 1024;
 constexpr int64_t kMvResidentWork = 600;       // row blocks x chunks (16 KB of codes each)
 static bool mv_resident(int64_t M, int64_t N, int64_t K, int type) {

@@ -209,7 +209,8 @@ int b2_sdot_static(int64_t n, const float *x, const float *y, float *result_dev,
 /* ---- layer norm ------------------------------------------------------------------------------ */
 
 /* Element types of the operators from here to the SGEMM on host arrays.  Whatever the type, every sum, mean, variance
- * and scale is held in FP32 and rounded to the type once, when it is stored. */
+ * and scale is held in FP32 and rounded to the type once, when it is stored.  But where a call says otherwise, what it writes
+ * (outputs, statistics, workspace) shares no memory with anything else it is given. */
 enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };
 
 /* y = (x - mean) * rstd * gamma + beta for each of `rows` rows of `cols` elements, with
@@ -266,7 +267,8 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 /* y = alpha * x * W^T + beta * y for M = 0..64 rows of x (M x K, ldx) and y (M x N, ldy), both of type `type`: the product of
  * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
  * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm.  y must not overlap x.
- * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.
+ * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.  They are formed from rows of x
+ * scaled to 2^15 by a power of two, so scales of a magnitude outside 2^-110 .. 2^90 may lose digits or overflow on the way.
  * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, N, K, type) bytes that no other call uses meanwhile, where x is
  * laid out for the tensor cores first; 0 (NULL will do) for smaller products, whose kernel lays it out itself.  A bounded wait
  * that runs out on the device is left for b2_check_status as for the SGEMM. */
