@@ -2,7 +2,8 @@
 
 ``python -m hpcdeepneuralnetworks_b200.build`` compiles every ``csrc/*.cu`` into objects under
 ``csrc/build/`` (skipping files whose object is newer than all sources/headers) and links
-``hpcdeepneuralnetworks_b200/libb2blas.so``.  nvcc cross-compiles without a GPU.
+``hpcdeepneuralnetworks_b200/libb2blas.so``, then the C++ driver and the Python extension that shortens the calls of
+``layer.py`` (``csrc/calls.cpp``).  nvcc cross-compiles without a GPU.
 """
 from __future__ import annotations
 
@@ -11,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -67,6 +69,7 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
               ["-Xlinker", "-rpath,/usr/local/cuda/lib64", "-ldl"]
         run(cmd)
     build_driver()
+    build_calls()
     return LIB
 
 
@@ -83,6 +86,26 @@ def build_driver() -> str:
         if r.returncode != 0:
             raise RuntimeError("driver build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
     return DRIVER_BIN
+
+
+CALLS_SRC = os.path.join(CSRC, "calls.cpp")
+CALLS = os.path.join(PKG, "_calls.so")
+
+
+def build_calls() -> str:
+    """The extension module ``_calls``, against the torch it will run with."""
+    if _stale(CALLS, [CALLS_SRC, os.path.join(PKG, "..", "include", "b2blas.h")]):
+        import torch
+        at = os.path.join(os.path.dirname(os.path.abspath(torch.__file__)))
+        cuda = os.path.dirname(os.path.dirname(nvcc()))
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(at, "include"),
+               "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(cuda, "include"), CALLS_SRC, "-o", CALLS,
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-L" + os.path.join(at, "lib"),
+               "-Wl,-rpath," + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("extension build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+    return CALLS
 
 
 if __name__ == "__main__":

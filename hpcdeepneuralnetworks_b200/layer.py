@@ -9,7 +9,9 @@ dimension given by name (in elements; ``ldq`` in bytes) takes the tensor as raw 
 """
 from __future__ import annotations
 
+import ctypes
 import functools
+import importlib
 
 import torch
 
@@ -20,6 +22,23 @@ from .blas import Handle, _default, default_handle
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 W4_GROUPS = (32, 64, 128, 256)
 W4_MAX_ROWS = 64
+
+# csrc/calls.cpp: the usual calls, checked and made without the Python below (which decides all others, with the same results)
+_quick = None
+
+
+def _load():
+    """The library; the first call hands its functions to ``_calls``."""
+    global _quick
+    L = _lib.load()
+    if _quick is None:
+        quick = importlib.import_module(__package__ + "._calls")
+        names = ("b2_layernorm", "b2_layernorm_backward_workspace_bytes", "b2_layernorm_backward", "b2_w4_quantize", "b2_w4_dequantize",
+                 "b2_w4_matvec_workspace_bytes", "b2_w4_matvec")
+        quick.bind(_default, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
+        _quick = quick
+    return L
+
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
@@ -111,6 +130,8 @@ def layernorm(rows, cols, eps, x, gamma, beta, y=None, *, mean=None, rstd=None, 
     """y = (x - mean) * rstd * gamma + beta over the rows of x.  ``gamma``, ``beta``: ``cols`` elements of float32 or x's
     type, or None.  ``mean``, ``rstd``: float32 tensors of ``rows`` elements that receive the statistics, or None.
     ``y``: x's type, x itself for the norm in place, or None for a new tensor.  Returns ``y``."""
+    if _quick and ldx is None and ldy is None and _quick.layernorm(handle, rows, cols, eps, x, gamma, beta, y, mean, rstd):
+        return y
     _tensor(x, "x")
     device = torch.cuda.current_device()
     if y is None:
@@ -120,7 +141,7 @@ def layernorm(rows, cols, eps, x, gamma, beta, y=None, *, mean=None, rstd=None, 
     py, ldy = _matrix(y, rows, cols, ldy, "y", device)
     _same_type(y, x.dtype, "y")
     pt = _params_type(x, (gamma, beta), ("gamma", "beta"))
-    check(_lib.load().b2_layernorm(_raw(handle, device), rows, cols, eps, t, px, ldx, pt, _vector(gamma, cols, "gamma", device),
+    check(_load().b2_layernorm(_raw(handle, device), rows, cols, eps, t, px, ldx, pt, _vector(gamma, cols, "gamma", device),
                                    _vector(beta, cols, "beta", device), py, ldy, _vector(mean, rows, "mean", device, torch.float32),
                                    _vector(rstd, rows, "rstd", device, torch.float32), _stream(device)))
     return y
@@ -128,7 +149,7 @@ def layernorm(rows, cols, eps, x, gamma, beta, y=None, *, mean=None, rstd=None, 
 
 @functools.lru_cache(maxsize=4096)
 def _layernorm_workspace(rows, cols) -> int:
-    return int(_lib.load().b2_layernorm_backward_workspace_bytes(rows, cols))
+    return int(_load().b2_layernorm_backward_workspace_bytes(rows, cols))
 
 
 def layernorm_backward_workspace_bytes(rows: int, cols: int) -> int:
@@ -142,7 +163,10 @@ def layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, 
     ``dbeta`` (gamma's type) are each written unless None.  ``workspace``: a tensor of at least
     ``layernorm_backward_workspace_bytes(rows, cols)`` bytes that no other call uses meanwhile; None takes one from torch's
     allocator on the current stream for this call.  Returns ``(dx, dgamma, dbeta)``."""
-    L = _lib.load()
+    if _quick and lddy is None and ldx is None and lddx is None and \
+            _quick.layernorm_backward(handle, rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, workspace):
+        return dx, dgamma, dbeta
+    L = _load()
     _tensor(x, "x")
     device = torch.cuda.current_device()
     t = _type(x, "x")
@@ -198,12 +222,14 @@ def w4_quantize(N, K, group, W, codes, scales, zeros=None, *, ldw=None, ldq=None
     """Quantises W (N x K) to 4 bits in groups of ``group`` along K: ``codes`` (uint8, two per byte), ``scales`` (any of the
     three types) and, when ``zeros`` (uint8) is given, zero points; otherwise symmetric around 8.  ``w4_empty`` makes the
     three tensors.  Returns ``(codes, scales, zeros)``."""
+    if _quick and ldw is None and ldq is None and _quick.w4_quantize(handle, N, K, group, W, codes, scales, zeros):
+        return codes, scales, zeros
     _tensor(W, "W")
     device = torch.cuda.current_device()
     t = _type(W, "W")
     pw, ldw = _matrix(W, N, K, ldw, "W", device)
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
-    check(_lib.load().b2_w4_quantize(_raw(handle, device), N, K, group, t, pw, ldw, pq, ldq, st, ps, pz, _stream(device)))
+    check(_load().b2_w4_quantize(_raw(handle, device), N, K, group, t, pw, ldw, pq, ldq, st, ps, pz, _stream(device)))
     return codes, scales, zeros
 
 
@@ -211,6 +237,8 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
                   handle: Handle | None = None):
     """Expands 4-bit weights to ``W``: N x K, or K x N with ``transpose`` (then the right operand of
     ``sgemm(M, N, K, alpha, X, W, beta, C)`` for C = X * W^T).  ``W`` None: a new tensor of ``dtype``.  Returns ``W``."""
+    if _quick and ldw is None and ldq is None and _quick.w4_dequantize(handle, N, K, group, codes, scales, zeros, 1 if transpose else 0, W):
+        return W
     _tensor(codes, "codes")
     device = torch.cuda.current_device()
     rows, cols = (K, N) if transpose else (N, K)
@@ -218,14 +246,14 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
         W = torch.empty((rows, cols), dtype=dtype, device=codes.device)
     pw, ldw = _matrix(W, rows, cols, ldw, "W", device)
     pq, ldq, st, ps, pz = _w4(N, K, group, codes, scales, zeros, ldq, device)
-    check(_lib.load().b2_w4_dequantize(_raw(handle, device), N, K, group, pq, ldq, st, ps, pz, _type(W, "W"), pw, ldw, 1 if transpose else 0,
+    check(_load().b2_w4_dequantize(_raw(handle, device), N, K, group, pq, ldq, st, ps, pz, _type(W, "W"), pw, ldw, 1 if transpose else 0,
                                        _stream(device)))
     return W
 
 
 @functools.lru_cache(maxsize=4096)
 def _w4_matvec_workspace(M, N, K, t) -> int:
-    return int(_lib.load().b2_w4_matvec_workspace_bytes(M, N, K, t))
+    return int(_load().b2_w4_matvec_workspace_bytes(M, N, K, t))
 
 
 def w4_matvec_workspace_bytes(M: int, N: int, K: int, dtype) -> int:
@@ -239,6 +267,9 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
     ``w4_dequantize`` once and ``sgemm``).  ``y`` None: a new tensor (beta must be 0).  ``workspace``: a tensor of at least
     ``w4_matvec_workspace_bytes(M, N, K, x.dtype)`` bytes that no other call uses meanwhile; None takes one from torch's allocator
     on the current stream for this call.  Returns ``y``."""
+    if _quick and ldx is None and ldy is None and ldq is None and \
+            _quick.w4_matvec(handle, M, N, K, group, alpha, x, codes, scales, zeros, beta, y, workspace):
+        return y
     _tensor(x, "x")
     device = torch.cuda.current_device()
     if y is None:
@@ -258,5 +289,5 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
             ws = workspace.data_ptr()
     else:
         ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
-    check(_lib.load().b2_w4_matvec(_raw(handle, device), M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
+    check(_load().b2_w4_matvec(_raw(handle, device), M, N, K, group, alpha, t, px, ldx, pq, ldq, st, ps, pz, beta, py, ldy, ws, ws_bytes, _stream(device)))
     return y

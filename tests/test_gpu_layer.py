@@ -765,3 +765,96 @@ def test_handles_and_devices(b2):
     own = b2.Handle()
     assert torch.equal(b2.layernorm(4, 64, 1e-5, x, gamma, beta, handle=own), b2.layernorm(4, 64, 1e-5, x, gamma, beta))
     own.close()
+
+
+def test_short_and_long_calls_agree(b2, monkeypatch):
+    """Usual calls go through the extension, others (a pitch by name, a handle of the caller's that is not the default, tensors that
+    are slices) through the checks in Python: the same bits, the same errors."""
+    from hpcdeepneuralnetworks_b200 import layer
+    b2.default_handle()
+    layer._load()
+    quick = layer._quick
+    x, gamma, beta, dy = [t.cuda() for t in norm_inputs(33, 300, torch.bfloat16, torch.float32, 4)]
+    W = weights(70, 500, 9, torch.bfloat16).cuda()
+    xs = torch.randn(9, 500, generator=gen(3)).to(torch.bfloat16).cuda()
+
+    def everything(pitch):
+        ld = dict(ldx=300) if pitch else {}
+        mean, rstd = torch.zeros(33, device="cuda"), torch.zeros(33, device="cuda")
+        y = b2.layernorm(33, 300, 1e-5, x, gamma, beta, torch.empty_like(x), mean=mean, rstd=rstd, **ld)
+        dx, dg, db = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(gamma)
+        b2.layernorm_backward(33, 300, dy, x, gamma, mean, rstd, dx, dg, db, **ld)
+        codes, scales, zeros = b2.w4_empty(70, 500, 64, zeros=True)
+        ldq = dict(ldq=codes.stride(0)) if pitch else {}
+        b2.w4_quantize(70, 500, 64, W, codes, scales, zeros, **ldq)
+        out = torch.empty(500, 70, device="cuda")
+        b2.w4_dequantize(70, 500, 64, codes, scales, zeros, out, transpose=True, **ldq)
+        p = b2.w4_matvec(9, 70, 500, 64, 1.0, xs, codes, scales, zeros, 0.0, torch.empty(9, 70, dtype=xs.dtype, device="cuda"), **ldq)
+        return [y, mean, rstd, dx, dg, db, codes.clone(), scales, zeros, out, p]
+
+    taken = []
+
+    class Spy:
+        def __getattr__(self, name):
+            def f(*args):
+                taken.append((name, getattr(quick, name)(*args)))
+                return taken[-1][1]
+            return f
+    monkeypatch.setattr(layer, "_quick", Spy())
+    short = everything(False)
+    assert taken == [(n, True) for n in ("layernorm", "layernorm_backward", "w4_quantize", "w4_dequantize", "w4_matvec")]
+    taken.clear()
+    long = everything(True)
+    assert not taken
+    for a, b in zip(short, long):
+        assert torch.equal(a, b)
+    # a batch of sequences, by its leading dimensions
+    three = b2.layernorm(33, 300, 1e-5, x.view(3, 11, 300), gamma, beta, torch.empty(3, 11, 300, dtype=x.dtype, device="cuda"))
+    assert taken.pop() == ("layernorm", True) and torch.equal(three.view(33, 300), short[0])
+    # what the library refuses, and what is no usual call, is said as before
+    with pytest.raises(b2.B2Error, match="overlaps"):
+        flat = torch.zeros(34 * 300, dtype=x.dtype, device="cuda")
+        b2.layernorm(33, 300, 1e-5, flat[:33 * 300].view(33, 300), gamma, beta, flat[300:].view(33, 300))
+    with pytest.raises(b2.B2Error, match="workspace"):
+        b2.layernorm_backward(33, 300, dy, x, gamma, short[1], short[2], None, short[4], None, workspace=torch.empty(8, device="cuda"))
+    with pytest.raises(TypeError):
+        b2.layernorm(33, 300, 1e-5, x, gamma.double(), beta, torch.empty_like(x))
+    with pytest.raises(ValueError):
+        b2.layernorm(34, 300, 1e-5, x, gamma, beta, torch.empty_like(x))
+    with pytest.raises(ValueError, match="group 33"):
+        b2.w4_quantize(70, 500, 33, W, short[6], short[7])
+    sliced = b2.layernorm(33, 200, 1e-5, x[:, :200], gamma[:200], beta[:200], torch.empty(33, 200, dtype=x.dtype, device="cuda"))
+    check_forward(x[:, :200].cpu(), gamma[:200].cpu(), beta[:200].cpu(), 1e-5, sliced, None, None, 200)
+    assert all(ok is False for _, ok in taken)
+    other = b2.Handle()
+    assert torch.equal(b2.layernorm(33, 300, 1e-5, x, gamma, beta, torch.empty_like(x), handle=other), short[0]) and taken.pop()[1] is True
+
+
+def test_first_calls_ever_inside_a_capture():
+    """A process whose first calls are captured: nothing that the first call of a kernel sets up may break the capture."""
+    import subprocess
+    import sys
+    code = """
+import torch, hpcdeepneuralnetworks_b200 as b2
+b2.default_handle()
+x = torch.randn(40, 512, device="cuda"); g = torch.randn(512, device="cuda"); y = torch.empty_like(x)
+m, r = torch.empty(40, device="cuda"), torch.empty(40, device="cuda"); dx = torch.empty_like(x); dg, db = torch.empty_like(g), torch.empty_like(g)
+codes, s, _ = b2.w4_empty(256, 512, 64); W = torch.randn(256, 512, device="cuda"); back = torch.empty_like(W); p = torch.empty(40, 256, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    b2.layernorm(40, 512, 1e-5, x, g, None, y, mean=m, rstd=r)
+    b2.layernorm_backward(40, 512, y, x, g, m, r, dx, dg, db)
+    b2.w4_quantize(256, 512, 64, W, codes, s)
+    b2.w4_dequantize(256, 512, 64, codes, s, None, back)
+    b2.w4_matvec(40, 256, 512, 64, 1.0, y, codes, s, None, 0.0, p)
+graph.replay()
+torch.cuda.synchronize()
+want = torch.nn.functional.layer_norm(x.double(), (512,), g.double())
+assert float((y - want).abs().max()) < 1e-4
+assert float((p - y.double() @ back.double().t()).abs().max()) < 1e-2
+print("captured")
+"""
+    import os
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]

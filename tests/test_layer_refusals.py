@@ -214,3 +214,17 @@ def test_reference_packing_round_trip():
     off = (ref.w4_values(codes, scales, zeros, 32) - W.double()).abs()
     # a code is off by half a step, and by up to half a step more where the zero point was rounded and the code clamped
     assert bool((off <= 1.001 * scales.double()[:, torch.arange(100) // 32]).all())
+
+
+def test_short_calls_leave_everything_unusual_to_the_checks(built_lib):
+    """The extension answers False to what it does not know, whatever that is, and never calls the library for it."""
+    layer._load()
+    quick, t, i = layer._quick, torch.zeros(4, 8), 2 ** 70
+    for name, count in (("layernorm", 10), ("layernorm_backward", 12), ("w4_quantize", 8), ("w4_dequantize", 9), ("w4_matvec", 13)):
+        f = getattr(quick, name)
+        for args in ([], [None] * (count - 1), [None] * count, [t] * count, [1] * count, [None] + [i] * (count - 1), ["x"] * count,
+                     [None] + [4] * 3 + [t] * (count - 4), [object()] + [4, 8] + [fake(4, 8)] * (count - 3)):
+            assert f(*args) is False, (name, args)
+    for args in ((), (1,) * 8, ({},) + ("x",) * 7):
+        with pytest.raises(TypeError):
+            quick.bind(*args)
