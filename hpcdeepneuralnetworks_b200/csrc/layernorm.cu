@@ -6,8 +6,8 @@
 // are off by the same amount in all matrices are taken in 16 bytes with their ends masked (PHASED).  Longer rows are read again
 // instead of held.
 // Measured, device time: forward 16384 x 4096 bf16 47.7 us (5.6 TB/s of the 268 MB it must move, 0.87 of a copy), 8192 x 4095
-// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 75 us (5.4 TB/s, 0.83), 8192 x 4095 73 us, 5003 x 1027 FP32
-// 22 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
+// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 72 us (5.6 TB/s, 0.87), 8192 x 4095 68 us, 5003 x 1027 FP32
+// 22 us, 64 x 4096 6.6 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
 // latency of a row's two sums, with 10 to 16 warps to an SM.
 #include <math.h>
 
@@ -519,8 +519,11 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(int64_t rows, int 
   }
 }
 
+constexpr __host__ __device__ int ln_padded(int cols) { return cols + (cols >> 5) + 1; }
+
 // Backward: a team walks over its rows and keeps the sums dy * xhat and dy of its columns in registers over all of them; the
-// teams' sums end as one line of `partial` per block.
+// teams' sums meet in shared memory and end as one line of `partial` per block (team after team into one line: 600 x 4096 bf16
+// 19.5 us instead of 11.6, 60 x 300 FP32 11.3 instead of 5.5).
 //   xhat = (x - mean) * rstd,  u = dy * gamma,  dx = rstd * (u - sum(u) / n - xhat * sum(u * xhat) / n)
 // dx may be dy: a thread writes only what it has read.
 template <class T, class P, int V, int E, bool FULL, bool PHASED>
@@ -533,7 +536,7 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
   constexpr bool RING = V * sizeof(T) >= 4, ALL = FULL || RING;      // ALL: accesses outside the row read zeros
   __shared__ LnScratch scratch[2];
   extern __shared__ __align__(16) unsigned char dynamic[];
-  float *const joined = reinterpret_cast<float *>(dynamic);                // at the end, with several teams: [2][cols]
+  float *const joined = reinterpret_cast<float *>(dynamic);                // at the end: [team][2][ln_padded(cols)]
   pdl_launch_dependents();
   const LnTeam t(share);
   if (FULL) turns = N;
@@ -655,37 +658,39 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
   }
   if constexpr (RING) ln_wait<0>();
   if (!partial) return;
-  float *line = partial + (int64_t)blockIdx.x * 2 * cols;
-  float *const sums = t.teams > 1 ? joined : line;
+  // each team's sums side by side in shared memory, then a column's over the teams in their order; a word in 33 is skipped, which
+  // spreads accesses V words apart over the banks
+  float *const line = partial + (int64_t)blockIdx.x * 2 * cols, *const sums = joined + t.team * 2 * ln_padded(cols);
   __syncthreads();                                   // the ring's memory is used again
-  for (int w = 0; w < t.teams; ++w) {                // team by team, in order
-    if (t.team == w) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (FULL || i < valid) {
+  for (int i = 0; i < N; ++i)
+    if (FULL || i < valid) {
 #pragma unroll
-          for (int k = 0; k < K; ++k) {
-            float two[2][2];
-            if constexpr (W == 2) {
-              const float2 p = dg[i * K + k].both(), q = db[i * K + k].both();
-              two[0][0] = p.x, two[0][1] = p.y, two[1][0] = q.x, two[1][1] = q.y;
-            } else {
-              two[0][0] = dg[i * K + k].v, two[1][0] = db[i * K + k].v;
-            }
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-              const int c = (int)col + i * 32 * V + k * W + e;
-              if (PHASED && !phase.inside(i, k * W + e)) continue;
-              sums[c] = w ? sums[c] + two[0][e] : two[0][e];
-              sums[cols + c] = w ? sums[cols + c] + two[1][e] : two[1][e];
-            }
-          }
+      for (int k = 0; k < K; ++k) {
+        float two[2][2];
+        if constexpr (W == 2) {
+          const float2 p = dg[i * K + k].both(), q = db[i * K + k].both();
+          two[0][0] = p.x, two[0][1] = p.y, two[1][0] = q.x, two[1][1] = q.y;
+        } else {
+          two[0][0] = dg[i * K + k].v, two[1][0] = db[i * K + k].v;
         }
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const int c = (int)col + i * 32 * V + k * W + e;
+          if (PHASED && !phase.inside(i, k * W + e)) continue;
+          sums[c + (c >> 5)] = two[0][e];
+          sums[ln_padded(cols) + c + (c >> 5)] = two[1][e];
+        }
+      }
     }
-    if (t.teams > 1) __syncthreads();
-  }
-  if (t.teams > 1)
-    for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) line[c] = joined[c];
+  __syncthreads();
+  for (int which = 0; which < 2; ++which)
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      const float *from = joined + which * ln_padded(cols) + c + (c >> 5);
+      float sum = from[0];
+      for (int w = 1; w < t.teams; ++w) sum += from[w * 2 * ln_padded(cols)];
+      line[which * cols + c] = sum;
+    }
 }
 
 // Rows too long for that: their sums of u and u * xhat first (one block per row), then everything else by tiles of columns,
@@ -1029,11 +1034,19 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
           const auto kernel = full ? layernorm_backward_kernel<T, P, V, E, !PHASED, PHASED> : layernorm_backward_kernel<T, P, V, E, false, PHASED>;
           const int64_t fit = share <= 256 ? 256 / share : 1;
           const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
-          if ((rows + teams - 1) / teams < parts) parts = (int)((rows + teams - 1) / teams);
+          // A block per SM before any block takes a second turn, then two turns before there are more blocks: a line of sums per
+          // block costs as much as a row or two (248 x 7424 FP32 17.5 -> 11.1 us with two turns, 2213 x 76 bf16 8.1 -> 6.3; with fewer
+          // blocks than SMs it loses: 60 x 300 5.5 -> 6.1)
+          const int64_t turn = (rows + teams - 1) / teams, wanted = turn <= ctx->sm_count ? turn : (turn + 1) / 2 < ctx->sm_count ? ctx->sm_count : (turn + 1) / 2;
+          const int limit = parts;
+          if (wanted < parts) parts = (int)wanted;
+          if (PHASED && (int64_t)parts * teams < rows) parts = (parts + V - 1) / V * V;
+          if (parts > limit) parts = limit;      // (all rows, one each, or 296, a multiple of V)
           size_t smem = V * sizeof(T) >= 4 ? (size_t)(kLnAhead + 1) * 2 * E * sizeof(T) * threads : 0;
           smem += (size_t)(PHASED ? threads : share) * E * sizeof(float);       // gamma
-          if (teams > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
-          result = ensure_func_attributes((const void *)kernel, ctx->device, ((kLnAhead + 1) * 2 * sizeof(T) + sizeof(float)) * E * 512);
+          const size_t joined = (size_t)teams * 2 * ln_padded((int)cols) * sizeof(float);
+          if (smem < joined) smem = joined;
+          result = ensure_func_attributes((const void *)kernel, ctx->device, 224 * 1024);
           if (result != B2_OK) return;
           kernel<<<parts, threads, smem, s>>>(rows, (int)cols, share, turns, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd,
                                               (T *)dx, lddx, partial);
