@@ -6,8 +6,8 @@
 // are off by the same amount in all matrices are taken in 16 bytes with their ends masked (PHASED).  Longer rows are read again
 // instead of held.
 // Measured, device time: forward 16384 x 4096 bf16 47.7 us (5.6 TB/s of the 268 MB it must move, 0.87 of a copy), 8192 x 4095
-// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 72 us (5.6 TB/s, 0.87), 8192 x 4095 68 us, 5003 x 1027 FP32
-// 22 us, 64 x 4096 6.6 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
+// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 72 us (5.6 TB/s, 0.87), 8192 x 4095 63 us, 5003 x 1027 FP32
+// 20.4 us, 64 x 4096 6.6 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
 // latency of a row's two sums, with 10 to 16 warps to an SM.
 #include <math.h>
 
@@ -799,10 +799,10 @@ __global__ void __launch_bounds__(1024) layernorm_reduce_kernel(int parts, int c
 constexpr int kLnBlock = 384;           // threads of a block of several teams, forward
 constexpr int kLnHeldBackward = 16;       // elements per thread, backward
 constexpr int kLnLongestBackward = 8192;  // 512 threads of 16 elements, or 1024 of 8
-// Most blocks, and lines of partial sums: two blocks on each of 148 SMs; the longest rows, whose lines are long and whose blocks
+// Most blocks, and lines of partial sums: three blocks on each of 148 SMs (as many as an SM may hold); the longest rows, whose lines are long and whose blocks
 // share the columns, take about 1184 blocks of 1024 columns and give each 8 rows at least (300 x 16384 bf16: 34 -> 18 us).
 static int64_t ln_parts(int64_t rows, int64_t cols) {
-  int64_t most = 296;
+  int64_t most = 444;
   if (cols > kLnLongestBackward) {
     most = 1184 * 1024 / cols;
     if (most > rows / 8) most = rows / 8;
@@ -1034,28 +1034,33 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
           const auto kernel = full ? layernorm_backward_kernel<T, P, V, E, !PHASED, PHASED> : layernorm_backward_kernel<T, P, V, E, false, PHASED>;
           const int64_t fit = share <= 256 ? 256 / share : 1;
           const int teams = (int)(fit < rows ? fit : rows), threads = share * teams;
-          // A block per SM before any block takes a second turn, then two turns before there are more blocks: a line of sums per
-          // block costs as much as a row or two (248 x 7424 FP32 17.5 -> 11.1 us with two turns, 2213 x 76 bf16 8.1 -> 6.3; with fewer
-          // blocks than SMs it loses: 60 x 300 5.5 -> 6.1)
-          const int64_t turn = (rows + teams - 1) / teams, wanted = turn <= ctx->sm_count ? turn : (turn + 1) / 2 < ctx->sm_count ? ctx->sm_count : (turn + 1) / 2;
-          const int limit = parts;
-          if (wanted < parts) parts = (int)wanted;
-          if (PHASED && (int64_t)parts * teams < rows) parts = (parts + V - 1) / V * V;
-          if (parts > limit) parts = limit;      // (all rows, one each, or 296, a multiple of V)
           size_t smem = V * sizeof(T) >= 4 ? (size_t)(kLnAhead + 1) * 2 * E * sizeof(T) * threads : 0;
           smem += (size_t)(PHASED ? threads : share) * E * sizeof(float);       // gamma
           const size_t joined = (size_t)teams * 2 * ln_padded((int)cols) * sizeof(float);
           if (smem < joined) smem = joined;
           result = ensure_func_attributes((const void *)kernel, ctx->device, 224 * 1024);
           if (result != B2_OK) return;
+          // A block per SM before any block takes a second turn, then two turns before there are more blocks: a line of sums per
+          // block costs as much as a row or two (248 x 7424 FP32 17.5 -> 11.1 us with two turns, 2213 x 76 bf16 8.1 -> 6.3; with fewer
+          // blocks than SMs it loses: 60 x 300 5.5 -> 6.1)
+          const int64_t turn = (rows + teams - 1) / teams, wanted = turn <= ctx->sm_count ? turn : (turn + 1) / 2 < ctx->sm_count ? ctx->sm_count : (turn + 1) / 2;
+          int held = 1;      // blocks that an SM holds at once (three where registers allow: 16384 x 2049 FP32 104 -> 94 us)
+          result = ln_blocks_per_sm((const void *)kernel, ctx->device, threads, smem, &held);
+          if (result != B2_OK) return;
+          if ((int64_t)held * ctx->sm_count < parts) parts = held * ctx->sm_count;
+          const int limit = parts;
+          if (wanted < parts) parts = (int)wanted;
+          if (PHASED && (int64_t)parts * teams < rows) parts = (parts + V - 1) / V * V;
+          if (parts > limit) parts = (int64_t)limit * teams < rows ? limit / V * V : limit;
           kernel<<<parts, threads, smem, s>>>(rows, (int)cols, share, turns, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd,
                                               (T *)dx, lddx, partial);
         };
         // Elements one by one take more registers and instructions each: fewer of them, in more threads (5003 x 1027 FP32: 35 -> 23 us)
         if constexpr (V == 16 / (int)sizeof(T)) {
           if (phased) {
-            // 16 bytes against the widest access that fits: 8192 x 4095 bf16 257 -> 73 us, 16384 x 2050 84 -> 63 (8 elements per thread:
-            // 93), 5003 x 1027 FP32 23.4 -> 21.9 (16 elements: 30.5), 40000 x 517 FP32 64 -> 59 (16: 108), 40000 x 131 FP16 47 -> 26.5 (16: 31)
+            // 16 bytes against the widest access that fits, when this was chosen: 8192 x 4095 bf16 257 -> 73 us, 16384 x 2050 84 -> 63 (8
+            // elements per thread: 93), 5003 x 1027 FP32 23.4 -> 21.9 (16 elements: 30.5), 40000 x 517 FP32 64 -> 59 (16: 108), 40000 x 131
+            // FP16 47 -> 26.5 (16: 31); by now 63, 52, 20.4, 59 and 21
             if (cols + V <= (V == 4 ? 512 : 32) * 8) run(std::integral_constant<int, 8>(), std::true_type());
             else run(std::integral_constant<int, kLnHeldBackward>(), std::true_type());
             return;
