@@ -114,7 +114,7 @@ __device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
   }
 }
 
-// Quantising should be bound by reading W; at 8 instructions per element it nearly is (8192 x 8192 bf16: 43 us, 3.9 TB/s; a copy
+// Quantising should be bound by reading W; at 8 instructions per element it nearly is (8192 x 8192 bf16: 45 us, 3.8 TB/s; a copy
 // of those bytes takes 26).  group / 16 lanes share a group, 16
 // elements (8 bytes of codes) each: a group's extremes take log2(group / 16) shuffles.  Nearly every element's code is what the
 // magic addition in w4_nearest gives at once: w / s + 1.5 * 2^23 holds it in its low bits.  Elements that are not nearer than
