@@ -114,8 +114,8 @@ __device__ __forceinline__ void w4_load(float (&v)[V], const T *p) {
   }
 }
 
-// Quantising should be bound by reading W; at 8 instructions per element it nearly is (8192 x 8192 bf16: 45 us, 3.8 TB/s; a copy
-// of those bytes takes 26).  group / 16 lanes share a group, 16
+// Quantising should be bound by reading W, and is by its 22 instructions per element, which take 82 % of the issue slots (8192 x 8192
+// bf16: 45 us, 3.8 TB/s; a copy of those bytes takes 26).  group / 16 lanes share a group, 16
 // elements (8 bytes of codes) each: a group's extremes take log2(group / 16) shuffles.  Nearly every element's code is what the
 // magic addition in w4_nearest gives at once: w / s + 1.5 * 2^23 holds it in its low bits.  Elements that are not nearer than
 // s / 2 to their codes' values (with 16-bit weights a third of the warps meet one that is exactly s / 2 away), and all of a group
@@ -296,9 +296,9 @@ __device__ __forceinline__ uint32_t w4_word(const uint8_t *row, int64_t at, int6
   return word;
 }
 
-// Expanding is bound by writing W (8192 x 8192 to bf16: 38 us, 4.5 TB/s, of a copy's 6.5).  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight.
+// Expanding is bound by writing W (8192 x 8192 to bf16: 37 us, 4.6 TB/s, of a copy's 6.5).  Rows as they lie: a thread takes 8 codes (one word) to 8 elements, four such units in flight.
 // CVEC: words of codes start on 4 bytes.  WVEC: 16 bytes of W start on 16; otherwise a warp's 256 elements pass through shared
-// memory, so that its stores lie side by side (8192 x 8190 bf16: 171 us with each lane writing its own elements).
+// memory, so that its stores lie side by side (8192 x 8190 bf16: 57 us; 171 with each lane writing its own elements).
 template <class T, class S, bool CVEC, bool WVEC>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K, int group_shift, const uint8_t *codes, int64_t ldq,
                                                             const S *scales, const uint8_t *zeros, T *W, int64_t ldw) {
@@ -308,27 +308,28 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
   };
   __shared__ Eight staged[WVEC ? 1 : 8][WVEC ? 1 : 32];
   const int64_t groups = (K + (1 << group_shift) - 1) >> group_shift, width = (K + 1) >> 1;
-  const int units = (int)((K + 7) >> 3), step = (int)(gridDim.x * blockDim.x);
+  // within a row 32 bits do (K < 2^31); a row's units are fewer than 2^28, and kFlight steps fewer than 2^30
+  const uint32_t units = (uint32_t)((K + 7) >> 3), step = gridDim.x * blockDim.x, k32 = (uint32_t)K;
   const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31, warp = (threadIdx.y * blockDim.x + threadIdx.x) >> 5;
   const bool wide = blockDim.x >= 32;                                     // a warp's lanes lie in one row
   // every thread takes every turn: warps work together
   for (int64_t nb = (int64_t)blockIdx.y * blockDim.y; nb < N; nb += (int64_t)gridDim.y * blockDim.y) {
     const int64_t n = nb + threadIdx.y;
-    const int mine = n < N ? units : 0;
+    const uint32_t mine = n < N ? units : 0;
     const uint8_t *row = codes + n * ldq;
     const S *scale_row = scales + n * groups;
     const uint8_t *zero_row = zeros ? zeros + n * groups : nullptr;
     T *out = W + n * ldw;
-    for (int64_t ub = (int64_t)blockIdx.x * blockDim.x; ub < units; ub += (int64_t)kFlight * step) {
+    for (uint32_t ub = blockIdx.x * blockDim.x; ub < units; ub += kFlight * step) {
       uint32_t word[kFlight];
       float scale[kFlight], zero[kFlight];
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
-        const int64_t u = ub + threadIdx.x + (int64_t)i * step;
+        const uint32_t u = ub + threadIdx.x + i * step;
         word[i] = 0;
         scale[i] = zero[i] = 0.f;
         if (u < mine) {
-          if (CVEC && 8 * u + 8 <= K) word[i] = __ldcs(reinterpret_cast<const unsigned int *>(row + 4 * u));
+          if (CVEC && 8 * u + 8 <= k32) word[i] = __ldcs(reinterpret_cast<const unsigned int *>(row + 4 * u));
           else word[i] = w4_word(row, 4 * u, width);
           scale[i] = to_f32(scale_row[(8 * u) >> group_shift]);
           zero[i] = zero_row ? (float)(zero_row[(8 * u) >> group_shift] & 15) : 8.f;
@@ -336,8 +337,8 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
       }
 #pragma unroll
       for (int i = 0; i < kFlight; ++i) {
-        const int64_t u = ub + threadIdx.x + (int64_t)i * step;
-        if (ub + (int64_t)i * step >= units) break;                       // for the whole block
+        const uint32_t u = ub + threadIdx.x + i * step;
+        if (ub + i * step >= units) break;                       // for the whole block
         float v[8];
         w4_expand(v, word[i], scale[i], zero[i]);
         union {
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
 #pragma unroll
         for (int k = 0; k < 8; ++k) o.all.e[k] = from_f32<T>(v[k]);
         T *to = out + 8 * u;
-        if (WVEC && 8 * u + 8 <= K) {
+        if (WVEC && 8 * u + 8 <= k32) {
           if (u < mine) {
 #pragma unroll
             for (int q = 0; q < (int)sizeof(T) / 2; ++q) __stcs(reinterpret_cast<uint4 *>(to) + q, o.q[q]);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
           staged[warp][lane] = o.all;
           __syncwarp();
           const T *flat = reinterpret_cast<const T *>(staged[warp]);
-          const int64_t from = 8 * (u - lane), behind = n < N ? K - from : 0;
+          const int64_t from = 8 * (int64_t)(u - lane), behind = n < N ? K - from : 0;
           T *const first = out + from + lane;
           const int end = (behind > 256 ? 256 : (int)behind) - lane;
 #pragma unroll
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(int64_t N, int64_t K
         } else if (u < mine) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            if (8 * u + k < K) to[k] = o.all.e[k];
+            if (8 * u + k < k32) to[k] = o.all.e[k];
         }
       }
     }

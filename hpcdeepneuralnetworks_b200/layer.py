@@ -32,7 +32,10 @@ def _load():
     global _quick
     L = _lib.load()
     if _quick is None:
-        quick = importlib.import_module(__package__ + "._calls")
+        try:
+            quick = importlib.import_module(__package__ + "._calls")
+        except ImportError as e:
+            raise ImportError("_calls.so is missing or was built for another torch: run `python -m hpcdeepneuralnetworks_b200.build`") from e
         names = ("b2_layernorm", "b2_layernorm_backward_workspace_bytes", "b2_layernorm_backward", "b2_w4_quantize", "b2_w4_dequantize",
                  "b2_w4_matvec_workspace_bytes", "b2_w4_matvec")
         quick.bind(_default, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
