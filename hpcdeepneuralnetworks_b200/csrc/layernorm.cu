@@ -757,14 +757,14 @@ __global__ void __launch_bounds__(128) layernorm_columns_kernel(int64_t rows, in
     if (dx) xv.store(dx + row * lddx + c);
   }
   if (!partial) return;
-  float *line = partial + (int64_t)blockIdx.y * 2 * cols + c;
+  float *const line = partial + (int64_t)blockIdx.y * 2 * cols + c, *const second = line + cols;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if constexpr (W == 2) {
       const float2 p = dg[k].both(), q = db[k].both();
-      line[2 * k] = p.x, line[2 * k + 1] = p.y, line[cols + 2 * k] = q.x, line[cols + 2 * k + 1] = q.y;
+      line[2 * k] = p.x, line[2 * k + 1] = p.y, second[2 * k] = q.x, second[2 * k + 1] = q.y;
     } else {
-      line[k] = dg[k].v, line[cols + k] = db[k].v;
+      line[k] = dg[k].v, second[k] = db[k].v;
     }
   }
 }

@@ -9,6 +9,7 @@
 namespace b2 {
 
 constexpr int kW4MaxRows = 64;   // rows of x that b2_w4_matvec takes
+constexpr int64_t kW4MaxK = 1 << 27;   // and their length: one block lays a row out, while the product's bounded waits run
 
 __device__ __forceinline__ float w4_warp_max(float v) {
 #pragma unroll
@@ -1414,7 +1415,7 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 }
 
 size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t N, int64_t K, int type) {
-  if (M <= 0 || M > kW4MaxRows || N <= 0 || K <= 0 || N > INT32_MAX || K > INT32_MAX || type_bytes(type) == 0) return 0;
+  if (M <= 0 || M > kW4MaxRows || N <= 0 || K <= 0 || N > INT32_MAX || K > kW4MaxK || type_bytes(type) == 0) return 0;
   if (mv_resident(M, N, K, type)) return 0;
   return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int2);
 }
@@ -1428,6 +1429,7 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   B2_REQUIRE(M >= 0, B2_ERR_INVALID_ARG, "b2_w4_matvec: M = %lld is negative", (long long)M);
   B2_REQUIRE(M <= kW4MaxRows, B2_ERR_UNSUPPORTED,
              "b2_w4_matvec: M = %lld exceeds %d rows: expand the weights with b2_w4_dequantize and use b2_sgemm", (long long)M, kW4MaxRows);
+  B2_REQUIRE(K <= kW4MaxK, B2_ERR_UNSUPPORTED, "b2_w4_matvec: K = %lld exceeds %lld", (long long)K, (long long)kW4MaxK);
   B2_REQUIRE(ldx >= K && ldy >= N, B2_ERR_INVALID_ARG, "b2_w4_matvec: ldx = %lld is less than K = %lld or ldy = %lld less than N = %lld",
              (long long)ldx, (long long)K, (long long)ldy, (long long)N);
   if (M == 0 || N == 0) return B2_OK;

@@ -266,7 +266,8 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 
 /* y = alpha * x * W^T + beta * y for M = 0..64 rows of x (M x K, ldx) and y (M x N, ldy), both of type `type`: the product of
  * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
- * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm.  y must not overlap x.
+ * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm; so does K above 2^27.  y must not
+ * overlap x.
  * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.  They are formed from rows of x
  * scaled to 2^15 by a power of two, so scales of a magnitude outside 2^-110 .. 2^90 may lose digits or overflow on the way.
  * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, N, K, type) bytes that no other call uses meanwhile, where x is

@@ -760,6 +760,30 @@ def test_offsets_beyond_32_bits(b2):
     assert torch.equal(big, c2)
 
 
+def test_w4_rows_as_long_as_they_may_be(b2):
+    """One row of nearly 2^31 weights, whole numbers that the codes reproduce, and a product of 2^27 of them."""
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 24 GB")
+    K, group = 2 ** 31 - 9, 256
+    codes = torch.randint(1, 16, (1, (K + 1) // 2), dtype=torch.uint8, device="cuda") * 16 + 1     # odd elements 1..15, even ones 1: -7
+    codes[0, -1] = 1
+    scales = torch.ones(1, -(-K // group), dtype=torch.float16, device="cuda")
+    W = b2.w4_dequantize(1, K, group, codes, scales, dtype=torch.float16)
+    for at in (0, 2 ** 28 - 4, 2 ** 30 - 4, K - 1001):
+        at -= at % 2
+        want = torch.stack([(codes[0, at // 2:at // 2 + 500] & 15), codes[0, at // 2:at // 2 + 500] >> 4], 1).view(-1).to(torch.int16) - 8
+        assert torch.equal(W[0, at:at + 1000][:K - at], want.to(torch.float16)[:K - at])
+    again, s2, _ = b2.w4_quantize(1, K, group, W, torch.empty_like(codes), torch.empty_like(scales))
+    assert torch.equal(again, codes) and bool((s2 == 1).all())
+    del W, again
+    K = 2 ** 27
+    x = torch.zeros(1, K, dtype=torch.float16, device="cuda")
+    x[0, 1::2 ** 12] = 1.0
+    got = b2.w4_matvec(1, 1, K, group, 1.0, x, codes[:, :K // 2], scales[:, :K // group].contiguous(), None, 0.0)
+    want = ((codes[0, :K // 2:2 ** 11] >> 4).double() - 8).sum()
+    assert abs(float(got) - float(want)) <= 2.0 ** -11 * abs(float(want)) + 1e-3
+
+
 def test_handles_and_devices(b2):
     x, gamma, beta, _ = [t.cuda() for t in norm_inputs(4, 64, torch.float32, torch.float32, 2)]
     own = b2.Handle()

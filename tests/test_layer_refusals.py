@@ -115,6 +115,12 @@ def test_w4_matvec_refuses_many_rows(L):
     assert b"b2_w4_dequantize" in L.b2_last_error()
 
 
+def test_w4_matvec_refuses_the_longest_rows(L):
+    K = 2 ** 27 + 1
+    assert matvec(L, K=K, ldx=K, ldq=K) == UNSUPPORTED
+    assert L.b2_w4_matvec_workspace_bytes(60, 4, K, BF16) == 0 < L.b2_w4_matvec_workspace_bytes(60, 4, K - 1, BF16)
+
+
 def test_w4_matvec_workspace(L):
     for type_ in (F32, BF16, F16):
         need = L.b2_w4_matvec_workspace_bytes(60, 4, 64, type_)
