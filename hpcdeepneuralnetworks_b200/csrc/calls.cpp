@@ -3,8 +3,10 @@
 // and 7.4).
 //
 // Every function takes the operator's arguments by position, looks whether they are the usual ones (contiguous CUDA tensors
-// of the right sizes and types on the current device; codes may have a pitch), and if so calls the C ABI and returns True.  Otherwise, and when the
-// library refuses the call, it returns False and has done nothing: layer.py then checks one by one and says what is wrong.
+// of the right sizes and types on the current device; codes may have a pitch), and if so calls the C ABI and returns True.  Otherwise,
+// and when the library refuses the arguments (which it does before it touches the device), it returns False and has done nothing:
+// layer.py then checks one by one and says what is wrong.  Any other status comes back as a number: work may have been enqueued by
+// then, and an operator that writes over its input must not be called a second time.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -125,16 +127,18 @@ struct Call {
 
 template <class F>
 PyObject *guarded(Py_ssize_t given, Py_ssize_t wanted, F &&f) {
-  int st = -1;
+  int st = B2_ERR_INVALID_ARG;
   if (given == wanted && lib.layernorm) {
     try {
       st = f();
-    } catch (...) {      // layer.py meets the same and reports it
-      st = -1;
+    } catch (...) {      // before the library's call, which throws nothing: layer.py meets the same and reports it
+      st = B2_ERR_INVALID_ARG;
     }
   }
   PyErr_Clear();
-  return PyBool_FromLong(st == B2_OK);
+  if (st == B2_OK) Py_RETURN_TRUE;
+  if (st == B2_ERR_INVALID_ARG || st == B2_ERR_UNSUPPORTED || st == B2_ERR_WORKSPACE) Py_RETURN_FALSE;
+  return PyLong_FromLong(st);
 }
 struct WithoutGil {
   PyThreadState *state = PyEval_SaveThread();

@@ -905,6 +905,7 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
     using T = decltype(t);
     using P = decltype(p);
     int result = B2_OK;
+    cudaError_t launched = cudaSuccess;
     ln_with_width<T>(width, [&](auto w) {
       constexpr int V = decltype(w)::value;
       // E elements per thread, teams of threads to a row in blocks of about 256
@@ -933,8 +934,8 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
         if (result != B2_OK) return;
         int64_t most = (int64_t)ctx->sm_count * held;
         if (PHASED && blocks > most) most = most / V * V;
-        kernel<<<(unsigned)(blocks < most ? blocks : most), threads, smem, s>>>(
-            rows, (int)cols, share, turns, ahead, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
+        launched = launch_kernel(kernel, (unsigned)(blocks < most ? blocks : most), threads, smem, s, rows, (int)cols, share, turns, ahead, eps,
+                                 (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
       };
       constexpr int kFew = V == 8 ? 8 : 4, kMost = V >= 4 ? 32 : 16, kLong = V == 1 ? 16 : 32;
       using Half = std::integral_constant<int, 512>;
@@ -956,15 +957,13 @@ int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, c
       else if (cols <= 512 * kMost) run(std::integral_constant<int, kMost>(), Half(), Even());
       else if (cols <= 1024 * kLong) run(std::integral_constant<int, kLong>(), Full(), Even());
       else
-        layernorm_long_kernel<T, P, V><<<(unsigned)(rows < 1 << 30 ? rows : 1 << 30), 1024, 0, s>>>(
-            rows, (int)cols, eps, (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
+        launched = launch_kernel(layernorm_long_kernel<T, P, V>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), 1024, 0, s, rows, (int)cols, eps,
+                                 (const T *)x, ldx, (const P *)gamma, (const P *)beta, (T *)y, ldy, mean, rstd);
     });
+    if (result == B2_OK) B2_CUDA(launched);
     return result;
   };
-  const int st = with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
-  if (st != B2_OK) return st;
-  B2_CUDA(cudaGetLastError());
-  return B2_OK;
+  return with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
 }
 
 size_t b2_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols) {
@@ -1021,6 +1020,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
     using T = decltype(t);
     using P = decltype(p);
     int result = B2_OK;
+    cudaError_t launched = cudaSuccess;
     ln_with_width<T>(width, [&](auto w) {
       constexpr int V = decltype(w)::value;
       if (!is_long) {
@@ -1052,8 +1052,8 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
           if (wanted < parts) parts = (int)wanted;
           if (PHASED && (int64_t)parts * teams < rows) parts = (parts + V - 1) / V * V;
           if (parts > limit) parts = (int64_t)limit * teams < rows ? limit / V * V : limit;
-          kernel<<<parts, threads, smem, s>>>(rows, (int)cols, share, turns, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd,
-                                              (T *)dx, lddx, partial);
+          launched = launch_kernel(kernel, parts, threads, smem, s, rows, (int)cols, share, turns, (const T *)dy, lddy, (const T *)x, ldx,
+                                   (const P *)gamma, mean, rstd, (T *)dx, lddx, partial);
         };
         // Elements one by one take more registers and instructions each: fewer of them, in more threads (5003 x 1027 FP32: 35 -> 23 us)
         if constexpr (V == 16 / (int)sizeof(T)) {
@@ -1070,12 +1070,14 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
         else run(std::integral_constant<int, kLnHeldBackward>(), std::false_type());
       } else {
         if (dx)
-          layernorm_row_sums_kernel<T, P, V><<<(unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s>>>(
-              rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums);
-        layernorm_columns_kernel<T, P, V><<<dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s>>>(
-            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
+          launched = launch_kernel(layernorm_row_sums_kernel<T, P, V>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows,
+                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums);
+        if (launched == cudaSuccess)
+          launched = launch_kernel(layernorm_columns_kernel<T, P, V>, dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s, rows,
+                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
       }
     });
+    if (result == B2_OK) B2_CUDA(launched);
     if (result == B2_OK && sums) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3((unsigned)((cols + 31) / 32));
@@ -1090,10 +1092,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
     }
     return result;
   };
-  const int st = with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
-  if (st != B2_OK) return st;
-  B2_CUDA(cudaGetLastError());
-  return B2_OK;
+  return with_type(type, [&](auto t) { return param_type == type ? launch(t, t) : launch(t, float()); });
 }
 
 }  // extern "C"

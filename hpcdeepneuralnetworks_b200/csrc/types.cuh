@@ -25,6 +25,18 @@ inline bool matrices_overlap(const void *a, int64_t rows_a, int64_t bytes_a, int
 }
 
 #ifdef __CUDACC__
+// kernel<<<grid, block, smem, stream>>>(args...), with the launch's own status.  cudaGetLastError after such a launch would also
+// report, for work that is on its way, what some earlier call of the thread has left behind.
+template <class... P, class... A>
+inline cudaError_t launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A &&...args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<A &&>(args)...);
+}
+
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }

@@ -1360,6 +1360,7 @@ int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const
   const uintptr_t place = (uintptr_t)W | (uintptr_t)(ldw * tb);
   const int align = (place & 15) == 0 ? 16 : (place & 3) == 0 ? 4 : 2;
   const bool qvec = (((uintptr_t)codes | (uintptr_t)ldq) & 7) == 0;
+  cudaError_t launched = cudaSuccess;
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
@@ -1371,9 +1372,9 @@ int b2_w4_quantize(b2_handle h, int64_t N, int64_t K, int group, int type, const
                           : (qvec ? w4_quantize_kernel<T, S, Z, kLeast, true> : w4_quantize_kernel<T, S, Z, kLeast, false>);
     };
     const auto kernel = zeros ? pick(std::true_type()) : pick(std::false_type());
-    kernel<<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
+    launched = launch_kernel(kernel, g.grid, g.block, 0, (cudaStream_t)stream, N, K, shift, (const T *)W, ldw, codes, ldq, (S *)scales, zeros);
   });
-  B2_CUDA(cudaGetLastError());
+  B2_CUDA(launched);
   return B2_OK;
 }
 
@@ -1390,6 +1391,7 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
              "b2_w4_dequantize: W overlaps the codes");
   B2_CONTEXT(ctx, h, "b2_w4_dequantize");
   const int shift = w4_group_shift(group);
+  cudaError_t launched = cudaSuccess;
   w4_with_types(type, scale_type, [&](auto t, auto s) {
     using T = decltype(t);
     using S = decltype(s);
@@ -1401,16 +1403,16 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
       const bool pair = kPair && (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 3) == 0;
       const auto kernel = pair ? (vec ? w4_transpose_kernel<T, S, true, kPair> : w4_transpose_kernel<T, S, false, kPair>)
                                : (vec ? w4_transpose_kernel<T, S, true, false> : w4_transpose_kernel<T, S, false, false>);
-      kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      launched = launch_kernel(kernel, grid, 256, 0, (cudaStream_t)stream, N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
     } else {
       const W4Grid g((K + 31) / 32, N, 1);      // four units of 8 to a thread
       const bool cvec = (((uintptr_t)codes | (uintptr_t)ldq) & 3) == 0, wvec = (((uintptr_t)W | (uintptr_t)(ldw * tb)) & 15) == 0;
       const auto kernel = cvec ? (wvec ? w4_dequantize_kernel<T, S, true, true> : w4_dequantize_kernel<T, S, true, false>)
                                : (wvec ? w4_dequantize_kernel<T, S, false, true> : w4_dequantize_kernel<T, S, false, false>);
-      kernel<<<g.grid, g.block, 0, (cudaStream_t)stream>>>(N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
+      launched = launch_kernel(kernel, g.grid, g.block, 0, (cudaStream_t)stream, N, K, shift, codes, ldq, (const S *)scales, zeros, (T *)W, ldw);
     }
   });
-  B2_CUDA(cudaGetLastError());
+  B2_CUDA(launched);
   return B2_OK;
 }
 
@@ -1457,13 +1459,14 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
     unsigned char *image = (unsigned char *)workspace;
     int2 *info = (int2 *)(image + mv_image_bytes(M, K, type));
     a.image = image, a.row_info = info;
+    cudaError_t launched = cudaSuccess;
     with_type(type, [&](auto t) {
       using T = decltype(t);
-      w4_x_kernel<T><<<(unsigned)M, kMvXThreads, 0, s>>>(K, ldx, a.vec, (const T *)x, a.chunks, nb, a.rows_per_item,
-                                                         a.group_shift < 7 ? a.group_shift : 7, image, info);
+      launched = launch_kernel(w4_x_kernel<T>, (unsigned)M, kMvXThreads, 0, s, K, ldx, a.vec, (const T *)x, a.chunks, nb, a.rows_per_item,
+                               a.group_shift < 7 ? a.group_shift : 7, image, info);
       return 0;
     });
-    B2_CUDA(cudaGetLastError());
+    B2_CUDA(launched);
   }
   const bool aligned = (((uintptr_t)codes | (uintptr_t)ldq) & 15) == 0;
   return w4_matvec_run(ctx, a, nb, resident, aligned, s);

@@ -43,6 +43,11 @@ def _load():
     return L
 
 
+def _done(answer) -> bool:
+    """Whether the extension made the call.  A status that may have come after a launch is an error, never a reason to call again."""
+    return answer is True or (answer is not False and check(answer) >= 0)
+
+
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
@@ -133,7 +138,7 @@ def layernorm(rows, cols, eps, x, gamma, beta, y=None, *, mean=None, rstd=None, 
     """y = (x - mean) * rstd * gamma + beta over the rows of x.  ``gamma``, ``beta``: ``cols`` elements of float32 or x's
     type, or None.  ``mean``, ``rstd``: float32 tensors of ``rows`` elements that receive the statistics, or None.
     ``y``: x's type, x itself for the norm in place, or None for a new tensor.  Returns ``y``."""
-    if _quick and ldx is None and ldy is None and _quick.layernorm(handle, rows, cols, eps, x, gamma, beta, y, mean, rstd):
+    if _quick and ldx is None and ldy is None and _done(_quick.layernorm(handle, rows, cols, eps, x, gamma, beta, y, mean, rstd)):
         return y
     _tensor(x, "x")
     device = torch.cuda.current_device()
@@ -167,7 +172,7 @@ def layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, 
     ``layernorm_backward_workspace_bytes(rows, cols)`` bytes that no other call uses meanwhile; None takes one from torch's
     allocator on the current stream for this call.  Returns ``(dx, dgamma, dbeta)``."""
     if _quick and lddy is None and ldx is None and lddx is None and \
-            _quick.layernorm_backward(handle, rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, workspace):
+            _done(_quick.layernorm_backward(handle, rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, workspace)):
         return dx, dgamma, dbeta
     L = _load()
     _tensor(x, "x")
@@ -225,7 +230,7 @@ def w4_quantize(N, K, group, W, codes, scales, zeros=None, *, ldw=None, ldq=None
     """Quantises W (N x K) to 4 bits in groups of ``group`` along K: ``codes`` (uint8, two per byte), ``scales`` (any of the
     three types) and, when ``zeros`` (uint8) is given, zero points; otherwise symmetric around 8.  ``w4_empty`` makes the
     three tensors.  Returns ``(codes, scales, zeros)``."""
-    if _quick and ldw is None and ldq is None and _quick.w4_quantize(handle, N, K, group, W, codes, scales, zeros):
+    if _quick and ldw is None and ldq is None and _done(_quick.w4_quantize(handle, N, K, group, W, codes, scales, zeros)):
         return codes, scales, zeros
     _tensor(W, "W")
     device = torch.cuda.current_device()
@@ -240,7 +245,8 @@ def w4_dequantize(N, K, group, codes, scales, zeros=None, W=None, *, transpose=F
                   handle: Handle | None = None):
     """Expands 4-bit weights to ``W``: N x K, or K x N with ``transpose`` (then the right operand of
     ``sgemm(M, N, K, alpha, X, W, beta, C)`` for C = X * W^T).  ``W`` None: a new tensor of ``dtype``.  Returns ``W``."""
-    if _quick and ldw is None and ldq is None and _quick.w4_dequantize(handle, N, K, group, codes, scales, zeros, 1 if transpose else 0, W):
+    if _quick and ldw is None and ldq is None and \
+            _done(_quick.w4_dequantize(handle, N, K, group, codes, scales, zeros, 1 if transpose else 0, W)):
         return W
     _tensor(codes, "codes")
     device = torch.cuda.current_device()
@@ -271,7 +277,7 @@ def w4_matvec(M, N, K, group, alpha, x, codes, scales, zeros, beta, y=None, *, l
     ``w4_matvec_workspace_bytes(M, N, K, x.dtype)`` bytes that no other call uses meanwhile; None takes one from torch's allocator
     on the current stream for this call.  Returns ``y``."""
     if _quick and ldx is None and ldy is None and ldq is None and \
-            _quick.w4_matvec(handle, M, N, K, group, alpha, x, codes, scales, zeros, beta, y, workspace):
+            _done(_quick.w4_matvec(handle, M, N, K, group, alpha, x, codes, scales, zeros, beta, y, workspace)):
         return y
     _tensor(x, "x")
     device = torch.cuda.current_device()
