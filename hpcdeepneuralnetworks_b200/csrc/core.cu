@@ -21,6 +21,7 @@ void set_error(const char *fmt, ...) {
 
 int cuda_fail(cudaError_t e, const char *what, const char *file, int line) {
   set_error("CUDA error %d (%s) in %s at %s:%d", (int)e, cudaGetErrorString(e), what, file, line);
+  (void)cudaGetLastError();   // the status reports it: left in the thread, the next check of anybody's launch would find it
   return B2_ERR_CUDA;
 }
 
@@ -39,6 +40,7 @@ static int context_init(Context *c) {
 Context *default_context() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    (void)cudaGetLastError();
     set_error("no usable CUDA device for the default handle");
     return nullptr;
   }
@@ -67,6 +69,7 @@ Context *resolve_context(b2_handle h, const char *who) {
   Context *c = reinterpret_cast<Context *>(h);
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev != c->device) {
+    if (dev < 0) (void)cudaGetLastError();
     set_error("%s: the handle belongs to device %d but device %d is current", who, c->device, dev);
     return nullptr;
   }
