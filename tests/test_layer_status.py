@@ -131,21 +131,19 @@ def test_an_error_left_by_an_earlier_call_does_not_touch_these(cuda):
         assert torch.equal(a, b)
 
 
-def test_an_error_that_a_status_reports_is_not_left_behind(built_lib):
-    """A runtime call that fails inside the library comes back as a status; the thread's last error, which other code of the process
-    (torch after each of its launches) would take for its own, is clear again.  The call that fails is
-    the first of a handle on a machine without a device."""
+@pytest.mark.gpu
+def test_an_error_that_a_status_reports_is_not_left_behind(cuda):
+    """A runtime call that fails inside the library (the time between two events that were never recorded) comes back as a status;
+    the thread's last error, which other code of the process would take for its own, is clear again."""
+    import hpcdeepneuralnetworks_b200 as b2
+    b2.default_handle()
     L = _lib.load()
     rt = C.CDLL("libcudart.so.12")
+    torch.cuda.synchronize()
+    timer, ms = C.c_void_p(), C.c_float()
+    assert L.b2_timer_create(C.byref(timer)) == 0
     rt.cudaGetLastError()
-    if torch.cuda.is_available():
-        pytest.skip("there is a device")
-    h = C.c_void_p()
-    assert L.b2_create(C.byref(h)) == CUDA
-    assert b"CUDA error" in L.b2_last_error()
-    assert rt.cudaPeekAtLastError() == 0
-    assert layer_call(L) == CUDA and rt.cudaPeekAtLastError() == 0
-
-
-def layer_call(L):
-    return L.b2_layernorm(None, 4, 8, 1e-5, 0, C.c_void_p(0x1000), 8, 0, None, None, C.c_void_p(0x2000), 8, None, None, None)
+    assert L.b2_timer_elapsed_ms(timer, C.byref(ms)) == CUDA
+    left = rt.cudaGetLastError()
+    L.b2_timer_destroy(timer)
+    assert left == 0 and b"CUDA error" in L.b2_last_error()
