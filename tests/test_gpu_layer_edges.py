@@ -1,0 +1,53 @@
+"""GPU tests of the layer operators where sums cancel, overflow or meet values that are not finite, and of launches that the sizes
+of the other tests do not reach.  u = 2^-24 is the largest relative error of one FP32 rounding."""
+import pytest
+import torch
+
+from oracle import layer as ref
+from test_gpu_layer import TYPES, U, check_forward, depth, gen, within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def b2(cuda):
+    import hpcdeepneuralnetworks_b200 as b2
+    return b2
+
+
+CONSTANTS = [0.1, 1.0 / 3.0, 6.6125484e7, -1e9, 6.734e8, 8.5e9, -3e15]
+
+
+@pytest.mark.parametrize("cols", [1000, 1027, 2000, 4095, 14336, 16390, 33000, 200003])
+@pytest.mark.parametrize("rows", [7, 601])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_layernorm_constant_rows_of_any_value(b2, rows, cols, kind):
+    """All elements equal some c whose sums are not exact.  A first mean is off by at most D*u*|c|, the mean of the equal distances
+    from it is right to D*u, so together they are off by (D*u)^2*|c|, less than half a step of c while D^2*u < 1 (D = 829 at 200003
+    columns): the second mean is c itself, every distance 0, rstd 1/sqrt(eps) but for its rounding, y beta."""
+    if cols > 40000 and rows > 7:
+        pytest.skip("the longest rows are taken a few at a time")
+    dtype = TYPES[kind]
+    values = torch.tensor(CONSTANTS if kind != "f16" else [0.1, 1.0 / 3.0, 4097.0, -65504.0, 1.1e-5, 777.7, 6e4]).to(dtype)
+    assert depth(cols) ** 2 * U < 1
+    c = values[torch.arange(rows) % 7]
+    x = c[:, None].expand(rows, cols).contiguous()
+    beta = torch.linspace(-1, 1, cols).to(dtype)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    y = b2.layernorm(rows, cols, 1e-5, x.cuda(), None, beta.cuda(), mean=mean, rstd=rstd).cpu()
+    assert torch.equal(mean.cpu(), c.float())
+    within(rstd, torch.full((rows,), float(torch.tensor(1e-5)) ** -0.5, dtype=torch.float64), 4 * U * 1e-5 ** -0.5, "rstd")
+    assert torch.equal(y, beta.expand(rows, cols))
+
+
+@pytest.mark.parametrize("cols", [1000, 1027, 2000, 4096, 14336, 33000])
+@pytest.mark.parametrize("rows", [6, 602])
+def test_layernorm_of_rows_a_few_steps_around_a_large_mean(b2, rows, cols):
+    """Values a few FP32 steps around -1e9 and around 6.7e8: what the first mean is off by is larger than the distances themselves."""
+    g = gen(cols + rows)
+    step = torch.tensor([64.0, 64.0])[torch.arange(rows) % 2]
+    base = torch.tensor([-1e9, 6.734e8])[torch.arange(rows) % 2]
+    x = base[:, None] + step[:, None] * torch.randint(-2, 3, (rows, cols), generator=g)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
+    y = b2.layernorm(rows, cols, 1e-5, x.cuda(), None, None, mean=mean, rstd=rstd)
+    check_forward(x, None, None, 1e-5, y, mean, rstd, cols)
