@@ -412,16 +412,17 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
     }
     if constexpr (PHASED) phase.clear_front(v[0]);
     F f[N * K], s(0.f);
+    const F part(inv);      // each term is divided: sums of values near the type's largest stay within FP32
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (ALL || i < valid) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           f[i * K + k] = v[i].get(k);
-          s = s + f[i * K + k];
+          s = ln_fma(f[i * K + k], part, s);
         }
       }
-    float m = ln_sum(s.sum(), scratch[0], t) * inv;
+    float m = ln_sum(s.sum(), scratch[0], t);
     F d1(0.f), d2(0.f);
     if constexpr (ALL && !FULL) {
       if (valid < N || (PHASED && phase.edge)) {      // what is outside the row lies at the mean
@@ -445,12 +446,12 @@ __global__ void __launch_bounds__(THREADS) layernorm_kernel(int64_t rows, int co
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const F e = f[i * K + k] + less;
-          d1 = d1 + e;
+          d1 = ln_fma(e, part, d1);
           d2 = ln_fma(e, e, d2);
         }
       }
     const float2 d = ln_sum2(make_float2(d1.sum(), d2.sum()), scratch[1], t);
-    const float off = d.x * inv;
+    const float off = d.x;
     m += off;
     const float r = rsqrtf(ln_variance(off, d.y * inv, noise) + eps);
     if (t.tid == 0) {
@@ -497,21 +498,21 @@ __global__ void __launch_bounds__(1024) layernorm_long_kernel(int64_t rows, int 
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
       v.load(xr + i);
 #pragma unroll
-      for (int k = 0; k < K; ++k) s = s + v.get(k);
+      for (int k = 0; k < K; ++k) s = ln_fma(v.get(k), F(inv), s);
     }
-    float m = ln_sum(s.sum(), scratch[0], t) * inv;
+    float m = ln_sum(s.sum(), scratch[0], t);
     F d1(0.f), d2(0.f);
     for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += 1024 * V) {
       v.load(xr + i);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const F e = v.get(k) + F(-m);
-        d1 = d1 + e;
+        d1 = ln_fma(e, F(inv), d1);
         d2 = ln_fma(e, e, d2);
       }
     }
     const float2 d = ln_sum2(make_float2(d1.sum(), d2.sum()), scratch[1], t);
-    const float off = d.x * inv;
+    const float off = d.x;
     m += off;
     const float r = rsqrtf(ln_variance(off, d.y * inv, noise) + eps);
     if (threadIdx.x == 0) {

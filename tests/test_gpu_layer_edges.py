@@ -51,3 +51,29 @@ def test_layernorm_of_rows_a_few_steps_around_a_large_mean(b2, rows, cols):
     mean, rstd = torch.zeros(rows, device="cuda"), torch.zeros(rows, device="cuda")
     y = b2.layernorm(rows, cols, 1e-5, x.cuda(), None, None, mean=mean, rstd=rstd)
     check_forward(x, None, None, 1e-5, y, mean, rstd, cols)
+
+
+@pytest.mark.parametrize("cols", [3, 1000, 1027, 4096, 14336, 33000])
+@pytest.mark.parametrize("rows", [5, 600])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_layernorm_of_rows_near_the_largest_values(b2, rows, cols, kind):
+    """Rows of a type's lowest value, as masks leave them, alone or beside ordinary elements: sums stay within FP32.  Constant rows
+    keep their value as the mean (as above) and give beta; in the others the squares of the distances pass FP32, so that rstd is 0
+    and the outputs are beta too.  The mean is right within D*u of the mean magnitude."""
+    dtype = TYPES[kind]
+    low = float(torch.finfo(torch.bfloat16).min)
+    x = torch.randn(rows, cols, generator=gen(rows + cols))
+    at = torch.arange(rows) % 5
+    x[at == 0] = low
+    x[at == 1, cols // 2:] = -8e37
+    x[at == 2, ::3] = 8e37
+    x[at == 3] = 2.0 ** 126
+    x = x.to(dtype)
+    beta = torch.linspace(-1, 1, cols).to(dtype)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.full((rows,), -1.0, device="cuda")
+    y = b2.layernorm(rows, cols, 1e-5, x.cuda(), None, beta.cuda(), mean=mean, rstd=rstd).cpu()
+    wide = x.double()
+    within(mean, wide.mean(1), (depth(cols) + 4) * U * wide.abs().mean(1) + 2.0 ** -140, "mean")
+    assert torch.equal(mean.cpu()[at == 0], x[at == 0, 0].float()) and torch.equal(mean.cpu()[at == 3], x[at == 3, 0].float())
+    assert torch.equal(y[at != 4], beta.expand(int((at != 4).sum()), cols))
+    assert bool(torch.isfinite(rstd).all()) and float(rstd[(at == 1).cuda()].abs().max()) == 0 == float(rstd[(at == 2).cuda()].abs().max())
