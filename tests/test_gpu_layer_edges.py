@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import layer as ref
-from test_gpu_layer import TYPES, U, check_forward, depth, gen, within
+from test_gpu_layer import TYPES, U, check_backward, check_forward, depth, gen, norm_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,23 @@ def test_layernorm_of_rows_near_the_largest_values(b2, rows, cols, kind):
     assert torch.equal(mean.cpu()[at == 0], x[at == 0, 0].float()) and torch.equal(mean.cpu()[at == 3], x[at == 3, 0].float())
     assert torch.equal(y[at != 4], beta.expand(int((at != 4).sum()), cols))
     assert bool(torch.isfinite(rstd).all()) and float(rstd[(at == 1).cuda()].abs().max()) == 0 == float(rstd[(at == 2).cuda()].abs().max())
+
+
+@pytest.mark.parametrize("cols", [64, 1000, 1027, 4096, 9000])
+@pytest.mark.parametrize("rows", [4, 700])
+def test_layernorm_backward_of_very_small_and_very_large_rows(b2, rows, cols):
+    """Rows of spread 1e-18 with rstd 1e18 .. 1e20, whose square passes FP32, and rows whose elements lie so far apart that the
+    forward pass gave rstd 0: dx is finite, 0 for the latter, and within the bound of every other row."""
+    x, gamma, _, dy = norm_inputs(rows, cols, torch.float32, torch.float32, cols + rows)
+    at = torch.arange(rows) % 4
+    x[at == 1] *= 1e-20
+    x[at == 2] *= 1e-18
+    x[at == 3, ::2] = 1e38
+    wide = x.double()
+    mean = wide.mean(1).float()
+    rstd = ((wide - mean.double()[:, None]) ** 2).mean(1).rsqrt().float()
+    rstd[at == 3] = 0.0
+    dx, dg, db = torch.full((rows, cols), 7.0, device="cuda"), torch.zeros(cols, device="cuda"), torch.zeros(cols, device="cuda")
+    b2.layernorm_backward(rows, cols, dy.cuda(), x.cuda(), gamma.cuda(), mean.cuda(), rstd.cuda(), dx, dg, db)
+    assert float(rstd.max()) > 1.9e19 and bool((dx[(at == 3).cuda()] == 0).all())
+    check_backward(dy, x, gamma, mean, rstd, dx, dg, db)
