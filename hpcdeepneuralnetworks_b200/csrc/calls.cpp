@@ -196,13 +196,13 @@ PyObject *layernorm_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::Tensor *ws = c.vector(0);
     c.place(h);
     at::Tensor own;
-    if (!ws) {
+    if (!ws && (dgamma || dbeta)) {
       own = scratch(x, lib.layernorm_backward_workspace_bytes(rows, cols));
       ws = &own;
     }
     return without_gil([&] {
       return lib.layernorm_backward(c.handle, rows, cols, type, dy.data_ptr(), cols, x.data_ptr(), cols, code < 0 ? type : code, gamma, mean,
-                                    rstd, dx, cols, dgamma, dbeta, ws->data_ptr(), ws->nbytes(), c.stream);
+                                    rstd, dx, cols, dgamma, dbeta, ws ? ws->data_ptr() : nullptr, ws ? ws->nbytes() : 0, c.stream);
     });
   });
 }

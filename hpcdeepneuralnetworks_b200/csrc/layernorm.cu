@@ -715,10 +715,12 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
 // times what one reading would take (158 us with 1024 threads to a row and a line of sums for every 28 rows).  Going over the rows
 // by panels that fit L2, both kernels for each, was slower: 191 us for panels of 48 MB, 164 for 80 MB; the kernels' ends cost more
 // than the second reading.
+// dx alone needs no second kernel and no place for the sums: the block that has a row's sums reads the row again (from L2).
 constexpr int kLnSumThreads = 512;
 template <class T, class P, int V>
 __global__ void __launch_bounds__(kLnSumThreads) layernorm_row_sums_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x, int64_t ldx,
-                                                                  const P *gamma, const float *mean, const float *rstd, float2 *out) {
+                                                                  const P *gamma, const float *mean, const float *rstd, float2 *out, T *dx,
+                                                                  int64_t lddx) {
   using F = typename LnPack<T, V>::F;
   constexpr int K = LnPack<T, V>::kParts;
   __shared__ LnScratch scratch[2];
@@ -742,7 +744,24 @@ __global__ void __launch_bounds__(kLnSumThreads) layernorm_row_sums_kernel(int64
       }
     }
     const float2 s = ln_sum2(make_float2(s1.sum(), s2.sum()), scratch[turn], t);
-    if (threadIdx.x == 0) out[row] = make_float2(s.x / (float)cols, s.y / (float)cols);
+    const float2 by_n = make_float2(s.x / (float)cols, s.y / (float)cols);
+    if (!dx) {
+      if (threadIdx.x == 0) out[row] = by_n;
+      continue;
+    }
+    for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += kLnSumThreads * V) {      // (dx may be dy: each thread reads its own again)
+      LnPack<T, V> xv, gv;
+      F g[K];
+      xv.load(x + row * ldx + i);
+      gv.load(dy + row * lddy + i);
+      ln_params<P, V>(g, gamma, (int)i, 1.f);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const F h = (xv.get(k) + F(-m)) * F(r);
+        xv.set(k, F(r) * (gv.get(k) * g[k] + ln_fma(h, F(-by_n.y), F(-by_n.x))));
+      }
+      xv.store(dx + row * lddx + i);
+    }
   }
 }
 template <class T, class P, int V>
@@ -1016,7 +1035,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
   B2_REQUIRE((((uintptr_t)gamma | (uintptr_t)dgamma | (uintptr_t)dbeta) & (pb - 1)) == 0, B2_ERR_INVALID_ARG,
              "b2_layernorm_backward: gamma, dgamma or dbeta is not aligned to its element type");
   const bool is_long = cols > kLnLongestBackward;
-  const size_t need = sums || is_long ? b2_layernorm_backward_workspace_bytes(rows, cols) : 0;
+  const size_t need = sums ? b2_layernorm_backward_workspace_bytes(rows, cols) : 0;
   B2_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need), B2_ERR_WORKSPACE,
              "b2_layernorm_backward: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
   B2_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, B2_ERR_INVALID_ARG, "b2_layernorm_backward: workspace is not 16-byte aligned");
@@ -1032,7 +1051,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
   const bool phased = width * tb < 16 && cols + 16 <= kLnLongestBackward && ln_phased({dy, x, dx}, {lddy * tb, ldx * tb, dx ? lddx * tb : ldx * tb});
   if (phased) width = 16 / tb;
   float *partial = sums ? (float *)workspace : nullptr;
-  float2 *row_sums = is_long ? (float2 *)((char *)workspace + (need - (size_t)rows * sizeof(float2))) : nullptr;
+  float2 *row_sums = is_long && sums ? (float2 *)((char *)workspace + (need - (size_t)rows * sizeof(float2))) : nullptr;
   auto launch = [&](auto t, auto p) -> int {
     using T = decltype(t);
     using P = decltype(p);
@@ -1088,8 +1107,8 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
       } else {
         if (dx)
           launched = launch_kernel(layernorm_row_sums_kernel<T, P, V>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows,
-                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums);
-        if (launched == cudaSuccess)
+                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, sums ? (T *)nullptr : (T *)dx, lddx);
+        if (sums && launched == cudaSuccess)
           launched = launch_kernel(layernorm_columns_kernel<T, P, V>, dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s, rows,
                                    (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
       }

@@ -188,7 +188,7 @@ def layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, dx, dgamma, dbeta, 
     ws, ws_bytes = None, 0
     if workspace is not None:
         ws, ws_bytes = _vector(workspace, 0, "workspace", device), workspace.numel() * workspace.element_size()
-    elif rows > 0:
+    elif rows > 0 and (dgamma is not None or dbeta is not None):
         ws_bytes = _layernorm_workspace(rows, cols)
         workspace = x.new_empty(-(-ws_bytes // x.element_size()))
         ws = workspace.data_ptr()

@@ -147,3 +147,38 @@ def test_an_error_that_a_status_reports_is_not_left_behind(cuda):
     left = rt.cudaGetLastError()
     L.b2_timer_destroy(timer)
     assert left == 0 and b"CUDA error" in L.b2_last_error()
+
+
+@pytest.mark.parametrize("cols", [8, 8192, 8193, 9000, 100000])
+def test_dx_alone_needs_no_workspace(built_lib, cols):
+    """As the header says: the workspace may be NULL when neither dgamma nor dbeta is asked for.  Without a device the call gets as far
+    as looking for one; a workspace that it wanted would be refused before."""
+    if torch.cuda.is_available():
+        pytest.skip("there is a device, and these addresses mean nothing to it")
+    L = _lib.load()
+    at = lambda n: C.c_void_p(n << 30)  # noqa: E731
+    call = lambda dg, db, ws, nws: L.b2_layernorm_backward(None, 4, cols, 0, at(1), cols, at(2), cols, 0, at(3), at(4), at(5), at(6), cols, dg, db,  # noqa: E731,E501
+                                                           ws, nws, None)
+    need = L.b2_layernorm_backward_workspace_bytes(4, cols)
+    assert call(None, None, None, 0) == CUDA
+    for dg, db in ((at(7), None), (None, at(8)), (at(7), at(8))):
+        assert call(dg, db, None, 0) == -6 and call(dg, db, at(9), need - 1) == -6 and call(dg, db, at(9), need) == CUDA
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(4, 9000), (300, 8200), (5, 100001), (3, 4096)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_dx_alone_without_a_workspace_equals_dx_beside_the_sums(cuda, rows, cols, inplace):
+    import hpcdeepneuralnetworks_b200 as b2
+    h = b2.default_handle()
+    L = _lib.load()
+    x, dy, gamma = torch.randn(rows, cols, device="cuda"), torch.randn(rows, cols, device="cuda"), torch.rand(cols, device="cuda")
+    mean, rstd = x.mean(1), x.var(1).rsqrt()
+    want, dg, db = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(gamma)
+    b2.layernorm_backward(rows, cols, dy, x, gamma, mean, rstd, want, dg, db)
+    dx = dy if inplace else torch.full_like(x, 7.0)
+    p = [C.c_void_p(t.data_ptr()) for t in (dy, x, gamma, mean, rstd, dx)]
+    torch.cuda.synchronize()
+    assert L.b2_layernorm_backward(h.raw, rows, cols, 0, p[0], cols, p[1], cols, 0, *p[2:], cols, None, None, None, 0, None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(dx, want)
