@@ -453,24 +453,22 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 
 // ---- matrix-vector product -----------------------------------------------------------------------
 // y = alpha * x * W^T + beta * y.  The codes are read once and should decide the time; what stands in the way is unpacking
-// them, so the arithmetic is arranged to need five instructions for eight codes.  It runs on mma.sync m16n8k16 (16 weight rows x
+// them, so the arithmetic is arranged to need nine instructions for eight codes.  It runs on mma.sync m16n8k16 (16 weight rows x
 // 8 columns of x), which has room for 8 columns at the price of one; a tcgen05 tile would want its operands written back to
 // shared memory in 16 bits first.
 //
-// Per group,  sum_k W x = s * (sum_k c x - z * sum_k x).  A code c in the lowest bits of a 16-bit half IS the FP16 number
-// c * 2^-24 (a subnormal; the tensor cores take those exactly), four bits higher it is 16 c * 2^-24, so a mask alone makes an
-// operand: words w and w >> 8 under 0x000f000f and 0x00f000f0 give the pairs of codes (0,4) (1,5) (2,6) (3,7), the odd pairs 16
-// times too large.  x takes part as FP16 too: a small kernel in front (w4_x_kernel) scales each row by a power of two that brings
-// its largest element to [2^14, 2^15), divides the odd elements by 16, and pairs them alike.  The scaled row is exact for every
-// element above 2^-28 of the largest (bf16 and FP16 in one term, FP32 in three terms of 11 bits, a column of the tile each), and
-// what lies below is off by 2^-39 of the largest at most: nothing beside the FP32 sums.  All products are exact in FP32; group
-// sums, scales and zero points are FP32.  The same kernel sums x over each group.
-// sum c x is larger than sum (c - z) x, and the tensor cores cut where they add: results in 16 bits do not show it, FP32 ones
-// would (2.6e-6 of the result's norm, against 5e-7 for a product of FP32 matrices).  So for FP32 x (EXACT) the zero point is
-// taken off while unpacking, in four more instructions per word: under 1024's upper bits a code reads 1024 + c, or 1024 + 16 c,
-// and a subtraction or an FMA with 1/16 leaves c - z exactly.
-// An infinity or NaN in x would make z * sum_k x meaningless: such elements count as 0 above and are added, with their exact
-// weights, by the thread that writes the output, which walks through its whole row for that.
+// Per group,  sum_k W x = s * sum_k (c - z) x.  The zero point is taken off while unpacking: taken off the sums it would leave, of an
+// element of x that meets weight 0, the rounding of z x, and that may be more than all the rest of the group.  Operands are of the
+// type that holds x exactly, and so are the differences c - z, whole numbers from -15 to 15.
+//   bf16 and FP32 x: a code in the lowest bits of a 16-bit half IS the bf16 number c * 2^-133, four bits higher it is 16 c * 2^-133
+//   (the first 256 bit patterns are the multiples of 2^-133); a mask and an FMA by 2^119 or 2^115 make (c - z) * 2^-14, exactly.  In
+//   that unit the largest bf16 and 128 of the largest weights stay within FP32, and the smallest are not lost below it.  FP32 x is
+//   cut into three bf16 terms of 8 bits, a column of the tile each: exact, but for what lies below 2^-135.
+//   FP16 x: under 1024's upper bits a code reads 1024 + c, or 1024 + 16 c, and a subtraction or an FMA with 1/16 leaves c - z.
+// Words w and w >> 8 give the pairs of codes (0,4) (1,5) (2,6) (3,7), and a small kernel in front (w4_x_kernel) pairs x alike.  All
+// products are exact in FP32; group sums are FP32, scaled and added in FP32.
+// An infinity or NaN in x counts as 0 above and is added, with its exact
+// weight, by the thread that writes the output, which walks through its whole row for that.
 //
 // A CTA streams tiles of 128 rows x 256 k (16 KB of codes and x of those k) through a ring of shared-memory stages.  Four
 // producer warps fill it: one thread issues the TMA loads (codes with the 128-byte swizzle: the 16-byte unit u of row r lies at
@@ -492,7 +490,7 @@ template <int NB, bool RESIDENT, bool ALIGNED>
 struct MvTile {
   // rows of codes that start anywhere are held from the 16-byte boundary in front of them on, 9 units of 16 bytes
   static constexpr int kRowPitch = ALIGNED ? kMvRowBytes : kMvRowBytes + 16, kCodeBytes = kMvRows * kRowPitch;
-  static constexpr int kXBytes = NB * (kMvChunk * 8 * 2 + 256);     // x of one chunk: fragments, then sums [part of a group][8 NB]
+  static constexpr int kXBytes = NB * kMvChunk * 8 * 2;            // x of one chunk
   static constexpr int kStage = RESIDENT ? kCodeBytes : (kCodeBytes + kXBytes + 1023) / 1024 * 1024;
   static constexpr int kSumBytes = 2 * 8 * NB * kMvPitch * 4;
   static constexpr int kCtasPerSm = NB <= 2 ? 2 : 1;
@@ -507,13 +505,13 @@ static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
 // memory.  That saves a kernel and a workspace, and costs the same work in every row block's CTAs.
 // (1 token, device time and the host's share of a call: 4096^2, 512 units, 8.4 us and 9 against 7.4 and 14 through w4_x_kernel;
 // 8192^2, 2048 units, 18 against 14 us on the device.)
-constexpr int kMvResidentBytes = 35 * 1024;
+constexpr int kMvResidentBytes = 32 * 1024;
 constexpr int64_t kMvResidentWork = 600;       // row blocks x chunks (16 KB of codes each)
 static bool mv_resident(int64_t M, int64_t N, int64_t K, int type) {
   const int nb = mv_blocks(M, type);
   const int64_t chunks = (K + kMvChunk - 1) / kMvChunk, per_cta = (chunks + 7) / 8;
   const int64_t blocks = (N + kMvRows - 1) / kMvRows;
-  return nb == 1 && per_cta * (kMvChunk * 8 * 2 + 256) <= kMvResidentBytes && blocks * chunks <= kMvResidentWork;
+  return nb == 1 && per_cta * kMvChunk * 8 * 2 <= kMvResidentBytes && blocks * chunks <= kMvResidentWork;
 }
 
 struct MvArgs {
@@ -526,7 +524,7 @@ struct MvArgs {
   const void *scales;
   void *y;
   const unsigned char *image;      // [item's rows][chunk][kXBytes], unless the CTAs lay x out themselves
-  const int2 *row_info;            // of each row of x: the power of two it was scaled by, and whether it holds an infinity or NaN
+  const int *row_info;             // of each row of x: whether it holds an infinity or NaN
   int *status;
   unsigned int seq;
 };
@@ -549,99 +547,74 @@ __device__ __forceinline__ void mv_load_x(float (&v)[8], const T *row, int64_t k
   }
 }
 
-// The power of two that brings `largest` to [2^14, 2^15), as an exponent, and as two factors (it may pass FP32's range).
-__device__ __forceinline__ int mv_exponent(float largest) {
-  int q = 0;
-  if (largest > 0.f) frexpf(largest, &q), q = 15 - q;
-  return q;
-}
-// Looks at 8 elements: the largest finite magnitude, and whether one is not finite.
-__device__ __forceinline__ void mv_look(const float (&e)[8], float &top, bool &bad) {
+// Whether one of 8 elements is not finite.
+__device__ __forceinline__ bool mv_look(const float (&e)[8]) {
+  bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (isfinite(e[i])) top = fmaxf(top, fabsf(e[i]));
-    else bad = true;
-  }
+  for (int i = 0; i < 8; ++i) bad |= !isfinite(e[i]);
+  return bad;
 }
-// Lays one unit (8 elements, the `u`-th of its chunk, a lane per unit) of columns col0.. out in a chunk's image: scaled by
-// f1 * f2, cut into `parts` FP16 terms, paired, and summed over parts of groups (1 << part_log elements: a group, or the 128 of
-// a longer one that a warp multiplies).
-__device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8], int u, int nb, int col0, int parts, int part_log, float f1,
-                                       float f2) {
-  const bool exact = parts > 1;              // FP32: no division of the odd elements, no sums
+// Lays one unit (8 elements, the `u`-th of its chunk) of columns col0.. out in a chunk's image: as FP16, or in `parts` bf16 terms,
+// each the upper half of what the one before has left, and paired.
+template <bool BF16>
+__device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8], int u, int nb, int col0, int parts) {
   float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? (e[i] * f1) * f2 * ((i & 1) && !exact ? 0.0625f : 1.f) : 0.f;
+  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? e[i] : 0.f;
   for (int p = 0; p < parts; ++p) {
     const int col = col0 + p;
-    __half h[8];
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      h[i] = __float2half_rn(r[i]);
-      const float back = __half2float(h[i]);
-      sum += (i & 1) ? 16.f * back : back;
-      r[i] = (r[i] - back) * 2048.f;       // what the term left, 11 bits up, for the next
-    }
     union {
-      __half2 h2[4];
+      uint16_t h[8];
       uint4 q;
     } out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out.h2[i] = __halves2half2(h[i], h[i + 4]);
+    for (int i = 0; i < 8; ++i) {
+      const int at = 2 * (i & 3) + (i >> 2);      // pairs (0,4) (1,5) (2,6) (3,7)
+      if constexpr (BF16) {
+        const uint32_t top = __float_as_uint(r[i]) & 0xffff0000u;
+        out.h[at] = (uint16_t)(top >> 16);
+        r[i] -= __uint_as_float(top);
+      } else {
+        out.h[at] = __half_as_ushort(__float2half_rn(r[i]));      // (x is FP16)
+      }
+    }
     reinterpret_cast<uint4 *>(chunk)[(((u >> 2) * nb + (col >> 3)) * 8 + (col & 7)) * 4 + (u & 3)] = out.q;
-    if (exact) continue;
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1)
-      if (o < (1 << (part_log - 3))) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((u & ((1 << (part_log - 3)) - 1)) == 0)
-      reinterpret_cast<float *>(chunk + nb * (kMvChunk * 8 * 2))[(u >> (part_log - 3)) * 8 * nb + col] = sum * 0x1p-24f;
   }
 }
 
-// One block per row of x: its largest finite element, then its image.  Four units per thread are kept between the two passes; a
+// One block per row of x: whether an element is not finite, then its image.  Four units per thread are kept between the two passes; a
 // longer row is read again.
 template <class T>
 __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ldx, int vec, const T *x, int chunks, int nb, int rows_per_item,
-                                                           int part_log, unsigned char *image, int2 *row_info) {
+                                                           unsigned char *image, int *row_info) {
   constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kKept = 4;
-  __shared__ float largest[kMvXThreads / 32];
-  __shared__ int odd[kMvXThreads / 32];
   pdl_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x;
   const int m = blockIdx.x, item = m / rows_per_item, col0 = (m - item * rows_per_item) * kParts;
   const T *row = x + m * ldx;
   const int units = chunks * (kMvChunk / 8);
   float v[kKept][8];
-  float top = 0.f;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
     if (tid + i * kMvXThreads < units) mv_load_x<T>(v[i], row, 8 * (int64_t)(tid + i * kMvXThreads), K, vec != 0);
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) mv_look(v[i], top, bad);
+    if (tid + i * kMvXThreads < units) bad |= mv_look(v[i]);
   for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
     float e[8];
     mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
-    mv_look(e, top, bad);
+    bad |= mv_look(e);
   }
-  top = w4_warp_max(top);
-  const bool any = __any_sync(0xffffffffu, bad);
-  if (lane == 0) largest[tid >> 5] = top, odd[tid >> 5] = any;
-  __syncthreads();
-  top = w4_warp_max(lane < kMvXThreads / 32 ? largest[lane] : 0.f);
-  bad = __any_sync(0xffffffffu, lane < kMvXThreads / 32 && odd[lane]);
-  const int q = mv_exponent(top);
-  if (tid == 0) row_info[m] = make_int2(q, bad);
-  const float f1 = ldexpf(1.f, q / 2), f2 = ldexpf(1.f, q - q / 2);
-  const int chunk_bytes = nb * (kMvChunk * 8 * 2 + 256);
+  bad = __syncthreads_or(bad);
+  if (tid == 0) row_info[m] = bad;
+  const int chunk_bytes = nb * (kMvChunk * 8 * 2);
   auto put = [&](const float (&e)[8], int u) {
-    mv_put(image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes, e, u & 31, nb, col0, kParts, part_log, f1, f2);
+    mv_put<!std::is_same<T, __half>::value>(image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes, e, u & 31, nb, col0, kParts);
   };
 #pragma unroll
   for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) put(v[i], tid + i * kMvXThreads);     // whole warps: units is a multiple of 32
+    if (tid + i * kMvXThreads < units) put(v[i], tid + i * kMvXThreads);
   for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
     float e[8];
     mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
@@ -655,29 +628,46 @@ __device__ __forceinline__ uint32_t mv_and_or(uint32_t w, uint32_t mask, uint32_
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
   return r;
 }
+// d = a * b + (FIRST: 0, else d)
+template <bool BF16, bool FIRST>
 __device__ __forceinline__ void mv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  if constexpr (FIRST) d[0] = d[1] = d[2] = d[3] = 0.f;
+  if constexpr (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// c - z of a word's codes 0 and 4 (even: in the lowest bits of its halves), or 1 and 5 (odd: four bits up), from 1024 + z.
+// What a group's zero point is held as, twice in 16 bits: what mv_even adds or takes off.
+constexpr float kMvUnit = 0x1p-14f;      // of bf16 weights
+template <bool BF16>
+__device__ __forceinline__ uint32_t mv_zero(uint32_t z) {
+  return BF16 ? (__float_as_uint(-(float)z * kMvUnit) >> 16) * 0x00010001u : 0x64006400u + z * 0x00010001u;
+}
+__device__ __forceinline__ uint32_t mv_fma_bf16(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// c - z of a word's codes 0 and 4 (even: in the lowest bits of its halves), or 1 and 5 (odd: four bits up).
+template <bool BF16>
 __device__ __forceinline__ uint32_t mv_even(uint32_t w, uint32_t zero) {
+  if constexpr (BF16) return mv_fma_bf16(w & 0x000f000fu, 0x7b007b00u, zero);      // 2^119
   const uint32_t v = mv_and_or(w, 0x000f000fu, 0x64006400u);
   const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&zero));
   return *reinterpret_cast<const uint32_t *>(&r);
 }
+template <bool BF16>
 __device__ __forceinline__ uint32_t mv_odd(uint32_t w, uint32_t zero) {
+  if constexpr (BF16) return mv_fma_bf16(w & 0x00f000f0u, 0x79007900u, zero);      // 2^115
   const uint32_t v = mv_and_or(w, 0x00f000f0u, 0x64006400u);
   const __half2 less = __hsub2(__float2half2_rn(960.f), *reinterpret_cast<const __half2 *>(&zero));      // -(64 + z)
   const __half2 r = __hfma2(*reinterpret_cast<const __half2 *>(&v), __float2half2_rn(0.0625f), less);
   return *reinterpret_cast<const uint32_t *>(&r);
-}
-
-__device__ __forceinline__ void mv_mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // d = a * b
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // A tensor map of `rows` rows of `cols` bytes, `pitch` bytes apart, in boxes of 128 bytes x box_rows.
@@ -730,11 +720,6 @@ __device__ __forceinline__ uint32_t ld_shared_32(uint32_t a) {
 __device__ __forceinline__ uint4 ld_shared_128(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float2 ld_shared_f32x2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
   return v;
 }
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) { return __uint_as_float(ld_shared_cluster_u32(cluster_addr)); }
@@ -801,7 +786,8 @@ __device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, i
 // ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
 // RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
 // BLOCKS: blocks of 32 k in a group, or in the 128 of a longer one that a warp multiplies.
-template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
+// BF16: operands in bf16 (for bf16 and FP32 x), else in FP16.
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool BF16>
 __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCtasPerSm)
     w4_matvec_kernel(const __grid_constant__ MvArgs a, const __grid_constant__ CUtensorMap code_map) {
   using Tile = MvTile<NB, RESIDENT, ALIGNED>;
@@ -813,13 +799,13 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
   int chunks = a.chunks - first;
   chunks = chunks < 0 ? 0 : chunks < a.chunks_per_cta ? chunks : a.chunks_per_cta;
   const int window_log = a.group_shift - 5;                                // chunks of a window: group / 32
-  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, zero point (EXACT: 1024 + z, twice in FP16)
+  float2 *const windows = reinterpret_cast<float2 *>(smem + a.stages * Tile::kStage);    // [kMvWindows][row][8]: scale, mv_zero of the zero point
   unsigned char *const xs = reinterpret_cast<unsigned char *>(windows + kMvWindows * kMvWindow);   // RESIDENT: [chunk][kXBytes]
   float *const sums = reinterpret_cast<float *>(xs + (RESIDENT ? a.chunks_per_cta * Tile::kXBytes : 0));   // [2][8 NB][kMvPitch]
   uint64_t *const full = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sums) + Tile::kSumBytes);
   uint64_t *const empty = full + kMvMaxStages, *const wfull = empty + kMvMaxStages, *const wempty = wfull + kMvWindows;
   uint64_t *const ready = wempty + kMvWindows, *const done = ready + 1;
-  int *const largest = reinterpret_cast<int *>(done + 1), *const odd = largest + 16;      // RESIDENT: of each row of x (at most 16)
+  int *const odd = reinterpret_cast<int *>(done + 1);      // RESIDENT: whether a row of x (8 at most) holds an infinity or NaN
   constexpr int kFillers = kMvProducers - 32;     // threads that write shared memory themselves
 
   if (tid == 0) {
@@ -958,7 +944,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
             }
 #pragma unroll
             for (int i = 0; i < kTurns; ++i)
-              if ((i + 1) * kFillers <= kMvWindow || me + i * kFillers < kMvWindow) to[i * kFillers] = make_float2(__uint_as_float(scale[i]), EXACT ? __uint_as_float(0x64006400u + zero[i] * 0x00010001u) : (float)zero[i]);
+              if ((i + 1) * kFillers <= kMvWindow || me + i * kFillers < kMvWindow) to[i * kFillers] = make_float2(__uint_as_float(scale[i]), __uint_as_float(mv_zero<BF16>(zero[i])));
             mbar_arrive(&wfull[window.at]);
             window.next();
           }
@@ -981,36 +967,20 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
       for (int b4 = 0; b4 < 4; ++b4) place[b4] = (wn * 32 + g) * kMvRowBytes + (((wk * 4 + b4) ^ g) << 4) + 4 * t;
     }
     if constexpr (RESIDENT) {
-      // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8.  Each
-      // row is scaled by its largest element here; the sums are scaled back before they leave the CTA.
-      if (tid < 16) largest[tid] = 0, odd[tid] = 0;
+      // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8
+      if (tid < 8) odd[tid] = 0;
       mv_consumers_sync();
-      for (int pass = 0; pass < 2; ++pass) {
-        for (int at = warp; at < a.M * chunks; at += kMvConsumers / 32) {
-          const int m = at / chunks, c = at - m * chunks;
-          const int64_t k = (int64_t)(first + c) * kMvChunk + 8 * lane;
-          float e[8];
-          if (a.type == B2_F32) mv_load_x(e, (const float *)a.x + m * a.ldx, k, a.K, a.vec != 0);
-          else if (a.type == B2_BF16) mv_load_x(e, (const __nv_bfloat16 *)a.x + m * a.ldx, k, a.K, a.vec != 0);
-          else mv_load_x(e, (const __half *)a.x + m * a.ldx, k, a.K, a.vec != 0);
-          if (pass == 0) {
-            float top = 0.f;
-            bool bad = false;
-            mv_look(e, top, bad);
-            top = w4_warp_max(top);
-            bad = __any_sync(0xffffffffu, bad);
-            if (lane == 0) {
-              atomicMax(&largest[m], __float_as_int(top));      // not negative: ordered as integers
-              if (bad) atomicOr(&odd[m], 1);
-            }
-          } else {
-            const int q = mv_exponent(__int_as_float(largest[m]));
-            mv_put(xs + c * Tile::kXBytes, e, lane, NB, m * a.parts, a.parts, a.group_shift < 7 ? a.group_shift : 7, ldexpf(1.f, q / 2),
-                   ldexpf(1.f, q - q / 2));
-          }
-        }
-        mv_consumers_sync();
+      for (int at = warp; at < a.M * chunks; at += kMvConsumers / 32) {
+        const int m = at / chunks, c = at - m * chunks;
+        const int64_t k = (int64_t)(first + c) * kMvChunk + 8 * lane;
+        float e[8];
+        if (a.type == B2_F32) mv_load_x(e, (const float *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+        else if (a.type == B2_BF16) mv_load_x(e, (const __nv_bfloat16 *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+        else mv_load_x(e, (const __half *)a.x + m * a.ldx, k, a.K, a.vec != 0);
+        if (mv_look(e)) atomicOr(&odd[m], 1);
+        mv_put<BF16>(xs + c * Tile::kXBytes, e, lane, NB, m * a.parts, a.parts);
       }
+      mv_consumers_sync();
     }
     for (int item = blockIdx.x; item < a.items; item += gridDim.x, ++turn) {
       const int mc = item / a.row_blocks;
@@ -1024,7 +994,7 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
           off[r] = 8 * (skew & 3u);
         }
       }
-#pragma unroll (EXACT ? 1 : 2)
+#pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int in_window = c & ((1 << window_log) - 1);
         if (in_window == 0) wait(&wfull[window.at], window.phase);
@@ -1032,7 +1002,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
         const uint32_t stage = smem_base + ring.at * Tile::kStage;
         const uint32_t image = RESIDENT ? xs_base + c * Tile::kXBytes : stage + Tile::kCodeBytes;
         const uint32_t xf = image + (wk * 4 * NB * 32 + lane) * 16;
-        const uint32_t xsum = image + NB * (kMvChunk * 8 * 2) + t * 8 + wk * (4 / BLOCKS) * 8 * NB * 4;
         // this warp's first group of the window
         const uint32_t sz = windows_base + window.at * (kMvWindow * 8) + (((in_window * 8 + wk * 4) >> window_log) << 3);
         // the warp's 128 k in straight-line code
@@ -1040,9 +1009,9 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
 #pragma unroll
           for (int b0 = 0; b0 < 4; b0 += BLOCKS) {
             float acc[2][NB][4];
-            uint32_t zero[4];                                         // EXACT: of rows g + 8 r
+            uint32_t zero[4];                                         // of rows g + 8 r
 #pragma unroll
-            for (int r = 0; r < 4; ++r) zero[r] = EXACT ? ld_shared_32(sz + (b0 / BLOCKS) * 8 + r * 8 * 64 + 4) : 0;
+            for (int r = 0; r < 4; ++r) zero[r] = ld_shared_32(sz + (b0 / BLOCKS) * 8 + r * 8 * 64 + 4);
 #pragma unroll
             for (int b4 = b0; b4 < b0 + BLOCKS; ++b4) {
               uint4 xv[NB];
@@ -1060,42 +1029,30 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
                   w1 = __funnelshift_r(ld_shared_32(at1), ld_shared_32(at1 + 4), off[2 * rt + 1]);
                 }
                 const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-                uint32_t f[4], h[4];
-                if constexpr (EXACT) {
-                  const uint32_t z0 = zero[2 * rt], z1 = zero[2 * rt + 1];
-                  f[0] = mv_even(w0, z0), f[1] = mv_even(w1, z1), f[2] = mv_odd(w0, z0), f[3] = mv_odd(w1, z1);
-                  h[0] = mv_even(v0, z0), h[1] = mv_even(v1, z1), h[2] = mv_odd(v0, z0), h[3] = mv_odd(v1, z1);
-                } else {
-                  f[0] = w0 & 0x000f000fu, f[1] = w1 & 0x000f000fu, f[2] = w0 & 0x00f000f0u, f[3] = w1 & 0x00f000f0u;
-                  h[0] = v0 & 0x000f000fu, h[1] = v1 & 0x000f000fu, h[2] = v0 & 0x00f000f0u, h[3] = v1 & 0x00f000f0u;
-                }
+                const uint32_t z0 = zero[2 * rt], z1 = zero[2 * rt + 1];
+                const uint32_t f[4] = {mv_even<BF16>(w0, z0), mv_even<BF16>(w1, z1), mv_odd<BF16>(w0, z0), mv_odd<BF16>(w1, z1)};
+                const uint32_t h[4] = {mv_even<BF16>(v0, z0), mv_even<BF16>(v1, z1), mv_odd<BF16>(v0, z0), mv_odd<BF16>(v1, z1)};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                  if (b4 == b0) mv_mma_first(acc[rt][nb], f, xv[nb].x, xv[nb].y);
-                  else mv_mma(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                  if (b4 == b0) mv_mma<BF16, true>(acc[rt][nb], f, xv[nb].x, xv[nb].y);
+                  else mv_mma<BF16, false>(acc[rt][nb], f, xv[nb].x, xv[nb].y);
                 }
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mv_mma(acc[rt][nb], h, xv[nb].z, xv[nb].w);
+                for (int nb = 0; nb < NB; ++nb) mv_mma<BF16, false>(acc[rt][nb], h, xv[nb].z, xv[nb].w);
               }
             }
-            float2 group[4];                                          // scale and zero point of rows g + 8 r
+            float scale[4];                                           // of rows g + 8 r
 #pragma unroll
-            for (int r = 0; r < 4; ++r) group[r] = ld_shared_f32x2(sz + (b0 / BLOCKS) * 8 + r * 8 * 64);
+            for (int r = 0; r < 4; ++r) scale[r] = __uint_as_float(ld_shared_32(sz + (b0 / BLOCKS) * 8 + r * 8 * 64));
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              const float2 x2 = EXACT ? make_float2(0.f, 0.f) : ld_shared_f32x2(xsum + (b0 / BLOCKS) * 8 * NB * 4 + nb * 32);
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float2 v = group[r];
-                float(&tot)[4] = total[r >> 1][nb];
-                const float(&ac)[4] = acc[r >> 1][nb];
+              for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  const float sum = EXACT ? ac[2 * (r & 1) + i] : fmaf(-v.y, i ? x2.y : x2.x, ac[2 * (r & 1) + i]);
-                  tot[2 * (r & 1) + i] = fmaf(v.x, sum, tot[2 * (r & 1) + i]);
+                  float &to = total[r >> 1][nb][2 * (r & 1) + i];
+                  to = fmaf(scale[r], acc[r >> 1][nb][2 * (r & 1) + i], to);
                 }
-              }
-            }
           }
         }
         const bool window_ends = in_window == (1 << window_log) - 1 || c + 1 == chunks;
@@ -1116,16 +1073,11 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int col = nb * 8 + 2 * t + i, m = col / a.parts;
-          // RESIDENT: the codes' 2^-24, this CTA's scale of the row and the term's
-          const int up = RESIDENT && m < a.M ? (EXACT ? 0 : 24) - 11 * (col - m * a.parts) - mv_exponent(__int_as_float(largest[m])) : 0;
+          const int col = nb * 8 + 2 * t + i;
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float v = total[rt][nb][i + 2 * h];
-              sums[(wk * 8 * NB + col) * kMvPitch + wn * 32 + rt * 16 + g + h * 8] = RESIDENT ? ldexpf(v, up) : v;
-            }
+            for (int h = 0; h < 2; ++h) sums[(wk * 8 * NB + col) * kMvPitch + wn * 32 + rt * 16 + g + h * 8] = total[rt][nb][i + 2 * h];
         }
       mv_consumers_sync();
       if constexpr (RESIDENT) {
@@ -1152,7 +1104,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
         if (n0 + r >= a.N) continue;
         float v = 0.f;
         if (a.chunks > 0) {
-          const int2 info = RESIDENT ? make_int2(0, 0) : a.row_info[m0 + m];
           for (int p = 0; p < a.parts; ++p) {
             const float *at = sums + (m * a.parts + p) * kMvPitch + r;
             float s = 0.f;
@@ -1164,9 +1115,10 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
             } else {
               s = at[0] + at[8 * NB * kMvPitch];
             }
-            v += RESIDENT ? s : ldexpf(s, (EXACT ? 0 : 24) - 11 * p - info.x);    // the codes' 2^-24, the row's scale and the term's
+            v += s;
           }
-          if (info.y) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
+          if constexpr (BF16) v *= 1.f / kMvUnit;
+          if (!RESIDENT && a.row_info[m0 + m]) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
           v *= a.alpha;
         }
         const int64_t to = (int64_t)(m0 + m) * a.ldy + n0 + r;
@@ -1219,10 +1171,10 @@ static int mv_clusters(const void *kernel, int device, int ctas, int smem, int *
   return B2_OK;
 }
 
-template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool EXACT>
+template <int NB, bool ALIGNED, bool RESIDENT, int BLOCKS, bool BF16>
 static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   using Tile = MvTile<NB, RESIDENT, ALIGNED>;
-  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS, EXACT>;
+  const auto kernel = w4_matvec_kernel<NB, ALIGNED, RESIDENT, BLOCKS, BF16>;
   const int st = ensure_func_attributes((const void *)kernel, ctx->device, Tile::kSmem);
   if (st != B2_OK) return st;
   const int64_t row_blocks = (a.N + kMvRows - 1) / kMvRows;
@@ -1275,15 +1227,15 @@ static int w4_matvec_launch(Context *ctx, MvArgs a, cudaStream_t s) {
   return B2_OK;
 }
 
-template <int NB, bool RESIDENT, bool ALIGNED, bool EXACT>
+template <int NB, bool RESIDENT, bool ALIGNED, bool BF16>
 static int w4_matvec_groups(Context *ctx, const MvArgs &a, cudaStream_t s) {
-  return a.group_shift == 5   ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 1, EXACT>(ctx, a, s)
-         : a.group_shift == 6 ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 2, EXACT>(ctx, a, s)
-                              : w4_matvec_launch<NB, ALIGNED, RESIDENT, 4, EXACT>(ctx, a, s);
+  return a.group_shift == 5   ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 1, BF16>(ctx, a, s)
+         : a.group_shift == 6 ? w4_matvec_launch<NB, ALIGNED, RESIDENT, 2, BF16>(ctx, a, s)
+                              : w4_matvec_launch<NB, ALIGNED, RESIDENT, 4, BF16>(ctx, a, s);
 }
 template <int NB, bool RESIDENT>
 static int w4_matvec_forms(Context *ctx, const MvArgs &a, bool aligned, cudaStream_t s) {
-  if (a.parts > 1) return aligned ? w4_matvec_groups<NB, RESIDENT, true, true>(ctx, a, s) : w4_matvec_groups<NB, RESIDENT, false, true>(ctx, a, s);
+  if (a.type != B2_F16) return aligned ? w4_matvec_groups<NB, RESIDENT, true, true>(ctx, a, s) : w4_matvec_groups<NB, RESIDENT, false, true>(ctx, a, s);
   return aligned ? w4_matvec_groups<NB, RESIDENT, true, false>(ctx, a, s) : w4_matvec_groups<NB, RESIDENT, false, false>(ctx, a, s);
 }
 static int w4_matvec_run(Context *ctx, const MvArgs &a, int nb, bool resident, bool aligned, cudaStream_t s) {
@@ -1297,7 +1249,7 @@ static int w4_matvec_run(Context *ctx, const MvArgs &a, int nb, bool resident, b
 static size_t mv_image_bytes(int64_t M, int64_t K, int type) {
   const int nb = mv_blocks(M, type);
   const int64_t items = (M + mv_rows(nb, type) - 1) / mv_rows(nb, type);
-  return (size_t)(items * ((K + kMvChunk - 1) / kMvChunk)) * nb * (kMvChunk * 8 * 2 + 256);
+  return (size_t)(items * ((K + kMvChunk - 1) / kMvChunk)) * nb * (kMvChunk * 8 * 2);
 }
 
 // The checks that the three calls share: sizes, types, the codes' rows.
@@ -1419,7 +1371,7 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t N, int64_t K, int type) {
   if (M <= 0 || M > kW4MaxRows || N <= 0 || K <= 0 || N > INT32_MAX || K > kW4MaxK || type_bytes(type) == 0) return 0;
   if (mv_resident(M, N, K, type)) return 0;
-  return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int2);
+  return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int);
 }
 
 int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
@@ -1457,13 +1409,13 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   const bool resident = mv_resident(M, N, K, type);
   if (a.chunks > 0 && !resident) {
     unsigned char *image = (unsigned char *)workspace;
-    int2 *info = (int2 *)(image + mv_image_bytes(M, K, type));
+    int *info = (int *)(image + mv_image_bytes(M, K, type));
     a.image = image, a.row_info = info;
     cudaError_t launched = cudaSuccess;
     with_type(type, [&](auto t) {
       using T = decltype(t);
       launched = launch_kernel(w4_x_kernel<T>, (unsigned)M, kMvXThreads, 0, s, K, ldx, a.vec, (const T *)x, a.chunks, nb, a.rows_per_item,
-                               a.group_shift < 7 ? a.group_shift : 7, image, info);
+                               image, info);
       return 0;
     });
     B2_CUDA(launched);

@@ -269,8 +269,9 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
  * decoding steps, bound by reading the codes.  beta == 0 means y is not read, alpha == 0 means x and W are not.  More than 64
  * rows return B2_ERR_UNSUPPORTED: expand the weights once (b2_w4_dequantize) and use b2_sgemm; so does K above 2^27.  y must not
  * overlap x.
- * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.  They are formed from rows of x
- * scaled to 2^15 by a power of two, so scales of a magnitude outside 2^-110 .. 2^90 may lose digits or overflow on the way.
+ * Sums are FP32 in a fixed order for given sizes and alignments: results repeat bit for bit.  They are those of x times the whole
+ * numbers (code - zero) of a group, times its scale, so an element that meets weight 0 takes no part.  Bf16 and FP32 products are
+ * formed at 2^-14 of their size: results below 2^-110, and elements of FP32 x below 2^-110, may lose digits.
  * `workspace`: 16-byte aligned, b2_w4_matvec_workspace_bytes(M, N, K, type) bytes that no other call uses meanwhile, where x is
  * laid out for the tensor cores first; 0 (NULL will do) for smaller products, whose kernel lays it out itself.  A bounded wait
  * that runs out on the device is left for b2_check_status as for the SGEMM. */

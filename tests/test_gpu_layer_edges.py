@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oracle import layer as ref
-from test_gpu_layer import TYPES, U, check_backward, check_forward, depth, gen, norm_inputs, within
+from test_gpu_layer import TYPES, U, check_backward, check_forward, depth, gen, held, norm_inputs, within
 
 pytestmark = pytest.mark.gpu
 
@@ -97,3 +97,72 @@ def test_layernorm_backward_of_very_small_and_very_large_rows(b2, rows, cols):
     b2.layernorm_backward(rows, cols, dy.cuda(), x.cuda(), gamma.cuda(), mean.cuda(), rstd.cuda(), dx, dg, db)
     assert float(rstd.max()) > 1.9e19 and bool((dx[(at == 3).cuda()] == 0).all())
     check_backward(dy, x, gamma, mean, rstd, dx, dg, db)
+
+
+# ---- products with 4-bit weights --------------------------------------------------------------------
+def product_bound(x, w, want, dtype, K):
+    """The product of exact weights: FP32 sums of exact products x (c - z), in chains of at most 64 + K/16 additions of two roundings'
+    worth each (the tensor cores cut), scaled and added in FP32, rounded once.  Only what has a weight counts: no term for the zero
+    point."""
+    size = x.double().abs() @ w.abs().t()
+    return ref.half_step(dtype) * want.abs() + 2 * U * (64 + K / 16) * size + 4 * U * want.abs() + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 12, 20, 64])
+@pytest.mark.parametrize("N,K", [(70, 4096), (33, 1000), (40, 16640), (17, 515)])
+@pytest.mark.parametrize("group,kind,with_zeros", [(32, "bf16", True), (64, "f16", True), (128, "f16", False), (128, "bf16", False), (256, "bf16", True),
+                                                    (64, "f32", True)])
+def test_w4_matvec_where_a_large_element_meets_weight_zero(b2, M, N, K, group, kind, with_zeros):
+    """One element of a row, at an even or odd place, is up to 2^100 (FP16: 2^27, FP32: 2^30) times the others, and all its weights are
+    0: it takes no part in the result, and must not take the digits of what does."""
+    dtype = TYPES[kind]
+    codes, s, z, _ = held(N, K, group, torch.float32, with_zeros, N + K)
+    x = torch.randn(M, K, generator=gen(M + K))
+    large, small = {"bf16": (2.0 ** 60, 2.0 ** -40), "f16": (16384.0, 2.0 ** -13), "f32": (2.0 ** 20, 2.0 ** -10)}[kind]
+    x = (x * small).to(dtype)
+    for m in range(M):
+        k = (37 * m + 6 + m % 2) % K
+        x[m, k] = large
+        codes[:, k] = 8 if z is None else z[:, k // group]
+    w = ref.w4_values(codes, s, z, group)
+    want = x.double() @ w.t()
+    y = b2.w4_matvec(M, N, K, group, 1.0, x.cuda(), ref.w4_pack(codes).cuda(), s.cuda(), None if z is None else z.to(torch.uint8).cuda(), 0.0)
+    within(y, want, product_bound(x, w, want, dtype, K), "y")
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 16, 33, 64])
+@pytest.mark.parametrize("N,K", [(129, 1000), (1000, 515), (40, 4096), (24, 8200)])
+@pytest.mark.parametrize("group,kind,scales,with_zeros,pad", [(32, "bf16", "bf16", False, 0), (64, "f16", "f16", True, 0), (128, "f32", "f32", True, 0),
+                                                              (256, "bf16", "f32", True, 4112), (128, "f16", "bf16", False, 4101)])
+def test_w4_matvec_within_the_bound_of_its_weights(b2, M, N, K, group, kind, scales, with_zeros, pad):
+    dtype = TYPES[kind]
+    codes, s, z, dev = held(N, K, group, TYPES[scales], with_zeros, N * 3 + K, pad)
+    x = torch.randn(M, K, generator=gen(M * 41 + K)).to(dtype)
+    w = ref.w4_values(codes, s, z, group)
+    want = x.double() @ w.t()
+    within(b2.w4_matvec(M, N, K, group, 1.0, x.cuda(), *dev, 0.0), want, product_bound(x, w, want, dtype, K), "y")
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 40, 512), (20, 40, 512)])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_w4_matvec_carries_every_element_of_16_bits_exactly(b2, M, N, K, kind):
+    """Rows with one element of each size a type has, a step above a power of two, against weights that pick a single one: the result is
+    that element, whatever stands beside it."""
+    dtype, group = TYPES[kind], 32
+    g = torch.finfo(dtype)
+    codes = torch.full((N, K), 8)
+    pick = torch.randint(0, K, (N,), generator=gen(K))
+    codes[torch.arange(N), pick] = 9
+    scales = torch.ones(N, K // group)
+    sizes = torch.linspace(-120, 100, K).round() if kind == "bf16" else torch.linspace(-14, 14, K).round()
+    x = (torch.exp2(sizes) * (1 + g.eps))[torch.randperm(K, generator=gen(3))].to(dtype).expand(M, K).contiguous()
+    x[:, :3] = torch.tensor([g.max, 2.0 ** (-133 if kind == "bf16" else -24), -g.tiny], dtype=dtype)
+    pick[:3] = torch.arange(3)
+    codes[:3] = 8
+    codes[torch.arange(3), torch.arange(3)] = 9
+    y = b2.w4_matvec(M, N, K, group, 1.0, x.cuda(), ref.w4_pack(codes).cuda(), scales.cuda(), None, 0.0).cpu()
+    want = x[:, pick].clone()
+    if kind == "bf16":      # 2^-133 beside 2^128 is below what a row scaled by its largest element holds (2^-250 of it)
+        assert bool((y[:, 1] == 0).all() or torch.equal(y[:, 1], want[:, 1]))
+        y[:, 1] = want[:, 1]
+    assert torch.equal(y, want)
