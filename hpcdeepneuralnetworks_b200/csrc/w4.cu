@@ -9,7 +9,7 @@
 namespace b2 {
 
 constexpr int kW4MaxRows = 64;   // rows of x that b2_w4_matvec takes
-constexpr int64_t kW4MaxK = 1 << 27;   // and their length: one block lays a row out, while the product's bounded waits run
+constexpr int64_t kW4MaxK = 1 << 27;   // and their length: units of a row are counted in 32 bits
 
 __device__ __forceinline__ float w4_warp_max(float v) {
 #pragma unroll
@@ -467,8 +467,7 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 //   FP16 x: under 1024's upper bits a code reads 1024 + c, or 1024 + 16 c, and a subtraction or an FMA with 1/16 leaves c - z.
 // Words w and w >> 8 give the pairs of codes (0,4) (1,5) (2,6) (3,7), and a small kernel in front (w4_x_kernel) pairs x alike.  All
 // products are exact in FP32; group sums are FP32, scaled and added in FP32.
-// An infinity or NaN in x counts as 0 above and is added, with its exact
-// weight, by the thread that writes the output, which walks through its whole row for that.
+// An infinity or NaN in x is one in its column of the tile: it meets the exact weights, 0 among them, and stays in its row's outputs.
 //
 // A CTA streams tiles of 128 rows x 256 k (16 KB of codes and x of those k) through a ring of shared-memory stages.  Four
 // producer warps fill it: one thread issues the TMA loads (codes with the 128-byte swizzle: the 16-byte unit u of row r lies at
@@ -484,7 +483,7 @@ constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns o
 constexpr int kMvWindow = 1024;             // scales and zero points held together: 8 groups of each row, the group / 32 chunks
 constexpr int kMvWindows = 2;               // they span
 constexpr int kMvMaxStages = 8, kMvBarrierBytes = 512 + 1024;   // barriers and flags, and room to align
-constexpr int kMvXThreads = 512;
+constexpr int kMvXThreads = 128;
 
 template <int NB, bool RESIDENT, bool ALIGNED>
 struct MvTile {
@@ -524,7 +523,6 @@ struct MvArgs {
   const void *scales;
   void *y;
   const unsigned char *image;      // [item's rows][chunk][kXBytes], unless the CTAs lay x out themselves
-  const int *row_info;             // of each row of x: whether it holds an infinity or NaN
   int *status;
   unsigned int seq;
 };
@@ -547,20 +545,13 @@ __device__ __forceinline__ void mv_load_x(float (&v)[8], const T *row, int64_t k
   }
 }
 
-// Whether one of 8 elements is not finite.
-__device__ __forceinline__ bool mv_look(const float (&e)[8]) {
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= !isfinite(e[i]);
-  return bad;
-}
 // Lays one unit (8 elements, the `u`-th of its chunk) of columns col0.. out in a chunk's image: as FP16, or in `parts` bf16 terms,
-// each the upper half of what the one before has left, and paired.
+// each the upper half of what the one before has left, and paired.  An infinity or NaN is the first term, and nothing is left of it.
 template <bool BF16>
 __device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8], int u, int nb, int col0, int parts) {
   float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = isfinite(e[i]) ? e[i] : 0.f;
+  for (int i = 0; i < 8; ++i) r[i] = e[i];
   for (int p = 0; p < parts; ++p) {
     const int col = col0 + p;
     union {
@@ -571,9 +562,9 @@ __device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8]
     for (int i = 0; i < 8; ++i) {
       const int at = 2 * (i & 3) + (i >> 2);      // pairs (0,4) (1,5) (2,6) (3,7)
       if constexpr (BF16) {
-        const uint32_t top = __float_as_uint(r[i]) & 0xffff0000u;
+        const uint32_t top = isnan(r[i]) ? 0x7fff0000u : __float_as_uint(r[i]) & 0xffff0000u;
         out.h[at] = (uint16_t)(top >> 16);
-        r[i] -= __uint_as_float(top);
+        r[i] = isfinite(r[i]) ? r[i] - __uint_as_float(top) : 0.f;
       } else {
         out.h[at] = __half_as_ushort(__float2half_rn(r[i]));      // (x is FP16)
       }
@@ -582,44 +573,18 @@ __device__ __forceinline__ void mv_put(unsigned char *chunk, const float (&e)[8]
   }
 }
 
-// One block per row of x: whether an element is not finite, then its image.  Four units per thread are kept between the two passes; a
-// longer row is read again.
+// The images of all rows of x: a unit per thread, blockIdx.y the row.
 template <class T>
 __global__ void __launch_bounds__(kMvXThreads) w4_x_kernel(int64_t K, int64_t ldx, int vec, const T *x, int chunks, int nb, int rows_per_item,
-                                                           unsigned char *image, int *row_info) {
-  constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kKept = 4;
+                                                           unsigned char *image) {
+  constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
   pdl_launch_dependents();
-  const int tid = threadIdx.x;
-  const int m = blockIdx.x, item = m / rows_per_item, col0 = (m - item * rows_per_item) * kParts;
-  const T *row = x + m * ldx;
-  const int units = chunks * (kMvChunk / 8);
-  float v[kKept][8];
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) mv_load_x<T>(v[i], row, 8 * (int64_t)(tid + i * kMvXThreads), K, vec != 0);
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) bad |= mv_look(v[i]);
-  for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
-    float e[8];
-    mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
-    bad |= mv_look(e);
-  }
-  bad = __syncthreads_or(bad);
-  if (tid == 0) row_info[m] = bad;
-  const int chunk_bytes = nb * (kMvChunk * 8 * 2);
-  auto put = [&](const float (&e)[8], int u) {
-    mv_put<!std::is_same<T, __half>::value>(image + ((int64_t)item * chunks + (u >> 5)) * chunk_bytes, e, u & 31, nb, col0, kParts);
-  };
-#pragma unroll
-  for (int i = 0; i < kKept; ++i)
-    if (tid + i * kMvXThreads < units) put(v[i], tid + i * kMvXThreads);
-  for (int u = tid + kKept * kMvXThreads; u < units; u += kMvXThreads) {
-    float e[8];
-    mv_load_x<T>(e, row, 8 * (int64_t)u, K, vec != 0);
-    put(e, u);
-  }
+  const int m = blockIdx.y, item = m / rows_per_item, u = blockIdx.x * kMvXThreads + threadIdx.x;
+  if (u >= chunks * (kMvChunk / 8)) return;
+  float e[8];
+  mv_load_x<T>(e, x + m * ldx, 8 * (int64_t)u, K, vec != 0);
+  mv_put<!std::is_same<T, __half>::value>(image + ((int64_t)item * chunks + (u >> 5)) * (nb * kMvChunk * 8 * 2), e, u & 31, nb,
+                                          (m - item * rows_per_item) * kParts, kParts);
 }
 
 // (w & mask) | bits in one instruction (left to itself the compiler makes two of it, having two constants)
@@ -770,19 +735,6 @@ __device__ __forceinline__ float mv_load_any_type(const void *p, int type, int64
   return to_f32(((const __half *)p)[at]);
 }
 
-// What the infinities and NaN of row m of x, elements k0 to k1, add to output n.
-__device__ __noinline__ float mv_not_finite(const MvArgs &a, int m, int64_t n, int64_t k0, int64_t k1) {
-  float v = 0.f;
-  for (int64_t k = k0; k < k1; ++k) {
-    const float e = mv_load_any_type(a.x, a.type, m * a.ldx + k);
-    if (isfinite(e)) continue;
-    const int c = (a.codes[n * a.ldq + (k >> 1)] >> (4 * (k & 1))) & 15;
-    const int64_t g = n * a.groups + (k >> a.group_shift);
-    v += e * (((float)c - w4_zero(a.zeros, g)) * mv_load_any_type(a.scales, a.scale_type, g));
-  }
-  return v;
-}
-
 // ALIGNED: rows of codes start on 16-byte boundaries (TMA); otherwise the producers copy them.
 // RESIDENT: the consumers lay out x of this CTA's k themselves, before the first item; the ring brings codes alone.
 // BLOCKS: blocks of 32 k in a group, or in the 128 of a longer one that a warp multiplies.
@@ -805,7 +757,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
   uint64_t *const full = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sums) + Tile::kSumBytes);
   uint64_t *const empty = full + kMvMaxStages, *const wfull = empty + kMvMaxStages, *const wempty = wfull + kMvWindows;
   uint64_t *const ready = wempty + kMvWindows, *const done = ready + 1;
-  int *const odd = reinterpret_cast<int *>(done + 1);      // RESIDENT: whether a row of x (8 at most) holds an infinity or NaN
   constexpr int kFillers = kMvProducers - 32;     // threads that write shared memory themselves
 
   if (tid == 0) {
@@ -968,8 +919,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
     }
     if constexpr (RESIDENT) {
       // x of this CTA's k, all rows of it (there is one item's worth): a warp takes a chunk of a row, a lane its unit of 8
-      if (tid < 8) odd[tid] = 0;
-      mv_consumers_sync();
       for (int at = warp; at < a.M * chunks; at += kMvConsumers / 32) {
         const int m = at / chunks, c = at - m * chunks;
         const int64_t k = (int64_t)(first + c) * kMvChunk + 8 * lane;
@@ -977,7 +926,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
         if (a.type == B2_F32) mv_load_x(e, (const float *)a.x + m * a.ldx, k, a.K, a.vec != 0);
         else if (a.type == B2_BF16) mv_load_x(e, (const __nv_bfloat16 *)a.x + m * a.ldx, k, a.K, a.vec != 0);
         else mv_load_x(e, (const __half *)a.x + m * a.ldx, k, a.K, a.vec != 0);
-        if (mv_look(e)) atomicOr(&odd[m], 1);
         mv_put<BF16>(xs + c * Tile::kXBytes, e, lane, NB, m * a.parts, a.parts);
       }
       mv_consumers_sync();
@@ -1080,25 +1028,13 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
             for (int h = 0; h < 2; ++h) sums[(wk * 8 * NB + col) * kMvPitch + wn * 32 + rt * 16 + g + h * 8] = total[rt][nb][i + 2 * h];
         }
       mv_consumers_sync();
-      if constexpr (RESIDENT) {
-        bool any = false;
-        for (int m = 0; m < a.M; ++m) any |= odd[m] != 0;
-        if (any && chunks > 0) {
-          const int64_t n0 = (int64_t)item * kMvRows, k0 = (int64_t)first * kMvChunk, k1 = k0 + (int64_t)chunks * kMvChunk;
-          for (int i = tid; i < a.M * kMvRows; i += kMvConsumers) {
-            const int m = i / kMvRows, r = i % kMvRows;
-            if (odd[m] && n0 + r < a.N) sums[m * a.parts * kMvPitch + r] += mv_not_finite(a, m, n0 + r, k0, k1 < a.K ? k1 : a.K);
-          }
-          mv_consumers_sync();
-        }
-      }
       if (ctas > 1) {
         if (tid < ctas) mbar_arrive_cluster(mapa_u32(smem_u32(ready), (uint32_t)tid));
         wait.cluster(ready, turn & 1);
       }
       const int m0 = mc * a.rows_per_item, mm = a.M - m0 < a.rows_per_item ? a.M - m0 : a.rows_per_item;
       const int64_t n0 = (int64_t)(item - mc * a.row_blocks) * kMvRows;
-      if (!RESIDENT && turn == 0) pdl_wait();                       // row_info is w4_x_kernel's
+      if (!RESIDENT && turn == 0) pdl_wait();                       // the outputs come after everything in front of this kernel
       for (int i = tid + rank * kMvConsumers; i < mm * kMvRows; i += kMvConsumers * ctas) {
         const int m = i / kMvRows, r = i % kMvRows;
         if (n0 + r >= a.N) continue;
@@ -1118,7 +1054,6 @@ __global__ void __launch_bounds__(kMvThreads, MvTile<NB, RESIDENT, ALIGNED>::kCt
             v += s;
           }
           if constexpr (BF16) v *= 1.f / kMvUnit;
-          if (!RESIDENT && a.row_info[m0 + m]) v += mv_not_finite(a, m0 + m, n0 + r, 0, a.K);
           v *= a.alpha;
         }
         const int64_t to = (int64_t)(m0 + m) * a.ldy + n0 + r;
@@ -1245,7 +1180,7 @@ static int w4_matvec_run(Context *ctx, const MvArgs &a, int nb, bool resident, b
                    : w4_matvec_forms<4, false>(ctx, a, aligned, s);
 }
 
-// The workspace of a product: the image of x, then row_info.
+// The workspace of a product: the image of x.
 static size_t mv_image_bytes(int64_t M, int64_t K, int type) {
   const int nb = mv_blocks(M, type);
   const int64_t items = (M + mv_rows(nb, type) - 1) / mv_rows(nb, type);
@@ -1371,7 +1306,7 @@ int b2_w4_dequantize(b2_handle h, int64_t N, int64_t K, int group, const uint8_t
 size_t b2_w4_matvec_workspace_bytes(int64_t M, int64_t N, int64_t K, int type) {
   if (M <= 0 || M > kW4MaxRows || N <= 0 || K <= 0 || N > INT32_MAX || K > kW4MaxK || type_bytes(type) == 0) return 0;
   if (mv_resident(M, N, K, type)) return 0;
-  return mv_image_bytes(M, K, type) + (size_t)kW4MaxRows * sizeof(int);
+  return mv_image_bytes(M, K, type);
 }
 
 int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float alpha, int type, const void *x, int64_t ldx,
@@ -1408,14 +1343,13 @@ int b2_w4_matvec(b2_handle h, int64_t M, int64_t N, int64_t K, int group, float 
   a.vec = (((uintptr_t)x | (uintptr_t)(ldx * tb)) & 15) == 0;
   const bool resident = mv_resident(M, N, K, type);
   if (a.chunks > 0 && !resident) {
-    unsigned char *image = (unsigned char *)workspace;
-    int *info = (int *)(image + mv_image_bytes(M, K, type));
-    a.image = image, a.row_info = info;
+    a.image = (unsigned char *)workspace;
     cudaError_t launched = cudaSuccess;
     with_type(type, [&](auto t) {
       using T = decltype(t);
-      launched = launch_kernel(w4_x_kernel<T>, (unsigned)M, kMvXThreads, 0, s, K, ldx, a.vec, (const T *)x, a.chunks, nb, a.rows_per_item,
-                               image, info);
+      const int64_t units = (int64_t)a.chunks * (kMvChunk / 8);
+      launched = launch_kernel(w4_x_kernel<T>, dim3((unsigned)((units + kMvXThreads - 1) / kMvXThreads), (unsigned)M), kMvXThreads, 0, s, K, ldx,
+                               a.vec, (const T *)x, a.chunks, nb, a.rows_per_item, (unsigned char *)workspace);
       return 0;
     });
     B2_CUDA(launched);

@@ -166,3 +166,38 @@ def test_w4_matvec_carries_every_element_of_16_bits_exactly(b2, M, N, K, kind):
         assert bool((y[:, 1] == 0).all() or torch.equal(y[:, 1], want[:, 1]))
         y[:, 1] = want[:, 1]
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("M,N,K,kind", [(64, 50304, 512, "bf16"), (64, 20000, 1000, "f32"), (3, 130, 1 << 20, "f16"), (9, 300, 70000, "f32"),
+                                        (1, 2000, 4096, "bf16"), (2, 5000, 1001, "f16")])
+def test_w4_matvec_whole_rows_that_are_not_finite(b2, M, N, K, kind):
+    """Rows of nothing but NaN, and single infinities at even and odd places, beside finite rows, in long rows and in more row blocks
+    than the device holds at once: no wait runs out, the finite rows keep their bound, an infinity meets its exact weight."""
+    dtype, group = TYPES[kind], 64
+    g = torch.Generator(device="cuda").manual_seed(M + N)
+    codes = torch.randint(0, 256, (N, (K + 1) // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.5 + torch.rand(N, -(-K // group), generator=g, device="cuda")) / 64
+    zeros = torch.randint(0, 16, scales.shape, generator=g, device="cuda", dtype=torch.uint8)
+    x = torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    x[0] = float("nan")
+    if M > 1:
+        x[1, K // 3], x[M - 1, K - 1] = -float("inf"), float("inf")
+        x[1, K // 3 + 1] = -float("inf")
+    y = b2.w4_matvec(M, N, K, group, 1.0, x, codes, scales, zeros, 0.0).double()
+    b2.check_status()
+    want, size = torch.zeros(M, N, dtype=torch.float64, device="cuda"), torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    for at in range(0, K, 1 << 14):         # the definition in 64 bits, in portions of K
+        end = min(K, at + (1 << 14))
+        part = codes[:, at // 2:(end + 1) // 2]
+        w = torch.stack([part & 15, part >> 4], 2).view(N, -1)[:, :end - at].double()
+        groups = torch.arange(at, end, device="cuda") // group
+        w = (w - zeros[:, groups].double()) * scales[:, groups].double()
+        want += x[:, at:end].double() @ w.t()
+        size += x[:, at:end].double().abs() @ w.abs().t()
+    assert bool(y[0].isnan().all())
+    assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf())
+    assert torch.equal(y[y.isinf()], want[want.isinf()])
+    fine = torch.isfinite(want).all(1)
+    assert int(fine.sum()) == max(M - 3, 0)
+    tol = ref.half_step(dtype) * want.abs() + 2 * U * (64 + K / 16) * size + 4 * U * want.abs() + (2.0 ** -25 if kind == "f16" else 0.0)
+    within(y[fine], want[fine].cpu(), tol[fine].cpu(), "the other rows")
