@@ -2,13 +2,15 @@
 
 ``python -m hpcdeepneuralnetworks_b200.build`` compiles every ``csrc/*.cu`` into objects under
 ``csrc/build/`` (skipping files whose object is newer than all sources/headers) and links
-``hpcdeepneuralnetworks_b200/libb2blas.so``, then the C++ driver and the Python extension that shortens the calls of
-``layer.py`` (``csrc/calls.cpp``).  nvcc cross-compiles without a GPU.
+``hpcdeepneuralnetworks_b200/libb2blas.so``, then the C++ driver and, where there is a torch for CUDA, the Python
+extension that shortens the calls of ``layer.py`` (``csrc/calls.cpp``).  nvcc cross-compiles without a GPU.
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -69,7 +71,7 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
               ["-Xlinker", "-rpath,/usr/local/cuda/lib64", "-ldl"]
         run(cmd)
     build_driver()
-    build_calls()
+    build_calls(force)
     return LIB
 
 
@@ -90,21 +92,47 @@ def build_driver() -> str:
 
 CALLS_SRC = os.path.join(CSRC, "calls.cpp")
 CALLS = os.path.join(PKG, "_calls.so")
+CALLS_STAMP = os.path.join(OBJ, "calls.stamp")
 
 
-def build_calls() -> str:
-    """The extension module ``_calls``, against the torch it will run with."""
-    if _stale(CALLS, [CALLS_SRC, os.path.join(PKG, "..", "include", "b2blas.h")]):
+def _torch() -> tuple[str, str] | None:
+    """(folder, version) of the torch that the extension can be built against, found without importing it; None without a torch for
+    CUDA: the library and the driver need none."""
+    spec = importlib.util.find_spec("torch")
+    at = spec.submodule_search_locations[0] if spec and spec.submodule_search_locations else None
+    if at is None or not glob.glob(os.path.join(at, "lib", "libc10_cuda.so*")):
+        return None
+    with open(os.path.join(at, "version.py")) as f:
+        found = re.search(r"__version__\s*=\s*['\"]([^'\"]+)", f.read())
+    return (at, found.group(1)) if found else None
+
+
+def build_calls(force: bool = False) -> str | None:
+    """The extension module ``_calls``, against the torch it will run with: made again when that is another one than last time.
+    Without a torch for CUDA there is none (None is returned), and ``layer.py`` makes every call itself."""
+    found = _torch()
+    if found is None:
+        sys.stderr.write("no torch for CUDA: the extension of layer.py's calls is not built\n")
+        return None
+    at, version = found
+    stamp = f"{version} {sys.implementation.cache_tag} {at}"
+    try:
+        with open(CALLS_STAMP) as f:
+            same = f.read() == stamp
+    except OSError:
+        same = False
+    if force or not same or _stale(CALLS, [CALLS_SRC, os.path.join(PKG, "..", "include", "b2blas.h")]):
         import torch
-        at = os.path.join(os.path.dirname(os.path.abspath(torch.__file__)))
         cuda = os.path.dirname(os.path.dirname(nvcc()))
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(at, "include"),
                "-I" + os.path.join(at, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(cuda, "include"), CALLS_SRC, "-o", CALLS,
-               "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-L" + os.path.join(at, "lib"),
+               f'-DB2_BUILT_FOR_TORCH="{version}"', "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-L" + os.path.join(at, "lib"),
                "-Wl,-rpath," + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("extension build failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
+        with open(CALLS_STAMP, "w") as f:
+            f.write(stamp)
     return CALLS
 
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import importlib
+import warnings
 
 import torch
 
@@ -25,21 +26,29 @@ W4_MAX_ROWS = 64
 
 # csrc/calls.cpp: the usual calls, checked and made without the Python below (which decides all others, with the same results)
 _quick = None
+_looked = False
 
 
 def _load():
-    """The library; the first call hands its functions to ``_calls``."""
-    global _quick
+    """The library; the first call hands its functions to ``_calls``.  Where that is missing, or was built for another torch, whose
+    tensors it would misread, every call goes through the checks below: slower, with the same results."""
+    global _quick, _looked
     L = _lib.load()
-    if _quick is None:
+    if not _looked:
+        _looked = True
         try:
             quick = importlib.import_module(__package__ + "._calls")
-        except ImportError as e:
-            raise ImportError("_calls.so is missing or was built for another torch: run `python -m hpcdeepneuralnetworks_b200.build`") from e
-        names = ("b2_layernorm", "b2_layernorm_backward_workspace_bytes", "b2_layernorm_backward", "b2_w4_quantize", "b2_w4_dequantize",
-                 "b2_w4_matvec_workspace_bytes", "b2_w4_matvec")
-        quick.bind(_default, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
-        _quick = quick
+            why = None if quick.torch_version == torch.__version__ else f"was built for torch {quick.torch_version}, this is {torch.__version__}"
+        except (ImportError, AttributeError) as e:
+            why = f"cannot be used ({e})"
+        if why:
+            warnings.warn(f"_calls.so {why}: calls of the layer operators take some microseconds longer; "
+                          "`python -m hpcdeepneuralnetworks_b200.build` makes it again", RuntimeWarning, stacklevel=3)
+        else:
+            names = ("b2_layernorm", "b2_layernorm_backward_workspace_bytes", "b2_layernorm_backward", "b2_w4_quantize", "b2_w4_dequantize",
+                     "b2_w4_matvec_workspace_bytes", "b2_w4_matvec")
+            quick.bind(_default, *(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names))
+            _quick = quick
     return L
 
 
