@@ -502,8 +502,9 @@ static int mv_blocks(int64_t M, int type) { return M * mv_parts(type) <= 8 ? 1 :
 static int mv_rows(int nb, int type) { return 8 * nb / mv_parts(type); }
 // Whether a product's CTAs lay x out themselves (RESIDENT): each keeps its part of k, cut over clusters of up to 8, in shared
 // memory.  That saves a kernel and a workspace, and costs the same work in every row block's CTAs.
-// (1 token, device time and the host's share of a call: 4096^2, 512 units, 8.4 us and 9 against 7.4 and 14 through w4_x_kernel;
-// 8192^2, 2048 units, 18 against 14 us on the device.)
+// (Device time against that through w4_x_kernel, groups of 128, bf16, K = 4096.  1 token, 64 to 1024 units: 5.0 / 5.8, 5.1 / 6.0, 5.9 /
+// 6.5, 6.5 / 7.4, 768: 9.1 / 9.7, 1024: 10.4 / 10.0 us, 8192^2, 2048 units: 15.2 / 14.4.  8 tokens: 5.9 / 6.8, 5.9 / 6.8, 7.4 / 7.7, 7.7 /
+// 8.3, 768: 10.0 / 10.2, 1024: 11.8 / 10.4, 2048: 18.1 / 15.2.  The host's share of a call: 4.5 / 8 us.)
 constexpr int kMvResidentBytes = 32 * 1024;
 constexpr int64_t kMvResidentWork = 600;       // row blocks x chunks (16 KB of codes each)
 static bool mv_resident(int64_t M, int64_t N, int64_t K, int type) {
