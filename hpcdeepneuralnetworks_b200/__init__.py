@@ -10,14 +10,22 @@ device memory, streams and ``torch.distributed``.
 from ._lib import B2Error, Fault, FtReport, LIB_PATH  # noqa: F401
 
 
+_module_of = {}     # operators that have been asked for: the module of each
+
+
 def __getattr__(name):
     # Operators are resolved lazily so that importing the package (and building the library)
     # works on a machine without a GPU; using an operator without the built library raises.
+    # The name is looked up in its module each time: what is replaced there is seen here.
+    m = _module_of.get(name)
+    if m is not None:
+        return getattr(m, name)
     import importlib
     if name in ("blas", "build", "dist", "gen_ft_sgemm", "layer", "_lib"):
         return importlib.import_module(f"{__name__}.{name}")
     for module in ("blas", "layer"):
         m = importlib.import_module(f"{__name__}.{module}")
         if hasattr(m, name):
-            return globals().setdefault(name, getattr(m, name))
+            _module_of[name] = m
+            return getattr(m, name)
     raise AttributeError(name)

@@ -84,3 +84,16 @@ def test_calls_go_through_the_checks_without_it(built_lib, monkeypatch, module):
 def test_the_extension_that_was_built_is_taken(built_lib):
     layer._load()
     assert layer._quick is not None and layer._quick.torch_version == torch.__version__
+
+
+def test_an_operator_replaced_in_its_module_is_seen_in_the_package(built_lib, monkeypatch):
+    import hpcdeepneuralnetworks_b200 as b2
+    for module, name in ((b2.blas, "sgemm"), (layer, "layernorm")):
+        real = getattr(b2, name)
+        assert real is getattr(module, name)
+        with monkeypatch.context() as m:
+            m.setattr(module, name, lambda *a: "replaced")
+            assert getattr(b2, name)() == "replaced"
+        assert getattr(b2, name) is real
+    with pytest.raises(AttributeError):
+        b2.no_such_operator
