@@ -10,22 +10,37 @@ device memory, streams and ``torch.distributed``.
 from ._lib import B2Error, Fault, FtReport, LIB_PATH  # noqa: F401
 
 
-_module_of = {}     # operators that have been asked for: the module of each
+import sys as _sys
+import types as _types
+
+
+class _Live:
+    """An operator of this package that has been asked for: looked up in its module each time, so that what is replaced there is seen
+    here (0.1 us an access; through ``__getattr__`` each time 0.5)."""
+
+    def __init__(self, module, name):
+        self.module, self.name = module, name
+
+    def __get__(self, package, kind):
+        return getattr(self.module, self.name)
+
+
+class _Package(_types.ModuleType):
+    pass
+
+
+_sys.modules[__name__].__class__ = _Package
 
 
 def __getattr__(name):
     # Operators are resolved lazily so that importing the package (and building the library)
     # works on a machine without a GPU; using an operator without the built library raises.
-    # The name is looked up in its module each time: what is replaced there is seen here.
-    m = _module_of.get(name)
-    if m is not None:
-        return getattr(m, name)
     import importlib
     if name in ("blas", "build", "dist", "gen_ft_sgemm", "layer", "_lib"):
         return importlib.import_module(f"{__name__}.{name}")
     for module in ("blas", "layer"):
         m = importlib.import_module(f"{__name__}.{module}")
         if hasattr(m, name):
-            _module_of[name] = m
+            setattr(_Package, name, _Live(m, name))
             return getattr(m, name)
     raise AttributeError(name)

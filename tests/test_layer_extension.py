@@ -95,5 +95,9 @@ def test_an_operator_replaced_in_its_module_is_seen_in_the_package(built_lib, mo
             m.setattr(module, name, lambda *a: "replaced")
             assert getattr(b2, name)() == "replaced"
         assert getattr(b2, name) is real
+        with monkeypatch.context() as m:          # or in the package itself, there alone
+            m.setattr(b2, name, lambda *a: "here")
+            assert getattr(b2, name)() == "here" and getattr(module, name) is real
+        assert getattr(b2, name) is real
     with pytest.raises(AttributeError):
         b2.no_such_operator
