@@ -201,3 +201,64 @@ def test_w4_matvec_whole_rows_that_are_not_finite(b2, M, N, K, kind):
     assert int(fine.sum()) == max(M - 3, 0)
     tol = ref.half_step(dtype) * want.abs() + 2 * U * (64 + K / 16) * size + 4 * U * want.abs() + (2.0 ** -25 if kind == "f16" else 0.0)
     within(y[fine], want[fine].cpu(), tol[fine].cpu(), "the other rows")
+
+
+def product_on_device(x, codes, scales, zeros, group):
+    """(x W^T, |x| |W|^T) in 64 bits on the device, in portions of rows."""
+    N, K = codes.shape[0], x.shape[1]
+    at = torch.arange(K, device="cuda") // group
+    want, size = torch.empty(x.shape[0], N, dtype=torch.float64, device="cuda"), torch.empty(x.shape[0], N, dtype=torch.float64, device="cuda")
+    for n in range(0, N, 2048):
+        part = codes[n:n + 2048]
+        w = torch.stack([part & 15, part >> 4], 2).view(part.shape[0], -1)[:, :K].double()
+        w = (w - (8.0 if zeros is None else zeros[n:n + 2048][:, at].double())) * scales[n:n + 2048][:, at].double()
+        want[:, n:n + 2048], size[:, n:n + 2048] = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    return want, size
+
+
+@pytest.mark.parametrize("M,N,K,kind", [(1, 50304, 4096, "bf16"), (16, 50304, 1024, "f16"), (64, 8192, 2048, "f32"), (33, 40000, 768, "bf16"),
+                                        (1, 50304, 256, "bf16"), (1, 19200, 1024, "f16"), (8, 50300, 255, "bf16"), (2, 75000, 130, "f32"),
+                                        (5, 19111, 1023, "bf16")])
+@pytest.mark.parametrize("group,with_zeros", [(64, True), (256, False)])
+def test_w4_matvec_of_more_row_blocks_than_the_device_holds(b2, M, N, K, kind, group, with_zeros):
+    """Each CTA, or cluster of CTAs, takes several row blocks one behind the other: a vocabulary head, FP32 rows in several items, small
+    products that lay x out themselves (one CTA to a row block and two), rows of codes that start anywhere; twice, for equal bits."""
+    dtype = TYPES[kind]
+    g = torch.Generator(device="cuda").manual_seed(N + K)
+    codes = torch.randint(0, 256, (N, (K + 1) // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.5 + torch.rand(N, -(-K // group), generator=g, device="cuda")) / 64
+    zeros = torch.randint(0, 16, scales.shape, generator=g, device="cuda", dtype=torch.uint8) if with_zeros else None
+    x = torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    y = torch.full((M, N), float("nan"), dtype=dtype, device="cuda")
+    b2.w4_matvec(M, N, K, group, 1.0, x, codes, scales, zeros, 0.0, y)
+    want, size = product_on_device(x, codes, scales, zeros, group)
+    tol = ref.half_step(dtype) * want.abs() + 2 * U * (64 + K / 16) * size + 4 * U * want.abs() + (2.0 ** -25 if kind == "f16" else 0.0)
+    within(y, want.cpu(), tol.cpu(), "y")
+    assert torch.equal(y, b2.w4_matvec(M, N, K, group, 1.0, x, codes, scales, zeros, 0.0))
+    b2.check_status()
+
+
+@pytest.mark.parametrize("N,K", [(3, 2), (5, 33), (33, 254), (130, 1000), (17, 2050), (257, 515), (9, 8206), (40, 4096)])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("group,with_zeros", [(32, True), (128, False), (256, True)])
+@pytest.mark.parametrize("pad,packed", [(0, True), (1, True), (2, False), (7, True), (8, True)])
+def test_w4_quantize_packed_codes_and_pitched_weights(b2, N, K, kind, group, with_zeros, pad, packed):
+    """Rows of codes directly behind one another (starting at any byte), rows of W `pad` elements apart from one that starts off the
+    16-byte boundaries: the definition bit for bit, and nothing beside the rows is read into them or written."""
+    dtype = TYPES[kind]
+    W = (torch.randn(N, K, generator=gen(N + K)) * 0.1).to(dtype)
+    base = torch.full((N * (K + pad) + pad + 8,), float("nan"), dtype=dtype, device="cuda")
+    at = base[pad:pad + N * (K + pad)].view(N, K + pad)[:, :K]
+    at.copy_(W.cuda())
+    width = (K + 1) // 2
+    want, ws, wz = ref.w4_quantize(W, group, torch.float32, with_zeros)
+    room = torch.full((N * width + 64,), 0x77, dtype=torch.uint8, device="cuda")
+    codes = room[32:32 + N * width].view(N, width) if packed else b2.w4_empty(N, K, group)[0]
+    s = torch.empty(N, -(-K // group), device="cuda")
+    z = torch.empty(s.shape, dtype=torch.uint8, device="cuda") if with_zeros else None
+    b2.w4_quantize(N, K, group, at, codes, s, z)
+    assert torch.equal(codes.cpu(), ref.w4_pack(want)) and torch.equal(s.cpu(), ws)
+    assert z is None or torch.equal(z.cpu().long(), wz)
+    assert bool((room[:32] == 0x77).all()) and bool((room[32 + N * width:] == 0x77).all())
+    back = b2.w4_dequantize(N, K, group, codes, s, z, dtype=dtype)
+    assert torch.equal(back.cpu(), ref.w4_values(want, ws, wz if with_zeros else None, group).float().to(dtype))
