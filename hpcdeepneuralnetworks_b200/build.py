@@ -109,10 +109,10 @@ def _torch() -> tuple[str, str] | None:
 
 def build_calls(force: bool = False) -> str | None:
     """The extension module ``_calls``, against the torch it will run with: made again when that is another one than last time.
-    Without a torch for CUDA there is none (None is returned), and ``layer.py`` makes every call itself."""
+    Without a torch for CUDA, or without Python's headers, there is none (None is returned), and ``layer.py`` makes every call itself."""
     found = _torch()
-    if found is None:
-        sys.stderr.write("no torch for CUDA: the extension of layer.py's calls is not built\n")
+    if found is None or not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        sys.stderr.write("no torch for CUDA, or no Python.h: the extension of layer.py's calls is not built\n")
         return None
     at, version = found
     stamp = f"{version} {sys.implementation.cache_tag} {at}"

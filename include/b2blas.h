@@ -219,7 +219,8 @@ enum { B2_F32 = 0, B2_BF16 = 1, B2_F16 = 2 };
  * `type`); NULL gamma means 1, NULL beta means 0.  mean, rstd: `rows` floats for the backward pass, or NULL.
  * eps >= 0.  rows = 0 is a no-op; cols must be at least 1.  y may be x itself (ldy = ldx); any other overlap of y with x is
  * refused.  A row that holds an infinity or a NaN gives NaN in its own outputs and nowhere else.  Squares are FP32: a row with
- * elements farther than 2^63 from its mean (a mask's -1e38 beside others) has rstd 0 and gives beta; values up to 2^126 never give NaN. */
+ * elements farther than 2^63 from its mean (a mask's -1e38 beside others) has rstd 0 and gives beta; values up to 2^126 never give NaN
+ * with eps > 0.  A row that varies by less than about a hundredth of its mean's last FP32 digit has variance 0. */
 int b2_layernorm(b2_handle h, int64_t rows, int64_t cols, float eps, int type, const void *x, int64_t ldx, int param_type,
                  const void *gamma, const void *beta, void *y, int64_t ldy, float *mean, float *rstd, void *stream);
 

@@ -54,11 +54,15 @@ def test_forced_builds_reach_the_extension(built_lib, monkeypatch):
     assert seen == [False, True]
 
 
-@pytest.mark.parametrize("what", ["no torch", "a torch without CUDA"])
+@pytest.mark.parametrize("what", ["no torch", "a torch without CUDA", "no Python.h"])
 def test_the_library_is_built_without_a_torch_for_cuda(compiler, monkeypatch, tmp_path, what):
-    spec = None if what == "no torch" else types.SimpleNamespace(submodule_search_locations=[str(tmp_path)])
-    monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: spec)
-    assert build._torch() is None and build.build_calls() is None and build.build_calls(force=True) is None
+    if what == "no Python.h":
+        monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    else:
+        spec = None if what == "no torch" else types.SimpleNamespace(submodule_search_locations=[str(tmp_path)])
+        monkeypatch.setattr(build.importlib.util, "find_spec", lambda name: spec)
+        assert build._torch() is None
+    assert build.build_calls() is None and build.build_calls(force=True) is None
     assert not compiler
 
 
