@@ -715,9 +715,9 @@ __global__ void __launch_bounds__(512, 1) layernorm_backward_kernel(int64_t rows
 // times what one reading would take (158 us with 1024 threads to a row and a line of sums for every 28 rows).  Going over the rows
 // by panels that fit L2, both kernels for each, was slower: 191 us for panels of 48 MB, 164 for 80 MB; the kernels' ends cost more
 // than the second reading.
-// dx alone needs no second kernel and no place for the sums: the block that has a row's sums reads the row again (from L2).
+// dx alone needs no second kernel and no place for the sums: the block that has a row's sums reads the row again, from L2 (DX).
 constexpr int kLnSumThreads = 512;
-template <class T, class P, int V>
+template <class T, class P, int V, bool DX>
 __global__ void __launch_bounds__(kLnSumThreads) layernorm_row_sums_kernel(int64_t rows, int cols, const T *dy, int64_t lddy, const T *x, int64_t ldx,
                                                                   const P *gamma, const float *mean, const float *rstd, float2 *out, T *dx,
                                                                   int64_t lddx) {
@@ -744,23 +744,23 @@ __global__ void __launch_bounds__(kLnSumThreads) layernorm_row_sums_kernel(int64
       }
     }
     const float2 s = ln_sum2(make_float2(s1.sum(), s2.sum()), scratch[turn], t);
-    const float2 by_n = make_float2(s.x / (float)cols, s.y / (float)cols);
-    if (!dx) {
-      if (threadIdx.x == 0) out[row] = by_n;
-      continue;
-    }
-    for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += kLnSumThreads * V) {      // (dx may be dy: each thread reads its own again)
-      LnPack<T, V> xv, gv;
-      F g[K];
-      xv.load(x + row * ldx + i);
-      gv.load(dy + row * lddy + i);
-      ln_params<P, V>(g, gamma, (int)i, 1.f);
+    if constexpr (DX) {
+      const float2 by_n = make_float2(s.x / (float)cols, s.y / (float)cols);
+      for (int64_t i = (int64_t)threadIdx.x * V; i < cols; i += kLnSumThreads * V) {      // (dx may be dy: each thread reads its own again)
+        LnPack<T, V> xv, gv;
+        F g[K];
+        xv.load(x + row * ldx + i);
+        gv.load(dy + row * lddy + i);
+        ln_params<P, V>(g, gamma, (int)i, 1.f);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const F h = (xv.get(k) + F(-m)) * F(r);
-        xv.set(k, F(r) * (gv.get(k) * g[k] + ln_fma(h, F(-by_n.y), F(-by_n.x))));
+        for (int k = 0; k < K; ++k) {
+          const F h = (xv.get(k) + F(-m)) * F(r);
+          xv.set(k, F(r) * (gv.get(k) * g[k] + ln_fma(h, F(-by_n.y), F(-by_n.x))));
+        }
+        xv.store(dx + row * lddx + i);
       }
-      xv.store(dx + row * lddx + i);
+    } else if (threadIdx.x == 0) {
+      out[row] = make_float2(s.x / (float)cols, s.y / (float)cols);
     }
   }
 }
@@ -1106,8 +1106,8 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
         else run(std::integral_constant<int, kLnHeldBackward>(), std::false_type());
       } else {
         if (dx)
-          launched = launch_kernel(layernorm_row_sums_kernel<T, P, V>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows,
-                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, sums ? (T *)nullptr : (T *)dx, lddx);
+          launched = launch_kernel(sums ? layernorm_row_sums_kernel<T, P, V, false> : layernorm_row_sums_kernel<T, P, V, true>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows,
+                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx);
         if (sums && launched == cudaSuccess)
           launched = launch_kernel(layernorm_columns_kernel<T, P, V>, dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s, rows,
                                    (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
