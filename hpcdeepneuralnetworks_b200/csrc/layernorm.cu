@@ -5,9 +5,9 @@
 // the widest access that every row pointer, the pitches and cols allow (16 bytes, 4 bytes, one element); rows that fit none but
 // are off by the same amount in all matrices are taken in 16 bytes with their ends masked (PHASED).  Longer rows are read again
 // instead of held.
-// Measured, device time: forward 16384 x 4096 bf16 47.7 us (5.6 TB/s of the 268 MB it must move, 0.87 of a copy), 8192 x 4095
-// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 72 us (5.6 TB/s, 0.87), 8192 x 4095 63 us, 5003 x 1027 FP32
-// 20.4 us, 64 x 4096 6.6 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
+// Measured, device time: forward 16384 x 4096 bf16 48.2 us (5.6 TB/s of the 268 MB it must move, 0.86 of a copy), 8192 x 4095
+// 43 us; 8 x 4096 2.7 us, a launch's latency.  Backward 16384 x 4096 68.4 us (5.9 TB/s, 0.91), 8192 x 4095 64 us, 5003 x 1027 FP32
+// 20.5 us, 64 x 4096 6.6 us.  Both run at memory speed where rows are whole accesses and there are waves of them; what holds the others back is the
 // latency of a row's two sums, with 10 to 16 warps to an SM.
 #include <math.h>
 
@@ -1096,7 +1096,7 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
           if (phased) {
             // 16 bytes against the widest access that fits, when this was chosen: 8192 x 4095 bf16 257 -> 73 us, 16384 x 2050 84 -> 63 (8
             // elements per thread: 93), 5003 x 1027 FP32 23.4 -> 21.9 (16 elements: 30.5), 40000 x 517 FP32 64 -> 59 (16: 108), 40000 x 131
-            // FP16 47 -> 26.5 (16: 31); by now 63, 52, 20.4, 59 and 21
+            // FP16 47 -> 26.5 (16: 31); by now 64, 52, 20.5, 58 and 21
             if (cols + V <= (V == 4 ? 512 : 32) * 8) run(std::integral_constant<int, 8>(), std::true_type());
             else run(std::integral_constant<int, kLnHeldBackward>(), std::true_type());
             return;

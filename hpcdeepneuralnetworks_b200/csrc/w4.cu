@@ -475,8 +475,9 @@ __global__ void __launch_bounds__(256) w4_transpose_kernel(int64_t N, int64_t K,
 // each row at a time.  Eight consumer warps, 4 (rows) x 2 (k), multiply 32 rows x 128 k each.  Where there are fewer row blocks
 // than CTAs, the k range is cut over the CTAs of a cluster, whose sums meet over distributed shared memory in the order of the
 // ranks: no atomics.
-// Measured on the device: 1 x 4096^2 bf16 8.4 us and 1 x 8192^2 13.9, latency; 16 x 32768 x 8192 45 us = 3.1 TB/s (30 us with
-// the loads alone, 43 with the codes in L2: unpacking and the waits around it decide); 3 x 6144^2 FP32 16.5 us.
+// Measured on the device: 1 x 4096^2 bf16 6.4 us and 1 x 8192^2 14.7, latency; 16 x 32768 x 8192 49 us = 2.9 TB/s (the loads alone
+// take 30: unpacking and the waits around it decide; with the zero point taken off the sums instead, four instructions less per
+// word, 45); 3 x 6144^2 FP32 15.2 us; 64 x 16384 x 4096 45 us, of which each of the two items of a row block unpacks the codes anew.
 constexpr int kMvConsumers = 256, kMvProducers = 128, kMvThreads = kMvConsumers + kMvProducers;
 constexpr int kMvRows = 128, kMvChunk = 256, kMvRowBytes = kMvChunk / 2;
 constexpr int kMvPitch = kMvRows + 4;       // of the sums: 8 rows x 4 columns of a warp's store in 32 banks
