@@ -1106,8 +1106,9 @@ int b2_layernorm_backward(b2_handle h, int64_t rows, int64_t cols, int type, con
         else run(std::integral_constant<int, kLnHeldBackward>(), std::false_type());
       } else {
         if (dx)
-          launched = launch_kernel(sums ? layernorm_row_sums_kernel<T, P, V, false> : layernorm_row_sums_kernel<T, P, V, true>, (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows,
-                                   (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx);
+          launched = launch_kernel(sums ? layernorm_row_sums_kernel<T, P, V, false> : layernorm_row_sums_kernel<T, P, V, true>,
+                                   (unsigned)(rows < 1 << 30 ? rows : 1 << 30), kLnSumThreads, 0, s, rows, (int)cols, (const T *)dy, lddy,
+                                   (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx);
         if (sums && launched == cudaSuccess)
           launched = launch_kernel(layernorm_columns_kernel<T, P, V>, dim3((unsigned)((cols / V + 127) / 128), (unsigned)parts), 128, 0, s, rows,
                                    (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)gamma, mean, rstd, row_sums, (T *)dx, lddx, partial);
